@@ -475,6 +475,118 @@ int yl_sampler_result(yl_sampler* s, uint32_t* id_out);
  * last token's logits; single-GPU models). */
 int yl_session_logits(const yl_session* s, float** logits);
 
+/* ---- serving: paged cache, shared prefixes, token probabilities ----------
+ *
+ * No counterpart in the reference, which keeps one contiguous f32 cache per
+ * session: these are additions of this library for callers that serve many
+ * sequences from one cache. All three enqueue on `stream`, allocate nothing,
+ * keep no state between calls and may be captured into a graph. */
+
+/* Element type of a paged cache, of its queries, and of logits. */
+enum yl_dtype { YL_DT_F32 = 0, YL_DT_F16 = 1, YL_DT_BF16 = 2 };
+
+/* One layer's paged key/value cache. Element d of head h of the token at
+ * offset t of page p lies at p*page_stride + t*token_stride + h*head_stride + d
+ * of k and of v (strides in elements, the same for both; any order of the
+ * three axes, so several layers may share one allocation). k and v and every
+ * stride are multiples of 16 bytes. page_size: a power of two, 8..256;
+ * head_size: 64 or 128. Filled in by the caller, or by yl_kv_pages_alloc
+ * (zeroed, [n_pages][page_size][n_kv_heads][head_size]). */
+typedef struct yl_kv_pages {
+  int32_t dtype; /* yl_dtype */
+  int32_t owned; /* 1 if freed by yl_kv_pages_free */
+  uint32_t n_pages, page_size, n_kv_heads, head_size;
+  uint64_t page_stride, token_stride, head_stride;
+  void* k;
+  void* v;
+} yl_kv_pages;
+int yl_kv_pages_alloc(int dtype, uint32_t n_pages, uint32_t page_size, uint32_t n_kv_heads, uint32_t head_size,
+                      yl_kv_pages* out);
+int yl_kv_pages_free(yl_kv_pages* p);
+
+/* The sequences of one call. Row arrays (qkv, q, output) hold n_rows rows;
+ * rows row_start[i] .. row_start[i+1]-1 are the newest tokens of sequence i
+ * (one per sequence when decoding, a chunk of the prompt when prefilling, none
+ * for an idle slot) and seq_len[i] is its token count with them, so that its
+ * last row is at position seq_len[i] - 1. Rows behind row_start[n_seqs] are
+ * padding: they are neither read nor written. Position p of sequence i lies
+ * at offset p % page_size of page page_table[i*table_stride + p/page_size];
+ * table entries behind the sequence's last position are not used.
+ * shared_len (a multiple of page_size): every sequence holds the same pages as
+ * the first sequence's table row for its first shared_len positions, as far as
+ * it is that long (the first row's entries for them are valid even if its slot
+ * is idle). Attention then reads those pages once for all sequences. With 0
+ * every sequence's pages are read for itself; the results agree to rounding.
+ * The arrays are on the device (one call's geometry may be computed there, and
+ * a captured graph replays with new contents), so they are checked there: a
+ * page id >= n_pages, or a position without a table slot, or beyond the rope
+ * table, is neither read (keys and values there count as zeros) nor written,
+ * and YL_ERR_RANGE is stored to *status (nullable; never cleared here).
+ * row_start values are limited to n_rows and to ascending order. */
+typedef struct yl_seq_batch {
+  uint32_t n_seqs, n_rows, table_stride, shared_len;
+  const uint32_t* row_start;  /* [n_seqs + 1] */
+  const uint32_t* seq_len;    /* [n_seqs] */
+  const uint32_t* page_table; /* [n_seqs][table_stride] */
+  int32_t* status;
+} yl_seq_batch;
+
+/* Rotates the new rows' queries and keys by their positions and writes keys
+ * and values to their page slots (forward.rs:154-175 for a paged cache). qkv:
+ * f32 rows [q (n_heads*hd) | k (n_kv_heads*hd) | v] as the fused projection
+ * leaves them, qkv_stride floats apart. rope_cs: f32 (cos, sin) table
+ * [rope_len][head_size/2][2] (yl_model_rope, or the caller's own), pairs as
+ * rope_mode says (yl_rope_mode); NULL: no rotation. q_out: rotated queries in
+ * the cache's type, rows q_stride elements apart; NULL: keys and values only
+ * (a row then still holds n_heads query heads, which are skipped). Products
+ * and sums in f32, one rounding to the cache's type. Two rows of one call
+ * must not have the same slot. */
+int yl_paged_append(void* q_out, uint64_t q_stride, const float* qkv, uint64_t qkv_stride, const yl_kv_pages* pages,
+                    const yl_seq_batch* batch, uint32_t n_heads, const float* rope_cs, uint32_t rope_len,
+                    int rope_mode, void* stream);
+
+/* Causal grouped-query attention of the batch's rows over the paged cache:
+ * a row at position p attends to positions 0..p of its sequence. q, output:
+ * rows of n_heads*head_size elements, q_stride / out_stride elements apart; q
+ * in the cache's type, output in the cache's type or f32 (out_dtype). lse
+ * (nullable): f32 [n_rows][n_heads], log of the sum of exp(scores). A row that
+ * sees no key (seq_len 0, or more rows than tokens) gives zeros and -inf.
+ * n_heads / n_kv_heads: a whole number, at most 16. Scores, softmax and sums
+ * in f32; products of an f32 cache as three tf32 products (about 2^-21
+ * relative); for a 16-bit cache the softmax weights are rounded to its type.
+ * Contents of the cache behind a sequence's last position do not matter,
+ * infinities and NaN included. The summation order depends on the batch's
+ * geometry alone: the same call gives the same bits.
+ * workspace: device memory of at least the bytes yl_paged_attention_workspace
+ * gives for a batch of these counts (n_seqs, n_rows, shared_len) and heads,
+ * 256-byte aligned, with any contents; not to be shared by calls that may
+ * overlap on the GPU. */
+int yl_paged_attention(void* output, uint64_t out_stride, int out_dtype, float* lse, const void* q, uint64_t q_stride,
+                       const yl_kv_pages* pages, const yl_seq_batch* batch, uint32_t n_heads, float attn_scale,
+                       void* workspace, uint64_t workspace_bytes, void* stream);
+int yl_paged_attention_workspace(const yl_kv_pages* pages, const yl_seq_batch* batch, uint32_t n_heads,
+                                 uint64_t* bytes);
+
+/* Log probabilities under softmax(logits row), without writing the
+ * probabilities: per row the given token's (tokens and logprobs, nullable
+ * together), the entropy in nats (nullable), and the top_k (0..32) most likely
+ * tokens with their log probabilities, most likely first, the lower id first
+ * among equals (top_ids, top_logprobs: [n_rows][top_k]; needed if top_k > 0).
+ * logits: device rows of `vocab` values (yl_dtype), row_stride elements apart
+ * (yl_session_logits, yl_batch_logits). Values of -inf have probability 0. A
+ * token outside the vocabulary gives NaN; a row that holds NaN or +inf, or
+ * nothing but -inf, gives NaN throughout and ids -1. Sums in f32, with the
+ * largest term kept apart, so that log probabilities near 0 keep their
+ * digits. */
+int yl_token_logprobs(const void* logits, int dtype, uint64_t row_stride, uint32_t n_rows, uint32_t vocab,
+                      const int32_t* tokens, float* logprobs, float* entropy, uint32_t top_k, int32_t* top_ids,
+                      float* top_logprobs, void* stream);
+/* Device views that the calls above take: the model's (cos, sin) table
+ * [*len][head_size/2][2] in the order of its rope_mode, and the batch's logits
+ * [max_sessions][vocab] after yl_batch_forward. */
+int yl_model_rope(const yl_model* m, const float** rope_cs, uint32_t* len);
+int yl_batch_logits(const yl_batch* b, float** logits);
+
 /* ---- synthetic model files (test and bench inputs) ----------------------- */
 typedef struct yl_synth_config {
   uint32_t dim, hidden_dim, n_layers, n_heads, n_kv_heads, vocab_size, context_length;

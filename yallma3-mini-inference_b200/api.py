@@ -69,6 +69,17 @@ class SynthC(C.Structure):
         ("seed", C.c_uint64), ("weight_std", C.c_float), ("threads", C.c_int32)]
 
 
+class KvPagesC(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("owned", C.c_int32), ("n_pages", C.c_uint32), ("page_size", C.c_uint32),
+                ("n_kv_heads", C.c_uint32), ("head_size", C.c_uint32), ("page_stride", C.c_uint64),
+                ("token_stride", C.c_uint64), ("head_stride", C.c_uint64), ("k", C.c_void_p), ("v", C.c_void_p)]
+
+
+class SeqBatchC(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("n_seqs", "n_rows", "table_stride", "shared_len")] + [
+        (n, C.c_void_p) for n in ("row_start", "seq_len", "page_table", "status")]
+
+
 _P = C.c_void_p
 _sigs = {
     "yl_last_error": (C.c_char_p, []),
@@ -145,6 +156,18 @@ _sigs = {
     "yl_sampler_sample": (C.c_int, [_P, _P, _P, _P]),
     "yl_sampler_result": (C.c_int, [_P, C.POINTER(C.c_uint32)]),
     "yl_session_logits": (C.c_int, [_P, C.POINTER(_P)]),
+    "yl_kv_pages_alloc": (C.c_int, [C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(KvPagesC)]),
+    "yl_kv_pages_free": (C.c_int, [C.POINTER(KvPagesC)]),
+    "yl_paged_append": (C.c_int, [_P, C.c_uint64, _P, C.c_uint64, C.POINTER(KvPagesC), C.POINTER(SeqBatchC), C.c_uint32,
+                                  _P, C.c_uint32, C.c_int, _P]),
+    "yl_paged_attention": (C.c_int, [_P, C.c_uint64, C.c_int, _P, _P, C.c_uint64, C.POINTER(KvPagesC),
+                                     C.POINTER(SeqBatchC), C.c_uint32, C.c_float, _P, C.c_uint64, _P]),
+    "yl_paged_attention_workspace": (C.c_int, [C.POINTER(KvPagesC), C.POINTER(SeqBatchC), C.c_uint32,
+                                               C.POINTER(C.c_uint64)]),
+    "yl_token_logprobs": (C.c_int, [_P, C.c_int, C.c_uint64, C.c_uint32, C.c_uint32, _P, _P, _P, C.c_uint32, _P, _P,
+                                    _P]),
+    "yl_model_rope": (C.c_int, [_P, C.POINTER(_P), C.POINTER(C.c_uint32)]),
+    "yl_batch_logits": (C.c_int, [_P, C.POINTER(_P)]),
     "yl_synth_write_gguf": (C.c_int, [C.c_char_p, C.POINTER(SynthC)]),
 }
 for _name, (_res, _args) in _sigs.items():
@@ -323,6 +346,180 @@ def fused_attention(output, sq, key_cache, value_cache, seq_len: int, batch: int
                                    n_heads, n_kv_heads, head_size, start_pos, kv_dim, attn_scale, _stream(stream)))
 
 
+# ------------------------------------------------------- serving ---
+
+class DType(enum.IntEnum):
+    """Element types of paged caches, queries and logits (yl_dtype)."""
+    F32 = 0
+    F16 = 1
+    BF16 = 2
+
+
+ROPE_GGUF, ROPE_LLAMA3 = 0, 1
+
+
+def _dtype(t) -> int:
+    """yl_dtype of a torch tensor."""
+    d = _DTYPES.get(str(t.dtype))
+    if d is None:
+        raise TypeError(f"no yl_dtype for {t.dtype}")
+    return d
+
+
+_DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+
+
+def _expect(t, what: str, dtype: str, numel: int):
+    """`t`, checked to be a contiguous tensor of the current device that holds numel values (raw addresses pass)."""
+    if t is None or isinstance(t, int):
+        return t
+    if str(t.dtype) not in dtype:
+        raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
+    if not t.is_contiguous() or t.numel() < numel:
+        raise ValueError(f"{what} must be contiguous and hold {numel} values, got shape {tuple(t.shape)}")
+    return _here(t, what)
+
+
+def _here(t, what: str):
+    import torch
+    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{what} must be on the current CUDA device")
+    return t
+
+
+def _row_stride(t, what: str, width: int, n_rows: int) -> int:
+    """Elements between rows of a tensor of at least n_rows rows ([rows, width], or [rows, heads, head_size])."""
+    inner = t[0].numel() if t.dim() > 1 and t.shape[0] else 0
+    if t.dim() < 2 or inner != width or t.shape[0] < n_rows or (n_rows and not t[0].is_contiguous()):
+        raise ValueError(f"{what} must hold {n_rows} rows of {width} consecutive values, got shape {tuple(t.shape)}")
+    return t.stride(0) if t.shape[0] > 1 else width
+
+
+class KvPages:
+    """One layer's paged key/value cache (yl_kv_pages): allocated by the library, or a view of torch tensors."""
+
+    def __init__(self, c: KvPagesC, keep=None):
+        self.c = c
+        self._keep = keep
+
+    @classmethod
+    def alloc(cls, dtype: DType, n_pages: int, page_size: int, n_kv_heads: int, head_size: int) -> "KvPages":
+        c = KvPagesC()
+        _check(_lib.yl_kv_pages_alloc(int(dtype), n_pages, page_size, n_kv_heads, head_size, C.byref(c)))
+        return cls(c)
+
+    @classmethod
+    def of(cls, k, v) -> "KvPages":
+        """View of two tensors [n_pages, page_size, n_kv_heads, head_size] of the same type and strides (last axis
+        consecutive; transposed and sliced tensors are fine)."""
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.stride(3) != 1:
+            raise ValueError("k and v must be [n_pages, page_size, n_kv_heads, head_size], alike, last axis consecutive")
+        _here(k, "k")
+        _here(v, "v")
+        n, ps, h, hd = k.shape
+        sp, st, sh, _ = (max(x, hd) for x in k.stride())
+        return cls(KvPagesC(_dtype(k), 0, n, ps, h, hd, sp, st, sh, k.data_ptr(), v.data_ptr()), (k, v))
+
+    def free(self) -> None:
+        if self.c.owned and self.c.k:
+            _lib.yl_kv_pages_free(C.byref(self.c))
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class SeqBatch:
+    """The sequences of one call (yl_seq_batch). Device int32 tensors: row_start [n_seqs + 1], seq_len [n_seqs],
+    page_table [n_seqs, slots]; status: one int32, set to -6 (YL_ERR_RANGE) for a bad page or position."""
+
+    def __init__(self, row_start, seq_len, page_table, n_rows: int, shared_len: int = 0, status=None):
+        n = seq_len.numel()
+        ints = ("torch.int32", "torch.uint32")
+        _expect(row_start, "row_start", ints, n + 1)
+        _expect(seq_len, "seq_len", ints, n)
+        if page_table.dim() != 2 or page_table.shape[0] != n:
+            raise ValueError("page_table must be [n_seqs, slots]")
+        _expect(page_table, "page_table", ints, n * page_table.shape[1])
+        _expect(status, "status", ints, 1)
+        self._keep = (row_start, seq_len, page_table, status)
+        self.c = SeqBatchC(n, n_rows, page_table.shape[1], shared_len, _ptr(row_start), _ptr(seq_len),
+                           _ptr(page_table), _ptr(status))
+
+
+def paged_append(qkv, pages: KvPages, batch: SeqBatch, n_heads: int, rope_cs=None, rope_mode: int = ROPE_GGUF,
+                 q_out=None, rope_len: Optional[int] = None, stream=None) -> None:
+    """Rotates the new rows' queries and keys and writes keys and values to their pages (yl_paged_append). qkv: f32
+    rows [q | k | v]; q_out: rows of rotated queries in the cache's type, or None; rope_cs: [len, head_size/2, 2]
+    (or an address from Transformer.rope_table, with rope_len), or None for no rotation."""
+    p = pages.c
+    n = batch.c.n_rows
+    if _dtype(qkv) != DType.F32:
+        raise TypeError("qkv must be float32")
+    if q_out is not None and _dtype(q_out) != p.dtype:
+        raise TypeError("q_out must have the cache's type")
+    if rope_cs is not None and not isinstance(rope_cs, int):
+        _expect(rope_cs, "rope_cs", ("torch.float32",), rope_cs.shape[0] * p.head_size)
+        rope_len = rope_cs.shape[0] if rope_len is None else min(rope_len, rope_cs.shape[0])
+    _here(qkv, "qkv")
+    if q_out is not None:
+        _here(q_out, "q_out")
+    _check(_lib.yl_paged_append(
+        _ptr(q_out), 0 if q_out is None else _row_stride(q_out, "q_out", n_heads * p.head_size, n), _ptr(qkv),
+        _row_stride(qkv, "qkv", (n_heads + 2 * p.n_kv_heads) * p.head_size, n), C.byref(p), C.byref(batch.c), n_heads,
+        _ptr(rope_cs), rope_len or 0, rope_mode, _stream(stream)))
+
+
+def paged_attention_workspace(pages: KvPages, batch: SeqBatch, n_heads: int) -> int:
+    """Bytes of device workspace paged_attention needs for a batch of these counts."""
+    n = C.c_uint64()
+    _check(_lib.yl_paged_attention_workspace(C.byref(pages.c), C.byref(batch.c), n_heads, C.byref(n)))
+    return n.value
+
+
+def paged_attention(output, q, pages: KvPages, batch: SeqBatch, n_heads: int, attn_scale: float, workspace, lse=None,
+                    stream=None) -> None:
+    """Causal attention of the batch's rows over the paged cache (yl_paged_attention). q: rows of the cache's type,
+    output: rows of that type or f32 ([rows, n_heads, head_size] or flat); lse: f32 [rows, n_heads] or None;
+    workspace: a uint8 tensor of at least paged_attention_workspace bytes."""
+    p = pages.c
+    n = batch.c.n_rows
+    if _dtype(q) != p.dtype:
+        raise TypeError("q must have the cache's type")
+    _expect(lse, "lse", ("torch.float32",), n * n_heads)
+    _here(q, "q")
+    _here(output, "output")
+    _here(workspace, "workspace")
+    width = n_heads * p.head_size
+    _check(_lib.yl_paged_attention(
+        output.data_ptr(), _row_stride(output, "output", width, n), _dtype(output), _ptr(lse), q.data_ptr(),
+        _row_stride(q, "q", width, n), C.byref(p), C.byref(batch.c), n_heads, attn_scale, workspace.data_ptr(),
+        workspace.numel() * workspace.element_size(), _stream(stream)))
+
+
+def token_logprobs(logits, tokens=None, logprobs=None, entropy=None, top_ids=None, top_logprobs=None,
+                   stream=None) -> None:
+    """Log probabilities of the given tokens, entropies and most likely tokens of rows of logits [rows, vocab]
+    (yl_token_logprobs). Device tensors: tokens int32 [rows], logprobs and entropy f32 [rows], top_ids int32 and
+    top_logprobs f32 [rows, k]; each of the three groups may be left out."""
+    if logits.dim() != 2 or logits.stride(1) != 1 and logits.shape[1] > 1:
+        raise ValueError("logits must be [rows, vocab] with consecutive values in a row")
+    n, vocab = logits.shape
+    k = 0 if top_ids is None else top_ids.shape[-1]
+    f, i = ("torch.float32",), ("torch.int32",)
+    _here(logits, "logits")
+    _expect(tokens, "tokens", i, n)
+    _expect(logprobs, "logprobs", f, n)
+    _expect(entropy, "entropy", f, n)
+    _expect(top_ids, "top_ids", i, n * k)
+    _expect(top_logprobs, "top_logprobs", f, n * k)
+    _check(_lib.yl_token_logprobs(logits.data_ptr(), _dtype(logits), logits.stride(0) if n > 1 else vocab, n, vocab,
+                                  _ptr(tokens), _ptr(logprobs), _ptr(entropy), k, _ptr(top_ids), _ptr(top_logprobs),
+                                  _stream(stream)))
+
+
 # -------------------------------------------------- transformer.rs ---
 
 class InferenceSession:
@@ -401,6 +598,12 @@ class SessionBatch:
             se.pos = int(p[i]) + 1
         return ids, logits
 
+    def logits(self) -> int:
+        """Device address of the batch's logits rows [max_sessions, vocab] after forward()."""
+        p = _P()
+        _check(_lib.yl_batch_logits(self._h, C.byref(p)))
+        return p.value
+
     def close(self) -> None:
         if self._h:
             _lib.yl_batch_free(self._h)
@@ -448,6 +651,12 @@ class Transformer:
         s = ShapeC()
         _check(_lib.yl_model_shape(self._h, C.byref(s)))
         return s
+
+    def rope_table(self):
+        """(device address, positions) of the model's (cos, sin) table [positions, head_size/2, 2]."""
+        p, n = _P(), C.c_uint32()
+        _check(_lib.yl_model_rope(self._h, C.byref(p), C.byref(n)))
+        return p.value, n.value
 
     def device_bytes(self) -> int:
         return int(_lib.yl_model_device_bytes(self._h))

@@ -1,0 +1,366 @@
+// Log probabilities of given tokens, entropy and the most likely tokens of
+// rows of logits, in one pass over each row.
+//
+// With m = max x, taken at index i*: S' = sum over i != i* of exp(x_i - m) and
+// W = sum of exp(x_i - m) (x_i - m) give
+//   lse = m + log1p(S'),  logprob(t) = x_t - lse,  entropy = log1p(S') - W / (1 + S').
+// Keeping the largest term out of S' keeps the digits of log probabilities
+// near 0. Partial (m, S', W) join as
+//   m1 >= m2, d = m2 - m1:  S' = S1 + e^d (1 + S2),  W = W1 + e^d (W2 + d (1 + S2)).
+//
+// Most likely tokens: every thread keeps the largest of the values it reads.
+// The k-th largest of the threads' maxima bounds the k-th largest value from
+// below, and only the k threads at or above it can hold one of the k largest,
+// so only their values (a few per cent of the row) are read a second time.
+// Values are compared as 64-bit keys, (value in integer order, ~index), which
+// are distinct, so that equals go to the lower index and nothing depends on
+// the order of atomics.
+//
+// Bound by reading the row (4 bytes and one exponential per value). A row is
+// read by a thread-block cluster of 1..8 blocks, more for few rows, so that
+// one row of a large vocabulary does not wait for one SM; its parts are joined
+// over distributed shared memory.
+#include <cooperative_groups.h>
+
+#include "serve.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace yl {
+namespace k {
+using namespace yl::dev;
+
+namespace {
+
+constexpr uint32_t LP_THREADS = 512;
+constexpr uint32_t LP_WARPS = LP_THREADS / 32;
+constexpr uint32_t LP_CAND = 1024;  // candidates ranked at once
+
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t idx) {
+  const uint32_t b = __float_as_uint(x + 0.0f);  // -0 counts as 0
+  const uint32_t o = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+  return (uint64_t)o << 32 | (0xFFFFFFFFu - idx);
+}
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t o = (uint32_t)(key >> 32);
+  return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+__device__ __forceinline__ uint32_t key_index(uint64_t key) { return 0xFFFFFFFFu - (uint32_t)key; }
+
+// Differences to the maximum are taken no lower: exp is 0 there in f32, and a
+// product with it is 0 too, where -inf, or the lowest f32 times a sum, would
+// give NaN.
+constexpr float FLOOR = -200.0f;
+
+struct Part {
+  float m, s, w;
+};
+__device__ __forceinline__ Part join(Part a, Part b) {
+  if (b.m > a.m) {
+    const Part t = a;
+    a = b;
+    b = t;
+  }
+  if (b.m == -INFINITY) return a;  // no value (a NaN sum stays with a, see below)
+  const float d = fmaxf(b.m - a.m, FLOOR), f = __expf(d);
+  return {a.m, a.s + f * (1.0f + b.s), a.w + f * (b.w + d * (1.0f + b.s))};
+}
+__device__ __forceinline__ Part warp_join(Part p) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    p = join(p, Part{__shfl_xor_sync(FULL, p.m, o), __shfl_xor_sync(FULL, p.s, o), __shfl_xor_sync(FULL, p.w, o)});
+  return p;
+}
+
+// Sorts a warp's 32 keys, largest in lane 0 (bitonic network).
+__device__ __forceinline__ uint64_t warp_sort_desc(uint64_t v, uint32_t lane) {
+#pragma unroll
+  for (uint32_t size = 2; size <= 32; size <<= 1) {
+#pragma unroll
+    for (uint32_t j = size >> 1; j > 0; j >>= 1) {
+      const uint64_t o = __shfl_xor_sync(FULL, v, j);
+      const bool desc = (lane & size) == 0 || size == 32, low = (lane & j) == 0;
+      v = (desc == low) == (v > o) ? v : o;
+    }
+  }
+  return v;
+}
+// The 32 largest of two sorted lists (a, and b in shared memory), sorted.
+__device__ __forceinline__ uint64_t warp_merge_desc(uint64_t a, const uint64_t* b, uint32_t lane) {
+  const uint64_t o = b[31 - lane];
+  uint64_t v = a > o ? a : o;
+#pragma unroll
+  for (uint32_t j = 16; j > 0; j >>= 1) {
+    const uint64_t x = __shfl_xor_sync(FULL, v, j);
+    v = ((lane & j) == 0) == (v > x) ? v : x;
+  }
+  return v;
+}
+// Joins `lists` sorted lists of 32 in shared memory into list 0; all threads.
+__device__ __forceinline__ void join_lists(uint64_t (*list)[32], uint32_t lists, uint32_t warp, uint32_t lane) {
+  for (uint32_t step = 1; step < lists; step <<= 1) {
+    __syncthreads();
+    const uint32_t at = warp * 2 * step;
+    if (at + step < lists) list[at][lane] = warp_merge_desc(list[at][lane], list[at + step], lane);
+  }
+  __syncthreads();
+}
+
+template <typename T>
+struct Row {
+  static constexpr uint32_t PER = 16 / sizeof(T);  // values per 16-byte load
+  const T* x;
+  uint32_t begin, head, vecs, end;  // [begin, begin+head) one by one, then vecs loads, then to end one by one
+
+  __device__ Row(const T* row, uint32_t b, uint32_t e) : x(row), begin(b), end(e) {
+    const uint32_t mis = (uint32_t)(reinterpret_cast<uintptr_t>(row + b) & 15) / sizeof(T);
+    head = mis ? PER - mis : 0;
+    if (head > e - b) head = e - b;
+    vecs = (e - b - head) / PER;
+  }
+  __device__ uint32_t vec_index(uint32_t v) const { return begin + head + v * PER; }
+  __device__ void load(uint32_t v, float (&o)[PER]) const {
+    const uint4 r = __ldg(reinterpret_cast<const uint4*>(x + vec_index(v)));
+    const T* t = reinterpret_cast<const T*>(&r);
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i) o[i] = to_f32(t[i]);
+  }
+  // Calls f(value, index) for every value that thread t reads, lane by lane
+  // of a warp that takes them together.
+  template <typename F>
+  __device__ void each(uint32_t t, uint32_t lane, F&& f) const {
+    if (lane == 0 && t < head) f(to_f32(x[begin + t]), begin + t);
+    for (uint32_t v = t + lane * LP_THREADS; v < vecs; v += 32 * LP_THREADS) {
+      float o[PER];
+      load(v, o);
+#pragma unroll
+      for (uint32_t i = 0; i < PER; ++i) f(o[i], vec_index(v) + i);
+    }
+    const uint32_t tail = vec_index(vecs) + t;
+    if (lane == 0 && tail < end) f(to_f32(x[tail]), tail);
+  }
+};
+
+struct LpShared {
+  uint64_t list[LP_WARPS][32];
+  uint64_t cand[LP_CAND];
+  Part part[LP_WARPS];
+  uint32_t group[LP_MAX_TOP];
+  uint64_t red[LP_WARPS];
+  uint32_t n_group, n_cand;
+  Part whole;
+  uint64_t top[32];  // this block's largest keys, in order
+};
+
+// A thread's running (m, S', W) and the index of m.
+struct Run {
+  float m = -INFINITY, s = 0.0f, w = 0.0f;
+  uint32_t idx = 0xFFFFFFFFu;
+
+  // N consecutive values, the first at index `first`.
+  template <uint32_t N>
+  __device__ __forceinline__ void add(const float (&v)[N], uint32_t first) {
+    float top = v[0];
+#pragma unroll
+    for (uint32_t i = 1; i < N; ++i) top = fmaxf(top, v[i]);
+    if (idx == 0xFFFFFFFFu) idx = first;  // the lowest index stands for a part of nothing but -inf
+    if (top > m) {
+      uint32_t at = 0;
+#pragma unroll
+      for (uint32_t i = N; i-- > 0;)
+        if (v[i] == top) at = i;
+      if (m != -INFINITY) {
+        const float d = fmaxf(m - top, FLOOR), f = __expf(d);
+        w = f * (w + d * (1.0f + s));
+        s = f * (1.0f + s);
+      }
+      m = top;
+      idx = first + at;
+#pragma unroll
+      for (uint32_t i = 0; i < N; ++i) {
+        const float d = v[i] - top, e = i == at ? 0.0f : __expf(d);
+        s += e;
+        w = fmaf(e, fmaxf(d, FLOOR), w);
+      }
+    } else {
+      const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (uint32_t i = 0; i < N; ++i) {
+        const float d = v[i] - ref, e = __expf(d);
+        s += e;
+        w = fmaf(e, fmaxf(d, FLOOR), w);
+      }
+    }
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(LogprobArgs a) {
+  __shared__ LpShared sh;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const uint32_t C = cluster.num_blocks(), rank = cluster.block_rank();
+  const uint32_t row = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const T* x = static_cast<const T*>(a.logits) + (uint64_t)row * a.row_stride;
+  // the given token's logit: asked for before the pass, so that it is there after it
+  int32_t token = -1;
+  float xt = 0.0f;
+  if (rank == 0 && tid == 0 && a.tokens) {
+    token = a.tokens[row];
+    if (token >= 0 && (uint32_t)token < a.vocab) xt = to_f32(x[token]);
+    else token = -1;
+  }
+  const uint32_t each = (a.vocab + C - 1) / C;
+  const uint32_t b = min(rank * each, a.vocab), e = min(b + each, a.vocab);
+  const Row<T> part(x, b, e);
+  constexpr uint32_t PER = Row<T>::PER;
+
+  Run r;
+  if (tid < part.head) {
+    const float v[1] = {to_f32(x[part.begin + tid])};
+    r.add(v, part.begin + tid);
+  }
+  constexpr uint32_t U = 64 / 16;  // 64 bytes in flight per thread
+  uint32_t v = tid;
+  for (; v + (U - 1) * LP_THREADS < part.vecs; v += U * LP_THREADS) {
+    float o[U][PER];
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) part.load(v + u * LP_THREADS, o[u]);
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) r.add(o[u], part.vec_index(v + u * LP_THREADS));
+  }
+  for (; v < part.vecs; v += LP_THREADS) {
+    float o[PER];
+    part.load(v, o);
+    r.add(o, part.vec_index(v));
+  }
+  const uint32_t tail = part.vec_index(part.vecs) + tid;
+  if (tail < e) {
+    const float o[1] = {to_f32(x[tail])};
+    r.add(o, tail);
+  }
+  // a part without a value keeps m = -inf; a NaN among them left a NaN sum
+  const bool nan = isnan(r.s);
+  if (nan) r.m = INFINITY;
+  const Part p = warp_join(Part{r.m, r.s, r.w});
+  if (lane == 0) sh.part[warp] = p;
+
+  if (a.top_k) {
+    const uint64_t mine = r.idx == 0xFFFFFFFFu || nan ? 0ull : key_of(r.m, r.idx);
+    sh.list[warp][lane] = warp_sort_desc(mine, lane);
+    if (tid == 0) sh.n_group = sh.n_cand = 0;
+    join_lists(sh.list, LP_WARPS, warp, lane);
+    // the k-th largest maximum (0 when fewer threads hold values: then all count)
+    const uint64_t thr = sh.list[0][a.top_k - 1];
+    if (mine && mine >= thr) sh.group[atomicAdd(&sh.n_group, 1u)] = tid;
+    __syncthreads();
+    const uint32_t ng = sh.n_group;  // at most top_k: the keys are distinct
+    for (uint32_t g = warp; g < ng; g += LP_WARPS)
+      part.each(sh.group[g], lane, [&](float val, uint32_t idx) {
+        const uint64_t key = key_of(val, idx);
+        if (key >= thr) {
+          const uint32_t at = atomicAdd(&sh.n_cand, 1u);
+          if (at < LP_CAND) sh.cand[at] = key;
+        }
+      });
+    __syncthreads();
+    const uint32_t nc = sh.n_cand;
+    if (tid < 32) sh.top[tid] = 0;
+    __syncthreads();
+    if (nc <= LP_CAND) {
+      for (uint32_t i = tid; i < nc; i += LP_THREADS) {
+        const uint64_t key = sh.cand[i];
+        uint32_t above = 0;
+        for (uint32_t j = 0; j < nc; ++j) above += sh.cand[j] > key;
+        if (above < a.top_k) sh.top[above] = key;
+      }
+    } else {
+      // many values of few threads: take them largest first, one at a time
+      uint64_t last = ~0ull;
+      for (uint32_t i = 0; i < a.top_k; ++i) {
+        uint64_t best = 0;
+        for (uint32_t g = warp; g < ng; g += LP_WARPS)
+          part.each(sh.group[g], lane, [&](float val, uint32_t idx) {
+            const uint64_t key = key_of(val, idx);
+            if (key < last && key > best) best = key;
+          });
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          const uint64_t other = __shfl_xor_sync(FULL, best, o);
+          best = best > other ? best : other;
+        }
+        if (lane == 0) sh.red[warp] = best;
+        __syncthreads();
+        for (uint32_t w = 0; w < LP_WARPS; ++w) best = sh.red[w] > best ? sh.red[w] : best;
+        if (tid == 0) sh.top[i] = best;
+        last = best;
+        __syncthreads();
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const Part q = warp_join(lane < LP_WARPS ? sh.part[lane] : Part{-INFINITY, 0.0f, 0.0f});
+    if (lane == 0) sh.whole = q;
+  }
+  // ---- join the cluster's blocks ----
+  if (C > 1) cluster.sync();
+  else __syncthreads();
+  if (rank == 0) {
+    if (warp < C && a.top_k) {
+      const LpShared* other = C > 1 ? cluster.map_shared_rank(&sh, warp) : &sh;
+      sh.list[warp][lane] = other->top[lane];
+    }
+    Part q = {-INFINITY, 0.0f, 0.0f};
+    if (warp == 0 && lane < C) q = C > 1 ? cluster.map_shared_rank(&sh, lane)->whole : sh.whole;
+    if (a.top_k) join_lists(sh.list, C, warp, lane);
+    if (warp == 0) {
+      q = warp_join(q);
+      // NaN, +inf, or nothing above -inf: no distribution
+      const bool none = isnan(q.s) || fabsf(q.m) == INFINITY;
+      const float nanf_ = __int_as_float(0x7FC00000);
+      const float log_sum = log1pf(q.s);
+      if (lane == 0) {
+        if (a.tokens) a.logprobs[row] = none || token < 0 ? nanf_ : (xt - q.m) - log_sum;
+        if (a.entropy) a.entropy[row] = none ? nanf_ : log_sum - q.w / (1.0f + q.s);
+      }
+      if (lane < a.top_k) {
+        const uint64_t key = sh.list[0][lane];
+        a.top_ids[(uint64_t)row * a.top_k + lane] = none ? -1 : (int32_t)key_index(key);
+        a.top_logprobs[(uint64_t)row * a.top_k + lane] = none ? nanf_ : (key_value(key) - q.m) - log_sum;
+      }
+    }
+  }
+  if (C > 1) cluster.sync();  // the other blocks' shared memory stays until it has been read
+}
+
+template <typename T>
+cudaError_t launch(const LogprobArgs& a, cudaStream_t stream) {
+  // blocks per row: enough to have two on every SM, while each still reads
+  // 4096 values or more
+  uint32_t c = 1;
+  while (c < 8 && (uint64_t)a.n_rows * c < 2 * 148 && a.vocab / (2 * c) >= 4096) c *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.n_rows * c);
+  cfg.blockDim = dim3(LP_THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = c;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, a);
+}
+
+}  // namespace
+
+cudaError_t token_logprobs(const LogprobArgs& a, int dtype, cudaStream_t stream) {
+  switch (dtype) {
+    case DT_F32: return launch<float>(a, stream);
+    case DT_F16: return launch<__half>(a, stream);
+    default: return launch<__nv_bfloat16>(a, stream);
+  }
+}
+
+}  // namespace k
+}  // namespace yl

@@ -1,0 +1,65 @@
+// Device helpers of the serving kernels: element types, finding a row's
+// sequence.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "device.cuh"
+#include "serve.h"
+
+namespace yl {
+namespace dev {
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Two values rounded and packed, the first in the low half.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The sequence whose rows include `row`, or n_seqs for a padding row: the
+// number of sequences that begin at or before the row, less one, skipping
+// empty ones. A 32-way search by a whole warp: two loads in turn for up to
+// 1024 sequences.
+__device__ __forceinline__ uint32_t warp_find_seq(const k::Seqs& s, uint32_t row, uint32_t lane) {
+  // invariant: row_start[lo] <= row < row_start[hi] (hi = n_seqs + 1 stands for infinity)
+  if (row >= row_begin(s, s.n_seqs) || row < row_begin(s, 0)) return s.n_seqs;
+  uint32_t lo = 0, hi = s.n_seqs;
+  while (hi - lo > 1) {
+    const uint32_t step = (hi - lo + 31) / 32;
+    const uint32_t at = lo + (lane + 1) * step;
+    const bool le = at < hi && row_begin(s, at) <= row;
+    const uint32_t n = __popc(__ballot_sync(FULL, le));
+    lo += n * step;
+    if (lo + step < hi) hi = lo + step;
+  }
+  return lo;
+}
+
+}  // namespace dev
+}  // namespace yl
