@@ -518,11 +518,16 @@ int yl_kv_pages_free(yl_kv_pages* p);
  * is idle). Attention then reads those pages once for all sequences. With 0
  * every sequence's pages are read for itself; the results agree to rounding.
  * The arrays are on the device (one call's geometry may be computed there, and
- * a captured graph replays with new contents), so they are checked there: a
- * page id >= n_pages, or a position without a table slot, or beyond the rope
- * table, is neither read (keys and values there count as zeros) nor written,
- * and YL_ERR_RANGE is stored to *status (nullable; never cleared here).
- * row_start values are limited to n_rows and to ascending order. */
+ * a captured graph replays with new contents), so they are checked there, and
+ * YL_ERR_RANGE is stored to *status (nullable; never cleared here) for
+ *  - a page id >= n_pages: nothing is written there, its keys and values read
+ *    as zeros;
+ *  - a position without a table slot (or from 2^31 - 256 on): nothing is
+ *    written, its key is left out;
+ *  - a row to append at a position before 0 or beyond the rope table: the row
+ *    is left out.
+ * row_start values are limited to n_rows and to ascending order. A device wait
+ * that runs out stores YL_ERR_TIMEOUT. */
 typedef struct yl_seq_batch {
   uint32_t n_seqs, n_rows, table_stride, shared_len;
   const uint32_t* row_start;  /* [n_seqs + 1] */

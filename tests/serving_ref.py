@@ -57,7 +57,7 @@ class Geometry:
         return torch.where(torch.from_numpy(good)[:, None, None], rows, 0.0)
 
 
-def attention(g: Geometry, q, k, v, scale):
+def attention(g: Geometry, q, k, v, scale, limit=1 << 31):
     """(out, lse, out_bound, lse_bound) in 64 bits. The bounds count, for scores of |terms| sum A: products and sums of
     hd terms, each off by at most two half steps of f32 (a tensor core may truncate) in chains of hd/4 + 16; for the
     softmax: exp of an f32 argument (its rounding: |s| * 2 U32; exp itself: 4 U32) and sums in chains of n/4 + 64; for a
@@ -74,7 +74,7 @@ def attention(g: Geometry, q, k, v, scale):
         for t, pos in enumerate(g.positions(i)):
             if pos < 0:
                 continue
-            r, m = int(g.row_start[i]) + t, int(pos) + 1
+            r, m = int(g.row_start[i]) + t, min(int(pos) + 1, limit)
             for h in range(g.heads):
                 qq, kk, vv = q[r, h].double(), ks[:m, h // group], vs[:m, h // group]
                 s = kk @ qq * scale

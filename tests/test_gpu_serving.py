@@ -240,7 +240,8 @@ def test_not_finite_keys_reach_their_readers_only(yl, torch_cuda):
         assert torch.equal(got[[0, 2]], clean[[0, 2]]) and got[1].isnan().all() and lse[1].isnan().all()
 
 
-def test_bad_pages_read_as_zeros(yl, torch_cuda):
+def test_bad_pages_and_missing_slots(yl, torch_cuda):
+    """Ids that are no pages read as zeros; keys behind the table's last slot are left out. The status word tells."""
     for t in DTYPES.values():
         for where in ("page", "slot"):
             g = ref.Geometry(13, 4, 2, 64, page=16, lens=[40, 130], rows=[1, 2], spare_slots=0)
@@ -248,9 +249,8 @@ def test_bad_pages_read_as_zeros(yl, torch_cuda):
             if where == "page":
                 g.table[1, 3] = 0xFFFFFFF0
                 want = ref.attention(g, q, k, v, 0.125)
-            else:  # the last slots are missing: the same as ids that are no pages
-                g.table[1, 6:] = 0xFFFFFFFF
-                want = ref.attention(g, q, k, v, 0.125)
+            else:  # both rows of the second sequence see what six pages hold
+                want = ref.attention(g, q, k, v, 0.125, limit=96)
                 g.table = g.table[:, :6].copy()
             status = torch.zeros(1, dtype=torch.int32, device="cuda")
             out, lse = attend(yl, g, q.cuda(), k.cuda(), v.cuda(), 0.125, status=status)

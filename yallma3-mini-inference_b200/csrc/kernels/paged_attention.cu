@@ -1,6 +1,42 @@
-// Causal grouped-query attention over the paged cache. One block per (row,
-// head): each of its warps takes every fourth key, keeps a running maximum,
-// sum and output, and the warps' parts are joined at the end.
+// Causal grouped-query attention over the paged cache.
+//
+// For a row r at position p and the keys j <= p of its sequence
+//   s_j = scale q.k_j,  m = max s_j,  l = sum e^(s_j - m),  o = sum e^(s_j - m) v_j / l
+// in one pass over keys and values with a running (m, l, O); parts over
+// different keys join as m = max m_i, l = sum l_i e^(m_i - m), O likewise.
+// Scores are kept times log2(e), so that every exponential is one ex2.
+//
+// Work: the rows of a sequence that share a key/value head (new tokens x query
+// heads of the group) are cut into row tiles, the keys into key tiles of 16 KB;
+// one (head, row tile) is an item, its key tiles are counted up to its last
+// row's position. All key tiles of all items form one line that is cut into
+// equal pieces, one per block: long and short sequences, few and many, load
+// every SM alike. An item cut by a piece's end leaves its parts (m, l, O) in
+// the workspace, and a second kernel joins them. The geometry is read from
+// device memory by every block, so a captured launch follows its arrays.
+//
+// Shared prefix: a first launch lets the rows of all sequences attend to the
+// prefix together, as rows of one sequence (its keys are read once per row
+// tile, not once per sequence), a second one to the rest; the parts are joined
+// likewise. Blocks of the second start as those of the first end (programmatic
+// dependent launch; it waits for the first only before it ends).
+//
+// Within a block one warp fetches key and value tiles page by page with TMA
+// (128-byte swizzle; a page id that is none goes to a coordinate outside the
+// tensor, which reads as zeros) into a ring of 16 KB buffers; the others
+// multiply with mma.sync, WM warps of 16 rows each times WK warps that split
+// the tile's keys and join at the item's end. Decoding has 1..16 rows per
+// item and is bound by reading the cache, so WK = 4; from 33 rows on WK = 1.
+// f32 operands are split into two tf32 numbers and multiplied as hi*hi + hi*lo
+// + lo*hi (2^-21 relative); 16-bit ones are exact, and the softmax weights are
+// rounded to their type for the second product (the sum l takes them
+// unrounded), f16 weights at 2^10 times their value so that small ones do not
+// fall below f16's range.
+#include <cuda.h>
+
+#include <atomic>
+#include <type_traits>
+
 #include "serve.cuh"
 
 namespace yl {
@@ -9,83 +45,911 @@ using namespace yl::dev;
 
 namespace {
 
-template <typename T, typename O, int HD>
-__global__ void __launch_bounds__(128) attend_kernel(PagedAttnArgs a) {
-  constexpr int PER = HD / 32;
-  __shared__ float part[4][HD + 2];
-  const uint32_t row = blockIdx.x, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t seq = warp_find_seq(a.seqs, row, lane);
-  if (seq == a.seqs.n_seqs) return;
-  const uint32_t back = row_end(a.seqs, seq) - row, len = a.seqs.seq_len[seq];
-  const uint32_t keys = len >= back ? len - back + 1 : 0;
-  const uint32_t kvh = head / (a.n_heads / a.pages.n_kv_heads);
-  const T* q = static_cast<const T*>(a.q) + (uint64_t)row * a.q_stride + (uint64_t)head * HD;
-  float qv[PER], o[PER];
+constexpr uint32_t BUF = 16384;  // bytes of a key or value tile
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int STATUS_TIMEOUT = -7;  // YL_ERR_TIMEOUT
+
+// One launch: over the sequences' own keys (from `from` on), or over the
+// shared prefix with all rows as one sequence.
+struct Pass {
+  PagedAttnArgs a;
+  uint32_t from, prefix;  // first key; 1: the prefix pass (keys 0 .. shared_len)
+  uint32_t group, min_chunk;
+  int joined;      // every item leaves its part in the workspace
+  uint2* desc;     // [n_rows][n_kv_heads] {first block, blocks << 16 | token in the tile}
+  float* slots;    // [2 * grid][BM][HD + 2]
+  float* rowpart;  // [n_rows][n_heads][HD + 2]: items of one block, where every item leaves its part
+};
+
+template <typename T, int HD, int WM_, int WK_>
+struct Shape {
+  static constexpr int WM = WM_, WK = WK_, NW = WM * WK, THREADS = 32 * (NW + 1);
+  static constexpr int BM = 16 * WM;
+  static constexpr int ROW = HD * (int)sizeof(T);  // bytes of a row
+  static constexpr int NH = ROW / 128;             // 128-byte columns
+  static constexpr int KT = BUF / ROW;             // keys per tile
+  static constexpr int WKEYS = KT / WK;
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int NBUF = F32 && HD == 128 ? (WM == 2 ? 3 : 4) : WK > 1 ? 4 : 5;  // what two blocks per SM leave room for
+  static constexpr int QP = HD + 4;  // f32 queries and the warps' joining: row stride in shared memory, no bank conflicts
+  static constexpr uint32_t Q_BYTES = F32 ? BM * QP * 4 : 0;
+  static constexpr uint32_t M_BYTES = WK > 1 ? NW * 16 * QP * 4 : 0;
+  static constexpr uint32_t SMEM = 1024 + NBUF * BUF + Q_BYTES + M_BYTES;
+  static_assert(SMEM <= 113 * 1024 - 1024, "two blocks per SM");
+  static_assert(WKEYS % (F32 ? 8 : 16) == 0, "whole MMA steps");
+};
+
+// ---- MMA -------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = hi + lo: hi the nearest tf32, lo exact in f32 (the MMA drops its last bits, 2^-21 of x)
+__device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  lo = __float_as_uint(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ float lds(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 4-D tiled load of a page's part: (element, head, token in the page, page).
+__device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t head, uint32_t tok,
+                                         uint32_t page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(tok), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Byte of 16-byte column c of row `key` in a tile.
+template <typename S>
+__device__ __forceinline__ uint32_t at(uint32_t key, uint32_t c) {
+  return (c >> 3) * (S::KT * 128) + key * 128 + (((c & 7) ^ (key & 7)) << 4);
+}
+
+// ---- work ------------------------------------------------------------------
+// A sequence as a pass sees it.
+struct Rows {
+  uint32_t row0, n;  // its rows
+  int64_t pos0;      // position of the first
+  uint32_t limit;    // keys that may be read: the prefix, or what the page table has slots for
+};
+__device__ __forceinline__ Rows rows_of(const Pass& p, uint32_t i) {
+  const Seqs& s = p.a.seqs;
+  Rows r;
+  if (p.prefix) {
+    r.row0 = row_begin(s, 0);
+    const uint32_t e = row_begin(s, s.n_seqs);
+    r.n = e > r.row0 ? e - r.row0 : 0;
+    r.pos0 = 0;
+    r.limit = s.shared_len;
+  } else {
+    r.row0 = row_begin(s, i);
+    r.n = row_end(s, i) - r.row0;
+    r.pos0 = (int64_t)s.seq_len[i] - r.n;
+    r.limit = table_limit(s, p.a.pages);
+  }
+  return r;
+}
+// First key behind those that tokens [.., t) of the sequence see.
+__device__ __forceinline__ uint32_t keys_end(const Pass& p, const Rows& r, uint32_t t) {
+  if (p.prefix) return r.limit;
+  const int64_t e = r.pos0 + (t < r.n ? t : r.n);
+  return e <= 0 ? 0 : e < (int64_t)r.limit ? (uint32_t)e : r.limit;
+}
+// Key tiles of the row tile that ends at token t (one where it sees no key).
+template <typename S>
+__device__ __forceinline__ uint32_t tiles_of(const Pass& p, const Rows& r, uint32_t t) {
+  const uint32_t e = keys_end(p, r, t);
+  return e > p.from + S::KT ? (e - p.from + S::KT - 1) / S::KT : 1;
+}
+template <typename S>
+__device__ __forceinline__ uint64_t tiles_per_head(const Pass& p, const Rows& r, uint32_t tpt) {
+  uint64_t n = 0;
+  if (p.prefix) return (uint64_t)((r.n + tpt - 1) / tpt) * tiles_of<S>(p, r, r.n);
+  for (uint32_t t = 0; t < r.n; t += tpt) n += tiles_of<S>(p, r, t + tpt);
+  return n;
+}
+
+// Where a block's piece of the line begins.
+struct Start {
+  uint64_t begin, end, chunk;  // in key tiles
+  uint32_t seq, head, t, kt;   // sequence, head, first token of the row tile, key tile
+  uint64_t g0;                 // where the item begins on the line
+  int masked;                  // prefix pass: some row does not see all of the prefix
+};
+
+template <typename S>
+__device__ void find_start(const Pass& p, uint32_t tpt, Start* out, uint64_t* scratch) {
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t n = p.prefix ? 1 : p.a.seqs.n_seqs;
+  const uint32_t heads = p.a.pages.n_kv_heads;
+  constexpr uint32_t NWARPS = S::THREADS / 32;
+  __shared__ int any_masked;
+  if (tid == 0) any_masked = 0, out->seq = 0xFFFFFFFFu;
+  __syncthreads();
+  if (p.prefix) {  // rows inside the prefix
+    bool m = false;
+    for (uint32_t i = tid; i < p.a.seqs.n_seqs; i += S::THREADS) {
+      const uint32_t rn = row_end(p.a.seqs, i) - row_begin(p.a.seqs, i);
+      m |= rn && (int64_t)p.a.seqs.seq_len[i] - rn + 1 < (int64_t)p.a.seqs.shared_len;
+    }
+    if (m) any_masked = 1;
+  }
+  // exclusive sums of the sequences' tiles, a block's width at a time; the
+  // second time over, the piece's place is looked for
+  uint64_t total = 0, begin = 0;
+  for (int round = 0; round < 2; ++round) {
+    uint64_t base = 0;
+    for (uint32_t c = 0; c < n; c += S::THREADS) {
+      const uint32_t i = c + tid;
+      Rows r{};
+      uint64_t per_head = 0;
+      if (i < n) {
+        r = rows_of(p, i);
+        per_head = tiles_per_head<S>(p, r, tpt);
+      }
+      const uint64_t mine = per_head * heads;
+      uint64_t inc = mine;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) qv[i] = to_f32(q[lane + 32 * i]) * a.scale, o[i] = 0.0f;
-  float m = -INFINITY, l = 0.0f;
-  for (uint32_t j = warp; j < keys; j += 4) {
-    const uint32_t page = page_of(a.seqs, a.pages, j < a.seqs.shared_len ? 0 : seq, j);
-    float kv[PER], vv[PER], s = 0.0f;
-    if (page == NO_PAGE) {
-      if (a.seqs.status) *a.seqs.status = STATUS_RANGE;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) kv[i] = vv[i] = 0.0f;
-    } else {
-      const uint64_t at = slot_offset(a.pages, page, j, kvh);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        kv[i] = to_f32(static_cast<const T*>(a.pages.k)[at + lane + 32 * i]);
-        vv[i] = to_f32(static_cast<const T*>(a.pages.v)[at + lane + 32 * i]);
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t v = __shfl_up_sync(FULL, inc, o);
+        if ((int)lane >= o) inc += v;
+      }
+      __syncthreads();
+      if (lane == 31) scratch[warp] = inc;
+      __syncthreads();
+      uint64_t before = base, sum = 0;
+      for (uint32_t w = 0; w < NWARPS; ++w) {
+        if (w < warp) before += scratch[w];
+        sum += scratch[w];
+      }
+      const uint64_t first = before + inc - mine;
+      if (round == 1 && begin >= first && begin < first + mine) {
+        uint64_t off = begin - first, g0 = first;
+        const uint64_t h = off / per_head;
+        off -= h * per_head;
+        g0 += h * per_head;
+        uint32_t t = 0, nt = tiles_of<S>(p, r, tpt);
+        while (off >= nt) {
+          off -= nt;
+          g0 += nt;
+          t += tpt;
+          nt = tiles_of<S>(p, r, t + tpt);
+        }
+        out->seq = i;
+        out->head = (uint32_t)h;
+        out->t = t;
+        out->kt = (uint32_t)off;
+        out->g0 = g0;
+      }
+      base += sum;
+    }
+    if (round == 0) {
+      total = base;
+      uint64_t chunk = (total + gridDim.x - 1) / gridDim.x;
+      if (chunk < p.min_chunk) chunk = p.min_chunk;
+      begin = chunk * blockIdx.x;
+      if (tid == 0) {
+        out->chunk = chunk;
+        out->begin = begin;
+        out->end = begin + chunk < total ? begin + chunk : total;
+      }
+      if (begin >= total) break;  // nothing for this block: seq stays unset
+    }
+  }
+  __syncthreads();
+  if (tid == 0) out->masked = any_masked;
+  __syncthreads();
+}
+
+// Walks a block's piece: one step per item, the same in every warp.
+template <typename S>
+struct Walk {
+  const Pass& p;
+  const uint32_t tpt;
+  uint64_t at, end, chunk, g0;
+  uint32_t seq, head, t, kt0, kt1, nt;
+  Rows r;
+
+  __device__ Walk(const Pass& pass, uint32_t tokens, const Start& s)
+      : p(pass), tpt(tokens), at(s.begin), end(s.end), chunk(s.chunk), g0(s.g0), seq(s.seq), head(s.head), t(s.t),
+        kt0(s.kt) {
+    r = rows_of(p, seq);
+    piece();
+  }
+  __device__ void piece() {
+    nt = tiles_of<S>(p, r, t + tpt);
+    const uint64_t left = end - at;
+    kt1 = nt - kt0 < left ? nt : kt0 + (uint32_t)left;
+  }
+  __device__ bool next() {
+    at += kt1 - kt0;
+    if (at >= end) return false;
+    g0 += nt;
+    kt0 = 0;
+    t += tpt;
+    if (t >= r.n) {
+      t = 0;
+      if (++head == p.a.pages.n_kv_heads) {
+        head = 0;
+        do {
+          if (++seq >= p.a.seqs.n_seqs || p.prefix) return false;
+          r = rows_of(p, seq);
+        } while (r.n == 0);
       }
     }
-#pragma unroll
-    for (int i = 0; i < PER; ++i) s += qv[i] * kv[i];
-    s = warp_sum(s);
-    const float top = fmaxf(m, s), f = m == -INFINITY ? 0.0f : expf(m - top), p = expf(s - top);
-    l = l * f + p;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) o[i] = o[i] * f + p * vv[i];
-    m = top;
+    piece();
+    return true;
   }
+  __device__ uint32_t tokens() const { return r.n - t < tpt ? r.n - t : tpt; }
+  __device__ uint32_t kend() const { return keys_end(p, r, t + tpt); }
+  // Whole in one block, or the blocks it lies in.
+  __device__ uint32_t first_block() const { return (uint32_t)(g0 / chunk); }
+  __device__ uint32_t blocks() const { return (uint32_t)((g0 + nt - 1) / chunk) - first_block() + 1; }
+};
+
+// Sequence of a row by bisection (rows inside the prefix only).
+__device__ uint32_t find_seq(const Seqs& s, uint32_t row) {
+  uint32_t lo = 0, hi = s.n_seqs;
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (row_begin(s, mid) <= row) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+template <typename T, typename O, int HD, int WM, int WK>
+__global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
+    attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                  const __grid_constant__ Pass p) {
+  using S = Shape<T, HD, WM, WK>;
+  constexpr float SHIFT = std::is_same<T, __half>::value ? 10.0f : 0.0f;
+  extern __shared__ uint8_t raw[];
+  __shared__ Start start;
+  __shared__ uint64_t scratch[16];
+  __shared__ __align__(8) uint64_t full[S::NBUF], empty[S::NBUF];
+  __shared__ float ml[S::NW][16][2];
+  __shared__ volatile int abort_flag;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  float* qs = reinterpret_cast<float*>(smem + S::NBUF * BUF);
+  float* join = reinterpret_cast<float*>(smem + S::NBUF * BUF + S::Q_BYTES);
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t tpt = S::BM / p.group;
+
+  if (threadIdx.x == 0) {
+    for (int b = 0; b < S::NBUF; ++b) {
+      mbar_init(&full[b], 1);
+      mbar_init(&empty[b], S::NW);
+    }
+    mbar_fence_init();
+    abort_flag = 0;
+  }
+  grid_dep_launch();  // what follows may be scheduled; it waits for this grid's end
+  find_start<S>(p, tpt, &start, scratch);
+  const bool idle = start.seq == 0xFFFFFFFFu;
+  const PagedAttnArgs& a = p.a;
+
+  if (!idle && warp == S::NW) {
+    // ---- producer: key and value tiles, page by page ----
+    Walk<S> w(p, tpt, start);
+    const uint32_t ps = 1u << a.pages.page_shift;
+    const uint32_t tb = ps < (uint32_t)S::KT ? ps : (uint32_t)S::KT;  // tokens per load
+    const uint32_t pieces = S::KT / tb;
+    uint32_t n = 0, issued = 0;
+    bool ok = true;
+    do {
+      const uint32_t kend = w.kend(), tseq = p.prefix ? 0 : w.seq;
+      if (lane == 0 && !p.prefix && a.seqs.status && w.r.pos0 + (int64_t)w.r.n > (int64_t)w.r.limit)
+        *a.seqs.status = STATUS_RANGE;
+      for (uint32_t kt = w.kt0; kt < w.kt1 && ok; ++kt) {
+        const uint32_t k0 = p.from + kt * S::KT;
+        const uint32_t live = kend > k0 ? min(pieces, (kend - k0 + tb - 1) / tb) : 0;  // loads with a visible key
+        for (uint32_t kv = 0; kv < 2 && ok; ++kv, ++n) {
+          const uint32_t b = n % S::NBUF, round = n / S::NBUF;
+          // one load per lane: lane l fetches column l % NH of piece l / NH
+          const uint32_t dst = smem_u32(smem) + b * BUF;
+          if (n >= (uint32_t)S::NBUF) {
+            if (lane == 0) ok = mbar_wait(&empty[b], (round - 1) & 1, nullptr);
+            ok = __shfl_sync(FULL, ok ? 1 : 0, 0) != 0 && !abort_flag;
+            ok = __all_sync(FULL, ok);
+            if (!ok) break;
+          }
+          if (lane == 0) mbar_arrive_expect_tx(&full[b], live * tb * 128 * S::NH);
+          __syncwarp();
+          for (uint32_t u = lane; u < live * S::NH; u += 32) {
+            const uint32_t piece = u / S::NH, col = u % S::NH, pos = k0 + piece * tb;
+            uint32_t page = page_of(a.seqs, a.pages, tseq, pos);
+            if (page == NO_PAGE) {
+              page = a.pages.n_pages;
+              if (a.seqs.status) *a.seqs.status = STATUS_RANGE;
+            }
+            tma_page(dst + col * (S::KT * 128) + piece * tb * 128, kv ? &map_v : &map_k, col * (128 / sizeof(T)),
+                     w.head, pos & (ps - 1), page, &full[b]);
+          }
+          issued = n + 1;
+        }
+      }
+    } while (ok && w.next());
+    if (!ok) {
+      abort_flag = 1;
+      if (lane == 0) {
+        if (a.seqs.status) *a.seqs.status = STATUS_TIMEOUT;
+        // the copies this warp issued land before the block ends
+        for (uint32_t i = issued > (uint32_t)S::NBUF ? issued - S::NBUF : 0; i < issued; ++i)
+          mbar_wait(&full[i % S::NBUF], (i / S::NBUF) & 1, nullptr, 200000000ull);
+      }
+      __syncwarp();
+    }
+  } else if (!idle) {
+    // ---- consumers ----
+    Walk<S> w(p, tpt, start);
+    const uint32_t wm = warp / WK, wk = warp % WK, g = lane >> 2, t4 = lane & 3;
+    const float scale2 = a.scale * LOG2E;
+    constexpr int NB = S::WKEYS / 8, OB = HD / 8;
+    uint32_t n = 0;
+    bool ok = true;
+    do {
+      const uint32_t ntok = w.tokens(), nrow = ntok * p.group, kend = w.kend();
+      // this thread's rows of the tile: token and query head
+      uint32_t row[2], head[2];
+      int32_t lim[2];  // keys the row sees
+      bool live[2];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) part[warp][lane + 32 * i] = o[i];
-  if (lane == 0) part[warp][HD] = m, part[warp][HD + 1] = l;
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t m = wm * 16 + g + 8 * i, tok = m / p.group;
+        live[i] = m < nrow;
+        row[i] = w.r.row0 + w.t + (live[i] ? tok : 0);
+        head[i] = w.head * p.group + (live[i] ? m % p.group : 0);
+        int64_t e = w.r.pos0 + w.t + tok + 1;
+        if (p.prefix) {
+          e = kend;
+          if (start.masked && live[i]) {
+            const uint32_t s = find_seq(a.seqs, row[i]);
+            e = (int64_t)a.seqs.seq_len[s] - row_end(a.seqs, s) + row[i] + 1;
+          }
+        }
+        lim[i] = live[i] ? (int32_t)(e < 0 ? 0 : e < (int64_t)kend ? e : kend) : 0x7FFFFFFF;
+      }
+      // smallest of the row tile: tiles that end before it need no mask
+      const uint32_t all_see = p.prefix ? (start.masked ? 0 : kend) : [&] {
+        const int64_t e = w.r.pos0 + w.t + 1;
+        return e < 0 ? 0u : e < (int64_t)kend ? (uint32_t)e : kend;
+      }();
+
+      uint32_t qf[S::F32 ? 1 : HD / 16][4];
+      if constexpr (S::F32) {
+        named_bar_sync(1, 32 * S::NW);  // every warp is done with the item before
+        for (uint32_t u = threadIdx.x; u < S::BM * (HD / 4); u += 32 * S::NW) {
+          const uint32_t m = u / (HD / 4), c = u % (HD / 4);
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (m < nrow)
+            v = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) +
+                                                 (uint64_t)(w.r.row0 + w.t + m / p.group) * a.q_stride +
+                                                 (uint64_t)(w.head * p.group + m % p.group) * HD + 4 * c);
+          *reinterpret_cast<float4*>(qs + m * S::QP + 4 * c) = v;
+        }
+        named_bar_sync(1, 32 * S::NW);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t* q = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.q) +
+                                                                (uint64_t)row[i] * a.q_stride + (uint64_t)head[i] * HD);
+#pragma unroll
+          for (int s = 0; s < HD / 16; ++s) {
+            qf[s][i] = live[i] ? q[8 * s + t4] : 0;
+            qf[s][2 + i] = live[i] ? q[8 * s + 4 + t4] : 0;
+          }
+        }
+      }
+      float o[OB][4];
+#pragma unroll
+      for (int j = 0; j < OB; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+      const bool busy = wm * 16 < nrow;  // a warp without a row only hands the buffers on
+
+      for (uint32_t kt = w.kt0; kt < w.kt1 && ok; ++kt) {
+        const uint32_t k0 = p.from + kt * S::KT;
+        uint32_t b = n % S::NBUF;
+        uint32_t base = smem_u32(smem) + b * BUF;
+        ok = mbar_wait(&full[b], (n / S::NBUF) & 1, nullptr);
+        ok = __all_sync(FULL, ok);
+        if (!ok) break;
+        float s[NB][4];
+        if (busy) {
+#pragma unroll
+          for (int j = 0; j < NB; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+          if constexpr (S::F32) {
+#pragma unroll 2
+            for (int ks = 0; ks < HD / 16; ++ks) {  // 16 elements: two k-steps of 8
+              uint32_t ah[2][4], al[2][4];
+              const float* q0 = qs + (wm * 16 + g) * S::QP + 16 * ks + t4;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                split(q0[8 * h], ah[h][0], al[h][0]);
+                split(q0[8 * h + 8 * S::QP], ah[h][1], al[h][1]);
+                split(q0[8 * h + 4], ah[h][2], al[h][2]);
+                split(q0[8 * h + 4 + 8 * S::QP], ah[h][3], al[h][3]);
+              }
+#pragma unroll
+              for (int j = 0; j < NB; ++j) {
+                uint32_t r[4];
+                ldsm4(r, base + at<S>(wk * S::WKEYS + 8 * j + (lane & 7), 4 * ks + (lane >> 3)));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  uint32_t bh[2], bl[2];
+                  split(__uint_as_float(r[2 * h]), bh[0], bl[0]);
+                  split(__uint_as_float(r[2 * h + 1]), bh[1], bl[1]);
+                  mma_tf32(s[j], al[h], bh[0], bh[1]);
+                  mma_tf32(s[j], ah[h], bl[0], bl[1]);
+                  mma_tf32(s[j], ah[h], bh[0], bh[1]);
+                }
+              }
+            }
+          } else {
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+              for (int j = 0; j < NB; j += 2) {
+                uint32_t r[4];
+                ldsm4(r, base + at<S>(wk * S::WKEYS + 8 * j + (lane & 7) + ((lane >> 4) << 3), 2 * ks + ((lane >> 3) & 1)));
+                mma16<T>(s[j], qf[ks], r[0], r[1]);
+                mma16<T>(s[j + 1], qf[ks], r[2], r[3]);
+              }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[b]);
+        ++n;
+        float corr[2];
+        if (busy) {
+          const bool mask = k0 + S::KT > all_see;
+          float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              s[j][c] *= scale2;
+              if (mask && (int32_t)(k0 + wk * S::WKEYS + 8 * j + 2 * t4 + (c & 1)) >= lim[c >> 1]) s[j][c] = -INFINITY;
+              top[c >> 1] = fmaxf(top[c >> 1], s[j][c]);
+            }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            top[i] = fmaxf(top[i], __shfl_xor_sync(FULL, top[i], 1));
+            top[i] = fmaxf(top[i], __shfl_xor_sync(FULL, top[i], 2));
+            const float mn = fmaxf(m[i], top[i]);
+            const float ref = mn == -INFINITY ? 0.0f : mn - SHIFT;
+            corr[i] = ex2(m[i] - (mn == -INFINITY ? 0.0f : mn));  // 0 from -inf
+            m[i] = mn;
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+              for (int c = 2 * i; c < 2 * i + 2; ++c) {
+                s[j][c] = ex2(s[j][c] - ref);
+                sum += s[j][c];
+              }
+            l[i] = l[i] * corr[i] + sum;
+          }
+          if (__any_sync(FULL, corr[0] != 1.0f || corr[1] != 1.0f)) {
+#pragma unroll
+            for (int j = 0; j < OB; ++j) {
+              o[j][0] *= corr[0], o[j][1] *= corr[0];
+              o[j][2] *= corr[1], o[j][3] *= corr[1];
+            }
+          }
+        }
+        b = n % S::NBUF;
+        base = smem_u32(smem) + b * BUF;
+        ok = mbar_wait(&full[b], (n / S::NBUF) & 1, nullptr);
+        ok = __all_sync(FULL, ok);
+        if (!ok) break;
+        if (busy) {
+          if (k0 + S::KT > kend) {
+            // values behind the last visible key may be anything: their weight is 0, and 0 times NaN is not
+            for (uint32_t u = lane; u < (uint32_t)S::WKEYS * S::NH * 8; u += 32) {
+              const uint32_t key = wk * S::WKEYS + u / (S::NH * 8), c = u % (S::NH * 8);
+              if (k0 + key >= kend)
+                *reinterpret_cast<uint4*>(smem + b * BUF + at<S>(key, c)) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async();  // before the next TMA write of the buffer
+            __syncwarp();
+          }
+          if constexpr (S::F32) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+              // keys 2i of the eight are the MMA's k = i, keys 2i+1 its k = 4+i: the weights are where QK left them
+              uint32_t ph[4], pl[4];
+              split(s[j][0], ph[0], pl[0]);
+              split(s[j][2], ph[1], pl[1]);
+              split(s[j][1], ph[2], pl[2]);
+              split(s[j][3], ph[3], pl[3]);
+              const uint32_t key = wk * S::WKEYS + 8 * j + 2 * t4;
+#pragma unroll
+              for (int d = 0; d < OB; ++d) {
+                const uint32_t c = 2 * d + (g >> 2), e = (g & 3) * 4;
+                uint32_t vh[2], vl[2];
+                split(lds(base + at<S>(key, c) + e), vh[0], vl[0]);
+                split(lds(base + at<S>(key + 1, c) + e), vh[1], vl[1]);
+                mma_tf32(o[d], pl, vh[0], vh[1]);
+                mma_tf32(o[d], ph, vl[0], vl[1]);
+                mma_tf32(o[d], ph, vh[0], vh[1]);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < NB; j += 2) {
+              const uint32_t pf[4] = {pack2<T>(s[j][0], s[j][1]), pack2<T>(s[j][2], s[j][3]),
+                                      pack2<T>(s[j + 1][0], s[j + 1][1]), pack2<T>(s[j + 1][2], s[j + 1][3])};
+#pragma unroll
+              for (int d = 0; d < OB; d += 2) {
+                uint32_t r[4];
+                ldsm4t(r, base + at<S>(wk * S::WKEYS + 8 * j + (lane & 15), d + (lane >> 4)));
+                mma16<T>(o[d], pf, r[0], r[1]);
+                mma16<T>(o[d + 1], pf, r[2], r[3]);
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[b]);
+        ++n;
+      }
+      if (!ok) break;
+
+      // ---- the item's end ----
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(FULL, l[i], 1);
+        l[i] += __shfl_xor_sync(FULL, l[i], 2);
+      }
+      const uint32_t blocks = w.blocks(), first = w.first_block();
+      const bool whole = blocks == 1;
+      if (w.kt0 == 0 && warp == 0)
+        for (uint32_t t = lane; t < ntok; t += 32)
+          p.desc[(uint64_t)(w.r.row0 + w.t + t) * a.pages.n_kv_heads + w.head] =
+              make_uint2(first, whole ? t : blocks << 16 | t);
+      float* const slot = p.slots + (uint64_t)(2 * blockIdx.x + (w.kt0 == 0 ? 1 : 0)) * S::BM * (HD + 2);
+      auto part = [&](uint32_t mrow, uint32_t r, uint32_t h) {
+        return whole ? p.rowpart + ((uint64_t)r * a.n_heads + h) * (HD + 2) : slot + mrow * (HD + 2);
+      };
+      const bool direct = whole && !p.joined;
+      if constexpr (WK > 1) {
+        // the warps of a row group join over shared memory
+        named_bar_sync(1, 32 * S::NW);  // the item before has been read
+        float* mine = join + warp * 16 * S::QP;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (t4 == 0) ml[warp][g + 8 * i][0] = m[i], ml[warp][g + 8 * i][1] = l[i];
+        if (busy) {
+#pragma unroll
+          for (int d = 0; d < OB; ++d) {
+            *reinterpret_cast<float2*>(mine + g * S::QP + 8 * d + 2 * t4) = make_float2(o[d][0], o[d][1]);
+            *reinterpret_cast<float2*>(mine + (g + 8) * S::QP + 8 * d + 2 * t4) = make_float2(o[d][2], o[d][3]);
+          }
+        }
+        named_bar_sync(1, 32 * S::NW);
+        for (uint32_t u = threadIdx.x; u < nrow * (HD / 4); u += 32 * S::NW) {
+          const uint32_t mr = u / (HD / 4), c = u % (HD / 4), w0 = mr / 16 * WK, rr = mr % 16;
+          float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+          for (int x = 0; x < WK; ++x) top = fmaxf(top, ml[w0 + x][rr][0]);
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int x = 0; x < WK; ++x) {
+            const float f = ex2(ml[w0 + x][rr][0] - (top == -INFINITY ? 0.0f : top));
+            const float4 v = *reinterpret_cast<const float4*>(join + ((w0 + x) * 16 + rr) * S::QP + 4 * c);
+            sum += f * ml[w0 + x][rr][1];
+            acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+          }
+          const uint32_t r = w.r.row0 + w.t + mr / p.group, h = w.head * p.group + mr % p.group;
+          if (direct) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            O* out = static_cast<O*>(a.out) + (uint64_t)r * a.out_stride + (uint64_t)h * HD + 4 * c;
+            if constexpr (sizeof(O) == 4)
+              *reinterpret_cast<float4*>(out) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            else
+              *reinterpret_cast<uint2*>(out) = make_uint2(pack2<O>(acc.x * inv, acc.y * inv), pack2<O>(acc.z * inv, acc.w * inv));
+            if (c == 0 && a.lse)
+              a.lse[(uint64_t)r * a.n_heads + h] = sum == 0.0f ? -INFINITY : (top - SHIFT + log2f(sum)) * LN2;
+          } else {
+            float* d = part(mr, r, h);
+            reinterpret_cast<float2*>(d + 4 * c)[0] = make_float2(acc.x, acc.y);
+            reinterpret_cast<float2*>(d + 4 * c)[1] = make_float2(acc.z, acc.w);
+            if (c == 0) d[HD] = top - SHIFT, d[HD + 1] = sum;
+          }
+        }
+      } else if (busy) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (!live[i]) continue;
+          if (direct) {
+            const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
+            O* out = static_cast<O*>(a.out) + (uint64_t)row[i] * a.out_stride + (uint64_t)head[i] * HD + 2 * t4;
+#pragma unroll
+            for (int d = 0; d < OB; ++d) {
+              const float x = o[d][2 * i] * inv, y = o[d][2 * i + 1] * inv;
+              if constexpr (sizeof(O) == 4) *reinterpret_cast<float2*>(out + 8 * d) = make_float2(x, y);
+              else *reinterpret_cast<uint32_t*>(out + 8 * d) = pack2<O>(x, y);
+            }
+            if (t4 == 0 && a.lse)
+              a.lse[(uint64_t)row[i] * a.n_heads + head[i]] =
+                  l[i] == 0.0f ? -INFINITY : (m[i] - SHIFT + log2f(l[i])) * LN2;
+          } else {
+            float* d0 = part(wm * 16 + g + 8 * i, row[i], head[i]);
+#pragma unroll
+            for (int d = 0; d < OB; ++d)
+              *reinterpret_cast<float2*>(d0 + 8 * d + 2 * t4) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+            if (t4 == 0) d0[HD] = m[i] - SHIFT, d0[HD + 1] = l[i];
+          }
+        }
+      }
+    } while (w.next());
+    if (!ok) {
+      abort_flag = 1;
+      if (lane == 0 && a.seqs.status) *a.seqs.status = STATUS_TIMEOUT;
+    }
+  }
   __syncthreads();
-  float top = -INFINITY, sum = 0.0f, f[4];
-  for (int w = 0; w < 4; ++w) top = fmaxf(top, part[w][HD]);
-  for (int w = 0; w < 4; ++w) {
-    f[w] = part[w][HD] == -INFINITY ? 0.0f : expf(part[w][HD] - top);
-    sum += f[w] * part[w][HD + 1];
+  grid_dep_wait();  // the launch before has ended when this one has
+}
+
+// ---- joining the parts -------------------------------------------------------
+struct JoinArgs {
+  PagedAttnArgs a;
+  uint32_t group, n_passes;
+  struct {
+    const uint2* desc;
+    const float* slots;
+    const float* rowpart;
+    uint32_t grid, bm;
+  } pass[2];
+  int joined;
+};
+
+// One warp per (row, query head): lanes hold HD/32 neighbours each.
+template <typename O, int HD>
+__global__ void __launch_bounds__(256) join_kernel(JoinArgs j) {
+  constexpr int PER = HD / 32;
+  const uint32_t lane = threadIdx.x & 31;
+  const uint64_t id = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const PagedAttnArgs& a = j.a;
+  const uint64_t row = id / a.n_heads;
+  const uint32_t head = (uint32_t)(id % a.n_heads);
+  grid_dep_wait();
+  if (row < row_begin(a.seqs, 0) || row >= row_begin(a.seqs, a.seqs.n_seqs)) return;
+  float m = -INFINITY, l = 0.0f, o[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) o[i] = 0.0f;
+  for (uint32_t ps = 0; ps < j.n_passes; ++ps) {
+    const uint2 d = j.pass[ps].desc[row * a.pages.n_kv_heads + head / j.group];
+    const uint32_t blocks = d.y >> 16, mr = (d.y & 0xFFFFu) * j.group + head % j.group;
+    uint32_t n = blocks ? blocks : 1;
+    if (!blocks && !j.joined) return;  // written by its one block
+    if (blocks && ((uint64_t)d.x + blocks > j.pass[ps].grid || mr >= j.pass[ps].bm)) return;
+    auto part = [&](uint32_t i) -> const float* {
+      if (!blocks) return j.pass[ps].rowpart + (row * a.n_heads + head) * (HD + 2);
+      const uint64_t slot = i == 0 ? 2ull * d.x + 1 : 2ull * (d.x + i);
+      return j.pass[ps].slots + (slot * j.pass[ps].bm + mr) * (HD + 2);
+    };
+    for (uint32_t i0 = 0; i0 < n; i0 += 32) {
+      const uint32_t c = min(32u, n - i0);
+      float pm = -INFINITY, pl = 0.0f;
+      if (lane < c) {
+        const float* q = part(i0 + lane);
+        pm = q[HD], pl = q[HD + 1];
+      }
+      const float top = fmaxf(m, warp_max(pm)), ref = top == -INFINITY ? 0.0f : top;
+      const float f0 = ex2(m - ref), f = ex2(pm - ref);
+      l = l * f0 + warp_sum(f * pl);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) o[i] *= f0;
+      m = top;
+#pragma unroll 4
+      for (uint32_t i = 0; i < c; ++i) {
+        const float fi = __shfl_sync(FULL, f, i);
+        const float2* q = reinterpret_cast<const float2*>(part(i0 + i) + PER * lane);
+#pragma unroll
+        for (int e = 0; e < PER / 2; ++e) {
+          const float2 v = q[e];
+          o[2 * e] += fi * v.x, o[2 * e + 1] += fi * v.y;
+        }
+      }
+    }
   }
-  for (uint32_t d = threadIdx.x; d < HD; d += 128) {
-    float v = 0.0f;
-    for (int w = 0; w < 4; ++w) v += f[w] * part[w][d];
-    static_cast<O*>(a.out)[(uint64_t)row * a.out_stride + (uint64_t)head * HD + d] =
-        from_f32<O>(keys ? v / sum : 0.0f);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  O* out = static_cast<O*>(a.out) + row * a.out_stride + (uint64_t)head * HD + PER * lane;
+#pragma unroll
+  for (int e = 0; e < PER / 2; ++e) {
+    const float x = o[2 * e] * inv, y = o[2 * e + 1] * inv;
+    if constexpr (sizeof(O) == 4) reinterpret_cast<float2*>(out)[e] = make_float2(x, y);
+    else reinterpret_cast<uint32_t*>(out)[e] = pack2<O>(x, y);
   }
-  if (threadIdx.x == 0 && a.lse)
-    a.lse[(uint64_t)row * a.n_heads + head] = keys ? top + logf(sum) : -INFINITY;
+  if (lane == 0 && a.lse) a.lse[row * a.n_heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
+// ---- host --------------------------------------------------------------------
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(p);
+  }();
+  return fn;
+}
+
+// (element, head, token, page), boxes of 128 bytes x 1 x `tokens` x 1, swizzled.
+bool encode_pages(CUtensorMap* m, const Pages& p, void* base, int dtype, uint32_t tokens) {
+  const EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const uint64_t size = dtype == DT_F32 ? 4 : 2, ps = 1ull << p.page_shift;
+  const cuuint64_t dims[4] = {p.head_size, p.n_kv_heads, ps, p.n_pages};
+  // an axis of one entry has no stride to speak of
+  auto bytes = [&](uint64_t stride, uint64_t n) { return (n > 1 ? stride : p.head_size) * size; };
+  const cuuint64_t strides[3] = {bytes(p.head_stride, p.n_kv_heads), bytes(p.token_stride, ps),
+                                 bytes(p.page_stride, p.n_pages)};
+  const cuuint32_t box[4] = {(cuuint32_t)(128 / size), 1, tokens, 1}, estr[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType t = dtype == DT_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                : dtype == DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return fn(m, t, 4, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr uint32_t BLOCKS = 2 * 148;  // two on every SM
+
+// Rows of a tile (16, 32 or 64) for items of `rows` rows.
+uint32_t tile_rows(uint64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
+// What a call launches, by its counts alone.
+struct Plan {
+  bool shared;        // a prefix pass of its own
+  uint32_t bm[2];     // row tiles of the sequences' pass, and of the prefix pass
+  uint64_t desc[2], slots[2], rowpart[2], bytes;  // workspace offsets
+};
+Plan plan_of(const Pages& p, const Seqs& s, uint32_t n_heads) {
+  const uint64_t group = n_heads / p.n_kv_heads, hd = p.head_size;
+  const uint64_t each = ((uint64_t)s.n_rows + s.n_seqs - 1) / s.n_seqs * group;
+  Plan pl{};
+  // Reading the prefix once pays where an item has few rows; items of many
+  // rows (prompts) read it a few times from L2, without parts to be joined.
+  pl.shared = s.shared_len && s.n_seqs > 1 && each <= 32;
+  pl.bm[0] = tile_rows(each);
+  pl.bm[1] = tile_rows((uint64_t)s.n_rows * group);
+  uint64_t at = 0;
+  auto take = [&](uint64_t n) {
+    const uint64_t o = at;
+    at = (at + n + 255) / 256 * 256;
+    return o;
+  };
+  for (int i = 0; i < (pl.shared ? 2 : 1); ++i) {
+    pl.desc[i] = take((uint64_t)s.n_rows * p.n_kv_heads * 8);
+    pl.slots[i] = take(2ull * BLOCKS * pl.bm[i] * (hd + 2) * 4);
+    pl.rowpart[i] = pl.shared ? take((uint64_t)s.n_rows * n_heads * (hd + 2) * 4) : 0;
+  }
+  pl.bytes = at;
+  return pl;
+}
+
+template <typename T, typename O, int HD, int WM, int WK>
+cudaError_t launch_pass(const CUtensorMap& mk, const CUtensorMap& mv, const Pass& p, const LaunchCfg& lc) {
+  using S = Shape<T, HD, WM, WK>;
+  static std::atomic<uint64_t> ready{0};  // one bit per device: the attribute is set
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(ready.load(std::memory_order_relaxed) & bit) || dev > 63) {
+    e = cudaFuncSetAttribute(attend_kernel<T, O, HD, WM, WK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)S::SMEM);
+    if (e != cudaSuccess) return e;
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  return launch_kernel(attend_kernel<T, O, HD, WM, WK>, dim3(BLOCKS), dim3(S::THREADS), S::SMEM, lc, mk, mv, p);
+}
+
+template <typename T, typename O, int HD>
+cudaError_t launch(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
+  constexpr uint32_t KT = BUF / (HD * sizeof(T));
+  const Plan pl = plan_of(a.pages, a.seqs, a.n_heads);
+  const uint32_t ps = 1u << a.pages.page_shift, tokens = ps < KT ? ps : KT;
+  CUtensorMap mk, mv;
+  if (!encode_pages(&mk, a.pages, a.pages.k, dtype, tokens) || !encode_pages(&mv, a.pages, a.pages.v, dtype, tokens))
+    return cudaErrorInvalidValue;
+  uint8_t* ws = static_cast<uint8_t*>(a.workspace);
+  JoinArgs j{};
+  j.a = a;
+  j.group = a.n_heads / a.pages.n_kv_heads;
+  j.n_passes = pl.shared ? 2 : 1;
+  j.joined = pl.shared;
+  LaunchCfg lc;
+  lc.stream = stream;
+  for (int i = pl.shared ? 1 : 0; i >= 0; --i) {  // the prefix first
+    Pass p{};
+    p.a = a;
+    p.prefix = i;
+    p.from = pl.shared && !i ? a.seqs.shared_len : 0;
+    p.group = j.group;
+    p.min_chunk = 2;
+    p.joined = pl.shared;
+    p.desc = reinterpret_cast<uint2*>(ws + pl.desc[i]);
+    p.slots = reinterpret_cast<float*>(ws + pl.slots[i]);
+    p.rowpart = reinterpret_cast<float*>(ws + pl.rowpart[i]);
+    j.pass[i].desc = p.desc;
+    j.pass[i].slots = p.slots;
+    j.pass[i].rowpart = p.rowpart;
+    j.pass[i].grid = BLOCKS;
+    j.pass[i].bm = pl.bm[i];
+    const cudaError_t e = pl.bm[i] == 16   ? launch_pass<T, O, HD, 1, 4>(mk, mv, p, lc)
+                          : pl.bm[i] == 32 ? launch_pass<T, O, HD, 2, 2>(mk, mv, p, lc)
+                                           : launch_pass<T, O, HD, 4, 1>(mk, mv, p, lc);
+    if (e != cudaSuccess) return e;
+    lc.pdl = true;
+  }
+  const uint64_t warps = (uint64_t)a.seqs.n_rows * a.n_heads;
+  return launch_kernel(join_kernel<O, HD>, dim3((uint32_t)((warps + 7) / 8)), dim3(256), 0, lc, j);
 }
 
 template <typename T, typename O>
-cudaError_t launch(const PagedAttnArgs& a, cudaStream_t stream) {
-  const dim3 grid(a.seqs.n_rows, a.n_heads);
-  LaunchCfg lc;
-  lc.stream = stream;
-  return a.pages.head_size == 128 ? launch_kernel(attend_kernel<T, O, 128>, grid, dim3(128), 0, lc, a)
-                                  : launch_kernel(attend_kernel<T, O, 64>, grid, dim3(128), 0, lc, a);
+cudaError_t launch_hd(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
+  return a.pages.head_size == 128 ? launch<T, O, 128>(a, dtype, stream) : launch<T, O, 64>(a, dtype, stream);
 }
 
 }  // namespace
 
 cudaError_t paged_attention(const PagedAttnArgs& a, int dtype, bool out_f32, cudaStream_t stream) {
-  if (dtype == DT_F32) return launch<float, float>(a, stream);
-  if (dtype == DT_F16) return out_f32 ? launch<__half, float>(a, stream) : launch<__half, __half>(a, stream);
-  return out_f32 ? launch<__nv_bfloat16, float>(a, stream) : launch<__nv_bfloat16, __nv_bfloat16>(a, stream);
+  if (dtype == DT_F32) return launch_hd<float, float>(a, dtype, stream);
+  if (dtype == DT_F16)
+    return out_f32 ? launch_hd<__half, float>(a, dtype, stream) : launch_hd<__half, __half>(a, dtype, stream);
+  return out_f32 ? launch_hd<__nv_bfloat16, float>(a, dtype, stream)
+                 : launch_hd<__nv_bfloat16, __nv_bfloat16>(a, dtype, stream);
 }
 
-uint64_t paged_attention_workspace(const Pages&, const Seqs&, int, uint32_t) { return 256; }
+uint64_t paged_attention_workspace(const Pages& p, const Seqs& s, int, uint32_t n_heads) {
+  const Plan pl = plan_of(p, s, n_heads);
+  return pl.bytes > 256 ? pl.bytes : 256;
+}
 
 }  // namespace k
 }  // namespace yl
