@@ -32,12 +32,7 @@
 // rounded to their type for the second product (the sum l takes them
 // unrounded), f16 weights at 2^10 times their value so that small ones do not
 // fall below f16's range.
-#include <cuda.h>
-
-#include <atomic>
-#include <type_traits>
-
-#include "serve.cuh"
+#include "paged_attention.cuh"
 
 namespace yl {
 namespace k {
@@ -46,21 +41,6 @@ using namespace yl::dev;
 namespace {
 
 constexpr uint32_t BUF = 16384;  // bytes of a key or value tile
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr int STATUS_TIMEOUT = -7;  // YL_ERR_TIMEOUT
-
-// One launch: over the sequences' own keys (from `from` on), or over the
-// shared prefix with all rows as one sequence.
-struct Pass {
-  PagedAttnArgs a;
-  uint32_t from, prefix;  // first key; 1: the prefix pass (keys 0 .. shared_len)
-  uint32_t group, min_chunk;
-  int joined;      // every item leaves its part in the workspace
-  uint2* desc;     // [n_rows][n_kv_heads] {first block, blocks << 16 | token in the tile}
-  float* slots;    // [2 * grid][BM][HD + 2]
-  float* rowpart;  // [n_rows][n_heads][HD + 2]: items of one block, where every item leaves its part
-};
-
 template <typename T, int HD, int WM_, int WK_>
 struct Shape {
   static constexpr int WM = WM_, WK = WK_, NW = WM * WK, THREADS = 32 * (NW + 1);
@@ -120,218 +100,10 @@ __device__ __forceinline__ float lds(uint32_t addr) {
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
   return v;
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// 4-D tiled load of a page's part: (element, head, token in the page, page).
-__device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t head, uint32_t tok,
-                                         uint32_t page, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-      "[%6];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(tok), "r"(page), "r"(smem_u32(bar))
-      : "memory");
-}
-__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // Byte of 16-byte column c of row `key` in a tile.
 template <typename S>
 __device__ __forceinline__ uint32_t at(uint32_t key, uint32_t c) {
   return (c >> 3) * (S::KT * 128) + key * 128 + (((c & 7) ^ (key & 7)) << 4);
-}
-
-// ---- work ------------------------------------------------------------------
-// A sequence as a pass sees it.
-struct Rows {
-  uint32_t row0, n;  // its rows
-  int64_t pos0;      // position of the first
-  uint32_t limit;    // keys that may be read: the prefix, or what the page table has slots for
-};
-__device__ __forceinline__ Rows rows_of(const Pass& p, uint32_t i) {
-  const Seqs& s = p.a.seqs;
-  Rows r;
-  if (p.prefix) {
-    r.row0 = row_begin(s, 0);
-    const uint32_t e = row_begin(s, s.n_seqs);
-    r.n = e > r.row0 ? e - r.row0 : 0;
-    r.pos0 = 0;
-    r.limit = s.shared_len;
-  } else {
-    r.row0 = row_begin(s, i);
-    r.n = row_end(s, i) - r.row0;
-    r.pos0 = (int64_t)s.seq_len[i] - r.n;
-    r.limit = table_limit(s, p.a.pages);
-  }
-  return r;
-}
-// First key behind those that tokens [.., t) of the sequence see.
-__device__ __forceinline__ uint32_t keys_end(const Pass& p, const Rows& r, uint32_t t) {
-  if (p.prefix) return r.limit;
-  const int64_t e = r.pos0 + (t < r.n ? t : r.n);
-  return e <= 0 ? 0 : e < (int64_t)r.limit ? (uint32_t)e : r.limit;
-}
-// Key tiles of the row tile that ends at token t (one where it sees no key).
-template <typename S>
-__device__ __forceinline__ uint32_t tiles_of(const Pass& p, const Rows& r, uint32_t t) {
-  const uint32_t e = keys_end(p, r, t);
-  return e > p.from + S::KT ? (e - p.from + S::KT - 1) / S::KT : 1;
-}
-template <typename S>
-__device__ __forceinline__ uint64_t tiles_per_head(const Pass& p, const Rows& r, uint32_t tpt) {
-  uint64_t n = 0;
-  if (p.prefix) return (uint64_t)((r.n + tpt - 1) / tpt) * tiles_of<S>(p, r, r.n);
-  for (uint32_t t = 0; t < r.n; t += tpt) n += tiles_of<S>(p, r, t + tpt);
-  return n;
-}
-
-// Where a block's piece of the line begins.
-struct Start {
-  uint64_t begin, end, chunk;  // in key tiles
-  uint32_t seq, head, t, kt;   // sequence, head, first token of the row tile, key tile
-  uint64_t g0;                 // where the item begins on the line
-  int masked;                  // prefix pass: some row does not see all of the prefix
-};
-
-template <typename S>
-__device__ void find_start(const Pass& p, uint32_t tpt, Start* out, uint64_t* scratch) {
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t n = p.prefix ? 1 : p.a.seqs.n_seqs;
-  const uint32_t heads = p.a.pages.n_kv_heads;
-  constexpr uint32_t NWARPS = S::THREADS / 32;
-  __shared__ int any_masked;
-  if (tid == 0) any_masked = 0, out->seq = 0xFFFFFFFFu;
-  __syncthreads();
-  if (p.prefix) {  // rows inside the prefix
-    bool m = false;
-    for (uint32_t i = tid; i < p.a.seqs.n_seqs; i += S::THREADS) {
-      const uint32_t rn = row_end(p.a.seqs, i) - row_begin(p.a.seqs, i);
-      m |= rn && (int64_t)p.a.seqs.seq_len[i] - rn + 1 < (int64_t)p.a.seqs.shared_len;
-    }
-    if (m) any_masked = 1;
-  }
-  // exclusive sums of the sequences' tiles, a block's width at a time; the
-  // second time over, the piece's place is looked for
-  uint64_t total = 0, begin = 0;
-  for (int round = 0; round < 2; ++round) {
-    uint64_t base = 0;
-    for (uint32_t c = 0; c < n; c += S::THREADS) {
-      const uint32_t i = c + tid;
-      Rows r{};
-      uint64_t per_head = 0;
-      if (i < n) {
-        r = rows_of(p, i);
-        per_head = tiles_per_head<S>(p, r, tpt);
-      }
-      const uint64_t mine = per_head * heads;
-      uint64_t inc = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t v = __shfl_up_sync(FULL, inc, o);
-        if ((int)lane >= o) inc += v;
-      }
-      __syncthreads();
-      if (lane == 31) scratch[warp] = inc;
-      __syncthreads();
-      uint64_t before = base, sum = 0;
-      for (uint32_t w = 0; w < NWARPS; ++w) {
-        if (w < warp) before += scratch[w];
-        sum += scratch[w];
-      }
-      const uint64_t first = before + inc - mine;
-      if (round == 1 && begin >= first && begin < first + mine) {
-        uint64_t off = begin - first, g0 = first;
-        const uint64_t h = off / per_head;
-        off -= h * per_head;
-        g0 += h * per_head;
-        uint32_t t = 0, nt = tiles_of<S>(p, r, tpt);
-        while (off >= nt) {
-          off -= nt;
-          g0 += nt;
-          t += tpt;
-          nt = tiles_of<S>(p, r, t + tpt);
-        }
-        out->seq = i;
-        out->head = (uint32_t)h;
-        out->t = t;
-        out->kt = (uint32_t)off;
-        out->g0 = g0;
-      }
-      base += sum;
-    }
-    if (round == 0) {
-      total = base;
-      uint64_t chunk = (total + gridDim.x - 1) / gridDim.x;
-      if (chunk < p.min_chunk) chunk = p.min_chunk;
-      begin = chunk * blockIdx.x;
-      if (tid == 0) {
-        out->chunk = chunk;
-        out->begin = begin;
-        out->end = begin + chunk < total ? begin + chunk : total;
-      }
-      if (begin >= total) break;  // nothing for this block: seq stays unset
-    }
-  }
-  __syncthreads();
-  if (tid == 0) out->masked = any_masked;
-  __syncthreads();
-}
-
-// Walks a block's piece: one step per item, the same in every warp.
-template <typename S>
-struct Walk {
-  const Pass& p;
-  const uint32_t tpt;
-  uint64_t at, end, chunk, g0;
-  uint32_t seq, head, t, kt0, kt1, nt;
-  Rows r;
-
-  __device__ Walk(const Pass& pass, uint32_t tokens, const Start& s)
-      : p(pass), tpt(tokens), at(s.begin), end(s.end), chunk(s.chunk), g0(s.g0), seq(s.seq), head(s.head), t(s.t),
-        kt0(s.kt) {
-    r = rows_of(p, seq);
-    piece();
-  }
-  __device__ void piece() {
-    nt = tiles_of<S>(p, r, t + tpt);
-    const uint64_t left = end - at;
-    kt1 = nt - kt0 < left ? nt : kt0 + (uint32_t)left;
-  }
-  __device__ bool next() {
-    at += kt1 - kt0;
-    if (at >= end) return false;
-    g0 += nt;
-    kt0 = 0;
-    t += tpt;
-    if (t >= r.n) {
-      t = 0;
-      if (++head == p.a.pages.n_kv_heads) {
-        head = 0;
-        do {
-          if (++seq >= p.a.seqs.n_seqs || p.prefix) return false;
-          r = rows_of(p, seq);
-        } while (r.n == 0);
-      }
-    }
-    piece();
-    return true;
-  }
-  __device__ uint32_t tokens() const { return r.n - t < tpt ? r.n - t : tpt; }
-  __device__ uint32_t kend() const { return keys_end(p, r, t + tpt); }
-  // Whole in one block, or the blocks it lies in.
-  __device__ uint32_t first_block() const { return (uint32_t)(g0 / chunk); }
-  __device__ uint32_t blocks() const { return (uint32_t)((g0 + nt - 1) / chunk) - first_block() + 1; }
-};
-
-// Sequence of a row by bisection (rows inside the prefix only).
-__device__ uint32_t find_seq(const Seqs& s, uint32_t row) {
-  uint32_t lo = 0, hi = s.n_seqs;
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (row_begin(s, mid) <= row) lo = mid;
-    else hi = mid;
-  }
-  return lo;
 }
 
 template <typename T, typename O, int HD, int WM, int WK>
@@ -644,9 +416,9 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
         for (uint32_t t = lane; t < ntok; t += 32)
           p.desc[(uint64_t)(w.r.row0 + w.t + t) * a.pages.n_kv_heads + w.head] =
               make_uint2(first, whole ? t : blocks << 16 | t);
-      float* const slot = p.slots + (uint64_t)(2 * blockIdx.x + (w.kt0 == 0 ? 1 : 0)) * S::BM * (HD + 2);
+      float* const slot = p.slots + (uint64_t)(2 * blockIdx.x + (w.kt0 == 0 ? 1 : 0)) * S::BM * PART<HD>;
       auto part = [&](uint32_t mrow, uint32_t r, uint32_t h) {
-        return whole ? p.rowpart + ((uint64_t)r * a.n_heads + h) * (HD + 2) : slot + mrow * (HD + 2);
+        return whole ? p.rowpart + ((uint64_t)r * a.n_heads + h) * PART<HD> : slot + mrow * PART<HD>;
       };
       const bool direct = whole && !p.joined;
       if constexpr (WK > 1) {
@@ -763,9 +535,9 @@ __global__ void __launch_bounds__(256) join_kernel(JoinArgs j) {
     if (!blocks && !j.joined) return;  // written by its one block
     if (blocks && ((uint64_t)d.x + blocks > j.pass[ps].grid || mr >= j.pass[ps].bm)) return;
     auto part = [&](uint32_t i) -> const float* {
-      if (!blocks) return j.pass[ps].rowpart + (row * a.n_heads + head) * (HD + 2);
+      if (!blocks) return j.pass[ps].rowpart + (row * a.n_heads + head) * PART<HD>;
       const uint64_t slot = i == 0 ? 2ull * d.x + 1 : 2ull * (d.x + i);
-      return j.pass[ps].slots + (slot * j.pass[ps].bm + mr) * (HD + 2);
+      return j.pass[ps].slots + (slot * j.pass[ps].bm + mr) * PART<HD>;
     };
     for (uint32_t i0 = 0; i0 < n; i0 += 32) {
       const uint32_t c = min(32u, n - i0);
@@ -804,43 +576,12 @@ __global__ void __launch_bounds__(256) join_kernel(JoinArgs j) {
 }
 
 // ---- host --------------------------------------------------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return reinterpret_cast<EncodeTiledFn>(p);
-  }();
-  return fn;
+// Row tile for items of `rows` rows.
+uint32_t tile_rows(uint64_t rows, int dtype) {
+  if (dtype != DT_F32 && rows > 32) return TC_TILE;
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
-
-// (element, head, token, page), boxes of 128 bytes x 1 x `tokens` x 1, swizzled.
-bool encode_pages(CUtensorMap* m, const Pages& p, void* base, int dtype, uint32_t tokens) {
-  const EncodeTiledFn fn = encode_fn();
-  if (!fn) return false;
-  const uint64_t size = dtype == DT_F32 ? 4 : 2, ps = 1ull << p.page_shift;
-  const cuuint64_t dims[4] = {p.head_size, p.n_kv_heads, ps, p.n_pages};
-  // an axis of one entry has no stride to speak of
-  auto bytes = [&](uint64_t stride, uint64_t n) { return (n > 1 ? stride : p.head_size) * size; };
-  const cuuint64_t strides[3] = {bytes(p.head_stride, p.n_kv_heads), bytes(p.token_stride, ps),
-                                 bytes(p.page_stride, p.n_pages)};
-  const cuuint32_t box[4] = {(cuuint32_t)(128 / size), 1, tokens, 1}, estr[4] = {1, 1, 1, 1};
-  const CUtensorMapDataType t = dtype == DT_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                : dtype == DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  return fn(m, t, 4, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-constexpr uint32_t BLOCKS = 2 * 148;  // two on every SM
-
-// Rows of a tile (16, 32 or 64) for items of `rows` rows.
-uint32_t tile_rows(uint64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+uint32_t blocks_of(uint32_t bm) { return bm == TC_TILE ? 148 : 2 * 148; }
 
 // What a call launches, by its counts alone.
 struct Plan {
@@ -848,15 +589,15 @@ struct Plan {
   uint32_t bm[2];     // row tiles of the sequences' pass, and of the prefix pass
   uint64_t desc[2], slots[2], rowpart[2], bytes;  // workspace offsets
 };
-Plan plan_of(const Pages& p, const Seqs& s, uint32_t n_heads) {
+Plan plan_of(const Pages& p, const Seqs& s, int dtype, uint32_t n_heads) {
   const uint64_t group = n_heads / p.n_kv_heads, hd = p.head_size;
   const uint64_t each = ((uint64_t)s.n_rows + s.n_seqs - 1) / s.n_seqs * group;
   Plan pl{};
   // Reading the prefix once pays where an item has few rows; items of many
   // rows (prompts) read it a few times from L2, without parts to be joined.
   pl.shared = s.shared_len && s.n_seqs > 1 && each <= 32;
-  pl.bm[0] = tile_rows(each);
-  pl.bm[1] = tile_rows((uint64_t)s.n_rows * group);
+  pl.bm[0] = tile_rows(each, dtype);
+  pl.bm[1] = tile_rows((uint64_t)s.n_rows * group, dtype);
   uint64_t at = 0;
   auto take = [&](uint64_t n) {
     const uint64_t o = at;
@@ -865,8 +606,8 @@ Plan plan_of(const Pages& p, const Seqs& s, uint32_t n_heads) {
   };
   for (int i = 0; i < (pl.shared ? 2 : 1); ++i) {
     pl.desc[i] = take((uint64_t)s.n_rows * p.n_kv_heads * 8);
-    pl.slots[i] = take(2ull * BLOCKS * pl.bm[i] * (hd + 2) * 4);
-    pl.rowpart[i] = pl.shared ? take((uint64_t)s.n_rows * n_heads * (hd + 2) * 4) : 0;
+    pl.slots[i] = take(2ull * blocks_of(pl.bm[i]) * pl.bm[i] * (hd + 4) * 4);
+    pl.rowpart[i] = pl.shared ? take((uint64_t)s.n_rows * n_heads * (hd + 4) * 4) : 0;
   }
   pl.bytes = at;
   return pl;
@@ -875,24 +616,16 @@ Plan plan_of(const Pages& p, const Seqs& s, uint32_t n_heads) {
 template <typename T, typename O, int HD, int WM, int WK>
 cudaError_t launch_pass(const CUtensorMap& mk, const CUtensorMap& mv, const Pass& p, const LaunchCfg& lc) {
   using S = Shape<T, HD, WM, WK>;
-  static std::atomic<uint64_t> ready{0};  // one bit per device: the attribute is set
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  static std::atomic<uint64_t> ready{0};
+  const cudaError_t e = allow_smem(ready, attend_kernel<T, O, HD, WM, WK>, S::SMEM);
   if (e != cudaSuccess) return e;
-  const uint64_t bit = 1ull << (dev & 63);
-  if (!(ready.load(std::memory_order_relaxed) & bit) || dev > 63) {
-    e = cudaFuncSetAttribute(attend_kernel<T, O, HD, WM, WK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)S::SMEM);
-    if (e != cudaSuccess) return e;
-    ready.fetch_or(bit, std::memory_order_relaxed);
-  }
-  return launch_kernel(attend_kernel<T, O, HD, WM, WK>, dim3(BLOCKS), dim3(S::THREADS), S::SMEM, lc, mk, mv, p);
+  return launch_kernel(attend_kernel<T, O, HD, WM, WK>, dim3(p.grid), dim3(S::THREADS), S::SMEM, lc, mk, mv, p);
 }
 
 template <typename T, typename O, int HD>
 cudaError_t launch(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
   constexpr uint32_t KT = BUF / (HD * sizeof(T));
-  const Plan pl = plan_of(a.pages, a.seqs, a.n_heads);
+  const Plan pl = plan_of(a.pages, a.seqs, dtype, a.n_heads);
   const uint32_t ps = 1u << a.pages.page_shift, tokens = ps < KT ? ps : KT;
   CUtensorMap mk, mv;
   if (!encode_pages(&mk, a.pages, a.pages.k, dtype, tokens) || !encode_pages(&mv, a.pages, a.pages.v, dtype, tokens))
@@ -908,6 +641,8 @@ cudaError_t launch(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
   for (int i = pl.shared ? 1 : 0; i >= 0; --i) {  // the prefix first
     Pass p{};
     p.a = a;
+    p.dtype = dtype;
+    p.grid = blocks_of(pl.bm[i]);
     p.prefix = i;
     p.from = pl.shared && !i ? a.seqs.shared_len : 0;
     p.group = j.group;
@@ -919,10 +654,11 @@ cudaError_t launch(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
     j.pass[i].desc = p.desc;
     j.pass[i].slots = p.slots;
     j.pass[i].rowpart = p.rowpart;
-    j.pass[i].grid = BLOCKS;
+    j.pass[i].grid = p.grid;
     j.pass[i].bm = pl.bm[i];
     const cudaError_t e = pl.bm[i] == 16   ? launch_pass<T, O, HD, 1, 4>(mk, mv, p, lc)
                           : pl.bm[i] == 32 ? launch_pass<T, O, HD, 2, 2>(mk, mv, p, lc)
+                          : pl.bm[i] == TC_TILE ? attend_tc(p, sizeof(O) == 4, lc)
                                            : launch_pass<T, O, HD, 4, 1>(mk, mv, p, lc);
     if (e != cudaSuccess) return e;
     lc.pdl = true;
@@ -946,8 +682,8 @@ cudaError_t paged_attention(const PagedAttnArgs& a, int dtype, bool out_f32, cud
                  : launch_hd<__nv_bfloat16, __nv_bfloat16>(a, dtype, stream);
 }
 
-uint64_t paged_attention_workspace(const Pages& p, const Seqs& s, int, uint32_t n_heads) {
-  const Plan pl = plan_of(p, s, n_heads);
+uint64_t paged_attention_workspace(const Pages& p, const Seqs& s, int dtype, uint32_t n_heads) {
+  const Plan pl = plan_of(p, s, dtype, n_heads);
   return pl.bytes > 256 ? pl.bytes : 256;
 }
 

@@ -1,0 +1,283 @@
+// What the paged-attention kernels share: how a call's work is laid out on a
+// line and cut into pieces (paged_attention.cu tells why), and the page loads.
+#pragma once
+#include <atomic>
+#include <type_traits>
+
+#include "serve.cuh"
+#include "tc.cuh"
+
+namespace yl {
+namespace k {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int STATUS_TIMEOUT = -7;  // YL_ERR_TIMEOUT
+
+// One launch: over the sequences' own keys (from `from` on), or over the
+// shared prefix with all rows as one sequence.
+struct Pass {
+  PagedAttnArgs a;
+  int dtype;
+  uint32_t from, prefix;  // first key; 1: the prefix pass (keys 0 .. shared_len)
+  uint32_t group, min_chunk;
+  uint32_t grid;   // blocks
+  int joined;      // every item leaves its part in the workspace
+  uint2* desc;     // [n_rows][n_kv_heads] {first block, blocks << 16 | token in the tile}
+  float* slots;    // [2 * grid][BM][HD + 4]: a part is O, m (in powers of two), l
+  float* rowpart;  // [n_rows][n_heads][HD + 4]: items of one block, where every item leaves its part
+};
+
+template <int HD>
+constexpr uint32_t PART = HD + 4;  // floats of a part, a multiple of 16 bytes
+constexpr uint32_t TC_TILE = 256;  // rows of an item of attend_tc
+
+// The pass on the 5th-generation tensor cores: items of up to TC_TILE rows,
+// 16-bit types, one block per SM (paged_attention_tc.cu).
+cudaError_t attend_tc(const Pass& p, bool out_f32, const LaunchCfg& lc);
+
+// Sets a kernel's dynamic shared memory once per device.
+template <typename F>
+cudaError_t allow_smem(std::atomic<uint64_t>& ready, F* kernel, uint32_t bytes) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (ready.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
+namespace {
+using namespace yl::dev;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 4-D tiled load of a page's part: (element, head, token in the page, page).
+__device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t head, uint32_t tok,
+                                         uint32_t page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(tok), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// ---- work ------------------------------------------------------------------
+// A sequence as a pass sees it.
+struct Rows {
+  uint32_t row0, n;  // its rows
+  int64_t pos0;      // position of the first
+  uint32_t limit;    // keys that may be read: the prefix, or what the page table has slots for
+};
+__device__ __forceinline__ Rows rows_of(const Pass& p, uint32_t i) {
+  const Seqs& s = p.a.seqs;
+  Rows r;
+  if (p.prefix) {
+    r.row0 = row_begin(s, 0);
+    const uint32_t e = row_begin(s, s.n_seqs);
+    r.n = e > r.row0 ? e - r.row0 : 0;
+    r.pos0 = 0;
+    r.limit = s.shared_len;
+  } else {
+    r.row0 = row_begin(s, i);
+    r.n = row_end(s, i) - r.row0;
+    r.pos0 = (int64_t)s.seq_len[i] - r.n;
+    r.limit = table_limit(s, p.a.pages);
+  }
+  return r;
+}
+// First key behind those that tokens [.., t) of the sequence see.
+__device__ __forceinline__ uint32_t keys_end(const Pass& p, const Rows& r, uint32_t t) {
+  if (p.prefix) return r.limit;
+  const int64_t e = r.pos0 + (t < r.n ? t : r.n);
+  return e <= 0 ? 0 : e < (int64_t)r.limit ? (uint32_t)e : r.limit;
+}
+// Key tiles of the row tile that ends at token t (one where it sees no key).
+template <typename S>
+__device__ __forceinline__ uint32_t tiles_of(const Pass& p, const Rows& r, uint32_t t) {
+  const uint32_t e = keys_end(p, r, t);
+  return e > p.from + S::KT ? (e - p.from + S::KT - 1) / S::KT : 1;
+}
+template <typename S>
+__device__ __forceinline__ uint64_t tiles_per_head(const Pass& p, const Rows& r, uint32_t tpt) {
+  uint64_t n = 0;
+  if (p.prefix) return (uint64_t)((r.n + tpt - 1) / tpt) * tiles_of<S>(p, r, r.n);
+  for (uint32_t t = 0; t < r.n; t += tpt) n += tiles_of<S>(p, r, t + tpt);
+  return n;
+}
+
+// Where a block's piece of the line begins.
+struct Start {
+  uint64_t begin, end, chunk;  // in key tiles
+  uint32_t seq, head, t, kt;   // sequence, head, first token of the row tile, key tile
+  uint64_t g0;                 // where the item begins on the line
+  int masked;                  // prefix pass: some row does not see all of the prefix
+};
+
+template <typename S>
+__device__ void find_start(const Pass& p, uint32_t tpt, Start* out, uint64_t* scratch) {
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t n = p.prefix ? 1 : p.a.seqs.n_seqs;
+  const uint32_t heads = p.a.pages.n_kv_heads;
+  constexpr uint32_t NWARPS = S::THREADS / 32;
+  __shared__ int any_masked;
+  if (tid == 0) any_masked = 0, out->seq = 0xFFFFFFFFu;
+  __syncthreads();
+  if (p.prefix) {  // rows inside the prefix
+    bool m = false;
+    for (uint32_t i = tid; i < p.a.seqs.n_seqs; i += S::THREADS) {
+      const uint32_t rn = row_end(p.a.seqs, i) - row_begin(p.a.seqs, i);
+      m |= rn && (int64_t)p.a.seqs.seq_len[i] - rn + 1 < (int64_t)p.a.seqs.shared_len;
+    }
+    if (m) any_masked = 1;
+  }
+  // exclusive sums of the sequences' tiles, a block's width at a time; the
+  // second time over, the piece's place is looked for
+  uint64_t total = 0, begin = 0;
+  for (int round = 0; round < 2; ++round) {
+    uint64_t base = 0;
+    for (uint32_t c = 0; c < n; c += S::THREADS) {
+      const uint32_t i = c + tid;
+      Rows r{};
+      uint64_t per_head = 0;
+      if (i < n) {
+        r = rows_of(p, i);
+        per_head = tiles_per_head<S>(p, r, tpt);
+      }
+      const uint64_t mine = per_head * heads;
+      uint64_t inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t v = __shfl_up_sync(FULL, inc, o);
+        if ((int)lane >= o) inc += v;
+      }
+      __syncthreads();
+      if (lane == 31) scratch[warp] = inc;
+      __syncthreads();
+      uint64_t before = base, sum = 0;
+      for (uint32_t w = 0; w < NWARPS; ++w) {
+        if (w < warp) before += scratch[w];
+        sum += scratch[w];
+      }
+      const uint64_t first = before + inc - mine;
+      if (round == 1 && begin >= first && begin < first + mine) {
+        uint64_t off = begin - first, g0 = first;
+        const uint64_t h = off / per_head;
+        off -= h * per_head;
+        g0 += h * per_head;
+        uint32_t t = 0, nt = tiles_of<S>(p, r, tpt);
+        while (off >= nt) {
+          off -= nt;
+          g0 += nt;
+          t += tpt;
+          nt = tiles_of<S>(p, r, t + tpt);
+        }
+        out->seq = i;
+        out->head = (uint32_t)h;
+        out->t = t;
+        out->kt = (uint32_t)off;
+        out->g0 = g0;
+      }
+      base += sum;
+    }
+    if (round == 0) {
+      total = base;
+      uint64_t chunk = (total + gridDim.x - 1) / gridDim.x;
+      if (chunk < p.min_chunk) chunk = p.min_chunk;
+      begin = chunk * blockIdx.x;
+      if (tid == 0) {
+        out->chunk = chunk;
+        out->begin = begin;
+        out->end = begin + chunk < total ? begin + chunk : total;
+      }
+      if (begin >= total) break;  // nothing for this block: seq stays unset
+    }
+  }
+  __syncthreads();
+  if (tid == 0) out->masked = any_masked;
+  __syncthreads();
+}
+
+// Walks a block's piece: one step per item, the same in every warp.
+template <typename S>
+struct Walk {
+  const Pass& p;
+  const uint32_t tpt;
+  uint64_t at, end, chunk, g0;
+  uint32_t seq, head, t, kt0, kt1, nt;
+  Rows r;
+
+  __device__ Walk(const Pass& pass, uint32_t tokens, const Start& s)
+      : p(pass), tpt(tokens), at(s.begin), end(s.end), chunk(s.chunk), g0(s.g0), seq(s.seq), head(s.head), t(s.t),
+        kt0(s.kt) {
+    r = rows_of(p, seq);
+    piece();
+  }
+  __device__ void piece() {
+    nt = tiles_of<S>(p, r, t + tpt);
+    const uint64_t left = end - at;
+    kt1 = nt - kt0 < left ? nt : kt0 + (uint32_t)left;
+  }
+  __device__ bool next() {
+    at += kt1 - kt0;
+    if (at >= end) return false;
+    g0 += nt;
+    kt0 = 0;
+    t += tpt;
+    if (t >= r.n) {
+      t = 0;
+      if (++head == p.a.pages.n_kv_heads) {
+        head = 0;
+        do {
+          if (++seq >= p.a.seqs.n_seqs || p.prefix) return false;
+          r = rows_of(p, seq);
+        } while (r.n == 0);
+      }
+    }
+    piece();
+    return true;
+  }
+  __device__ uint32_t tokens() const { return r.n - t < tpt ? r.n - t : tpt; }
+  __device__ uint32_t kend() const { return keys_end(p, r, t + tpt); }
+  // Whole in one block, or the blocks it lies in.
+  __device__ uint32_t first_block() const { return (uint32_t)(g0 / chunk); }
+  __device__ uint32_t blocks() const { return (uint32_t)((g0 + nt - 1) / chunk) - first_block() + 1; }
+};
+
+// Sequence of a row by bisection (rows inside the prefix only).
+__device__ uint32_t find_seq(const Seqs& s, uint32_t row) {
+  uint32_t lo = 0, hi = s.n_seqs;
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (row_begin(s, mid) <= row) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// (element, head, token, page), boxes of 128 bytes x 1 x `tokens` x 1, swizzled.
+inline bool encode_pages(CUtensorMap* m, const Pages& p, void* base, int dtype, uint32_t tokens) {
+  const EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const uint64_t size = dtype == DT_F32 ? 4 : 2, ps = 1ull << p.page_shift;
+  const cuuint64_t dims[4] = {p.head_size, p.n_kv_heads, ps, p.n_pages};
+  // an axis of one entry has no stride to speak of
+  auto bytes = [&](uint64_t stride, uint64_t n) { return (n > 1 ? stride : p.head_size) * size; };
+  const cuuint64_t strides[3] = {bytes(p.head_stride, p.n_kv_heads), bytes(p.token_stride, ps),
+                                 bytes(p.page_stride, p.n_pages)};
+  const cuuint32_t box[4] = {(cuuint32_t)(128 / size), 1, tokens, 1}, estr[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType t = dtype == DT_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                : dtype == DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return fn(m, t, 4, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+
+}  // namespace
+}  // namespace k
+}  // namespace yl

@@ -1,0 +1,501 @@
+// Paged attention of items with many rows (prompts, and the rows of a whole
+// batch over a shared prefix) on the 5th-generation tensor cores. The
+// mathematics and the cutting of the work are paged_attention.cu's; here an
+// item is two tiles of 128 rows that read the same keys, one block per SM.
+//
+// Per key tile of 128 keys: S = Q K^T into tensor memory (128 x 128 f32 per row
+// tile, operands in 128-byte-swizzled shared memory); one thread per row reads
+// its row of S, takes the exponentials and writes the weights P, rounded to 16
+// bits, over the first half of S; O += P V with P as the operand from tensor
+// memory, V from shared memory ([key][element], so its descriptor is that of an
+// operand whose rows run along the columns of the product). The two row tiles
+// take turns: while one's softmax runs, the tensor cores multiply for the
+// other. All MMAs are issued by one thread and run in its order, so the next
+// S may be issued right behind the product that reads P from the same columns.
+//
+// O stays in tensor memory. It is rescaled only when a row's maximum has grown
+// by more than 2^8 since the last time: until then P is taken relative to the
+// old maximum (at most 2^8, 2^15 with f16's shift), which changes nothing in the
+// quotient O / l. The commit that announces S of a tile covers the product of
+// the tile before, so O is at rest while its rows are rescaled.
+//
+// Warps: 0-3 softmax of the first row tile, 4-7 of the second (warp w reads
+// tensor-memory lanes 32 (w % 4) ..), 8 issues the MMAs, 9 loads Q (a box of
+// group heads x tokens), and keys and values page by page, 10 and 11 only hand
+// their registers to the softmax warps (a row of S is 128 registers).
+#include "paged_attention.cuh"
+
+namespace yl {
+namespace k {
+
+namespace {
+
+template <typename T, int HD>
+struct TcShape {
+  static constexpr int THREADS = 384;
+  static constexpr int KT = 128;                      // keys per tile
+  static constexpr int NH = HD / 64;                  // 128-byte columns of a row
+  static constexpr uint32_t COL = 128 * 128;          // bytes of a column of 128 rows
+  static constexpr uint32_t TILE = NH * COL;          // bytes of 128 rows
+  static constexpr int NBUF = HD == 128 ? 5 : 8;      // key / value tiles in the ring
+  static constexpr uint32_t SMEM = 1024 + (2 + NBUF) * TILE;
+  static constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0 : 1;
+  // f32 accumulators, 16-bit operands, M = 128; S: N = 128 keys; O: N = HD, its second operand along N
+  static constexpr uint32_t IDESC_S = (1u << 4) | (FMT << 7) | (FMT << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+  static constexpr uint32_t IDESC_O =
+      (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((128u >> 4) << 24);
+  static_assert(SMEM <= 226 * 1024, "shared memory");
+  static_assert(SMEM > 114 * 1024, "one block per SM: it holds all of tensor memory");
+};
+constexpr uint32_t TMEM_S = 0, TMEM_O = 256, TMEM_COLS = 512;  // per row tile: 128 columns of each
+
+// V [key][element]: rows of 128 bytes run along N, 8-key groups 1024 bytes apart, 64-element columns COL apart.
+__device__ __forceinline__ uint64_t smem_desc_n(uint32_t saddr, uint32_t col_bytes) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(col_bytes >> 4) << 16) | (64ull << 32) | (1ull << 46) |
+         (2ull << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " YL_V32 ";" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+               "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+               "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+               "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 3-D tiled load: (element, head, row).
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t head, uint32_t row,
+                                         uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(row), "r"(smem_u32(bar))
+      : "memory");
+}
+
+template <typename T, typename O, int HD>
+__global__ void __launch_bounds__(384, 1)
+    attend_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ Pass p) {
+  using S = TcShape<T, HD>;
+  constexpr float SHIFT = std::is_same<T, __half>::value ? 7.0f : 0.0f;  // weights up to 2^(SHIFT + 8)
+  constexpr float GROWN = 8.0f;
+  extern __shared__ uint8_t raw[];
+  __shared__ Start start;
+  __shared__ uint64_t scratch[16];
+  __shared__ __align__(8) uint64_t full[S::NBUF], empty[S::NBUF], q_full, q_empty, s_full[2], p_full[2], o_full[2], drain;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  const uint32_t q_smem = smem_u32(smem), ring = q_smem + 2 * S::TILE;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t tok_tile = 128 / p.group, tpt = 2 * tok_tile;
+  const PagedAttnArgs& a = p.a;
+
+  if (threadIdx.x == 0) {
+    for (int b = 0; b < S::NBUF; ++b) {
+      mbar_init(&full[b], 1);
+      mbar_init(&empty[b], 1);
+    }
+    mbar_init(&q_full, 1);
+    mbar_init(&q_empty, 1);
+    mbar_init(&drain, 1);
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&s_full[x], 1);
+      mbar_init(&p_full[x], 4);
+      mbar_init(&o_full[x], 1);
+    }
+    mbar_fence_init();
+    abort_flag = 0;
+  }
+  grid_dep_launch();
+  find_start<S>(p, tpt, &start, scratch);
+  const bool idle = start.seq == 0xFFFFFFFFu;
+  if (!idle && warp == 8) {
+    tmem_alloc(&tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = idle ? 0 : tmem_slot;
+
+  // 384 threads at 168 registers are launched; 256 x 208 + 128 x 80 fit in them
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+  if (!idle && warp == 9) {
+    // ---- loads ----
+    Walk<S> w(p, tpt, start);
+    const uint32_t ps = 1u << a.pages.page_shift;
+    const uint32_t tb = ps < (uint32_t)S::KT ? ps : (uint32_t)S::KT, pieces = S::KT / tb;
+    uint32_t n = 0, items = 0;
+    bool ok = true;
+    do {
+      const uint32_t kend = w.kend(), tseq = p.prefix ? 0 : w.seq;
+      if (lane == 0 && !p.prefix && a.seqs.status && w.r.pos0 + (int64_t)w.r.n > (int64_t)w.r.limit)
+        *a.seqs.status = STATUS_RANGE;
+      const uint32_t tiles = w.tokens() > tok_tile ? 2 : 1;
+      if (items > 0) {
+        ok = mbar_wait(&q_empty, (items - 1) & 1, nullptr);
+        ok = __all_sync(FULL, ok);
+        if (!ok) break;
+      }
+      if (lane == 0) mbar_arrive_expect_tx(&q_full, tiles * S::NH * 128 * p.group * tok_tile);
+      __syncwarp();
+      if (lane < tiles * S::NH) {
+        const uint32_t x = lane / S::NH, c = lane % S::NH;
+        tma_rows(q_smem + x * S::TILE + c * S::COL, &map_q, c * 64, w.head * p.group, w.r.row0 + w.t + x * tok_tile,
+                 &q_full);
+      }
+      ++items;
+      for (uint32_t kt = w.kt0; kt < w.kt1 && ok; ++kt) {
+        const uint32_t k0 = p.from + kt * S::KT;
+        const uint32_t live = kend > k0 ? min(pieces, (kend - k0 + tb - 1) / tb) : 0;  // loads with a visible key
+        // the tile's pages, one per lane: the same for keys and values (pieces <= 16, NH <= 2)
+        const uint32_t piece = lane / S::NH, col = lane % S::NH, pos = k0 + piece * tb;
+        uint32_t page = 0;
+        if (piece < live) {
+          page = page_of(a.seqs, a.pages, tseq, pos);
+          if (page == NO_PAGE) {
+            page = a.pages.n_pages;
+            if (a.seqs.status) *a.seqs.status = STATUS_RANGE;
+          }
+        }
+        for (uint32_t kv = 0; kv < 2; ++kv, ++n) {
+          const uint32_t b = n % S::NBUF;
+          if (n >= (uint32_t)S::NBUF) {
+            ok = mbar_wait(&empty[b], (n / S::NBUF - 1) & 1, nullptr) && !abort_flag;
+            ok = __all_sync(FULL, ok);
+            if (!ok) break;
+          }
+          if (lane == 0) mbar_arrive_expect_tx(&full[b], live * tb * 128 * S::NH);
+          __syncwarp();
+          if (piece < live)
+            tma_page(ring + b * S::TILE + col * S::COL + piece * tb * 128, kv ? &map_v : &map_k, col * 64, w.head,
+                     pos & (ps - 1), page, &full[b]);
+        }
+      }
+    } while (ok && w.next());
+    if (!ok) {
+      abort_flag = 1;
+      if (lane == 0) {
+        if (a.seqs.status) *a.seqs.status = STATUS_TIMEOUT;
+        // the copies this warp issued land before the block ends
+        if (items) mbar_wait(&q_full, (items - 1) & 1, nullptr, 200000000ull);
+        for (uint32_t i = n > (uint32_t)S::NBUF ? n - S::NBUF : 0; i < n; ++i)
+          mbar_wait(&full[i % S::NBUF], (i / S::NBUF) & 1, nullptr, 200000000ull);
+      }
+      __syncwarp();
+    }
+  } else if (!idle && warp == 8) {
+    // ---- MMAs: one lane issues; all wait, and clear what lies behind the last key ----
+    Walk<S> w(p, tpt, start);
+    uint32_t n = 0, items = 0, p_phase[2] = {0, 0};
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = ok && mbar_wait(bar, parity, nullptr) && !abort_flag;
+      ok = __all_sync(FULL, ok);
+      tc_fence_after();
+      return ok;
+    };
+    auto qk = [&](uint32_t x, uint32_t buf) {
+      if (lane == 0) {
+        const uint32_t q = q_smem + x * S::TILE, kb = ring + buf * S::TILE;
+#pragma unroll
+        for (uint32_t s = 0; s < HD / 16; ++s) {
+          const uint32_t off = (s >> 2) * S::COL + (s & 3) * 32;
+          mma_ss(tmem + TMEM_S + 128 * x, smem_desc_sw128(q + off), smem_desc_sw128(kb + off), S::IDESC_S, s > 0);
+        }
+        tc_commit(&s_full[x]);
+      }
+    };
+    auto pv = [&](uint32_t x, uint32_t buf, bool first, bool last) {
+      if (lane == 0) {
+        const uint32_t vb = ring + buf * S::TILE;
+#pragma unroll
+        for (uint32_t s = 0; s < S::KT / 16; ++s)
+          mma_ts(tmem + TMEM_O + 128 * x, tmem + TMEM_S + 128 * x + 8 * s, smem_desc_n(vb + s * 16 * 128, S::COL),
+                 S::IDESC_O, !first || s > 0);
+        if (last) tc_commit(&o_full[x]);
+      }
+    };
+    do {
+      const uint32_t kend = w.kend(), tiles = w.tokens() > tok_tile ? 2 : 1, nt = w.kt1 - w.kt0;
+      if (!wait(&q_full, items & 1) || !wait(&full[n % S::NBUF], (n / S::NBUF) & 1)) break;
+      for (uint32_t x = 0; x < tiles; ++x) qk(x, n % S::NBUF);
+      if (lane == 0) {
+        tc_commit(&empty[n % S::NBUF]);
+        if (nt == 1) tc_commit(&q_empty);
+      }
+      for (uint32_t i = 0; i < nt && ok; ++i) {
+        const uint32_t v = n + 1, kn = n + 2, k0 = p.from + (w.kt0 + i) * S::KT;
+        const bool more = i + 1 < nt;
+        if (!wait(&full[v % S::NBUF], (v / S::NBUF) & 1)) break;
+        if (k0 + S::KT > kend) {
+          // values behind the last visible key may be anything: their weight is 0, and 0 times NaN is not
+          uint8_t* vb = smem + (2 + v % S::NBUF) * S::TILE;
+          const uint32_t from = kend > k0 ? kend - k0 : 0;
+          for (uint32_t u = lane; u < (S::KT - from) * 8 * S::NH; u += 32) {
+            const uint32_t c = u / ((S::KT - from) * 8), o = u % ((S::KT - from) * 8);
+            *reinterpret_cast<uint4*>(vb + c * S::COL + from * 128 + o * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();
+          __syncwarp();
+        }
+        for (uint32_t x = 0; x < tiles; ++x) {
+          if (!wait(&p_full[x], p_phase[x])) break;
+          p_phase[x] ^= 1;
+          pv(x, v % S::NBUF, i == 0, !more);
+          if (more) {
+            if (x == 0 && !wait(&full[kn % S::NBUF], (kn / S::NBUF) & 1)) break;
+            qk(x, kn % S::NBUF);
+          }
+        }
+        if (!ok) break;
+        if (lane == 0) {
+          tc_commit(&empty[v % S::NBUF]);
+          if (more) tc_commit(&empty[kn % S::NBUF]);
+          if (i + 2 == nt) tc_commit(&q_empty);
+        }
+        n += 2;
+      }
+      ++items;
+    } while (ok && w.next());
+    if (!ok) {
+      abort_flag = 1;
+      if (lane == 0 && a.seqs.status) *a.seqs.status = STATUS_TIMEOUT;
+    }
+    if (lane == 0) {
+      tc_commit(&drain);  // every MMA has completed when this flips
+      mbar_wait(&drain, 0, nullptr);
+    }
+    __syncwarp();
+  }
+  } else {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+  if (!idle) {
+    // ---- softmax: one thread per row ----
+    Walk<S> w(p, tpt, start);
+    const uint32_t x = warp >> 2, quarter = (warp & 3) << 21;  // lane 32 * (warp % 4) in the address's upper half
+    const uint32_t ts = tmem + TMEM_S + 128 * x + quarter, to = tmem + TMEM_O + 128 * x + quarter;
+    const uint32_t m = 32 * (warp & 3) + lane;
+    const bool flip = a.scale < 0.0f;
+    const float sc = fabsf(a.scale) * LOG2E;
+    uint32_t s_phase = 0, o_phase = 0;
+    bool ok = true;
+    do {
+      const uint32_t all = w.tokens(), t0 = x * tok_tile, kend = w.kend();
+      const uint32_t tok = m / p.group + t0, gh = m % p.group;
+      if (warp == 0 && w.kt0 == 0) {
+        const uint32_t first = w.first_block(), blocks = w.blocks();
+        for (uint32_t t = lane; t < all; t += 32)
+          p.desc[(uint64_t)(w.r.row0 + w.t + t) * a.pages.n_kv_heads + w.head] =
+              make_uint2(first, blocks == 1 ? t : blocks << 16 | t);
+      }
+      if (all <= t0) continue;  // this row tile has no rows (no barrier of it moves)
+      const bool live = m < tok_tile * p.group && tok < all;
+      const bool busy = __any_sync(FULL, live);
+      const uint32_t row = w.r.row0 + w.t + (live ? tok : 0), head = w.head * p.group + gh;
+      // keys this row sees, and those that every row of the tile sees
+      int64_t e = w.r.pos0 + w.t + tok + 1, e0 = w.r.pos0 + w.t + t0 + 1;
+      if (p.prefix) {
+        e = e0 = kend;
+        if (start.masked) {
+          e0 = 0;
+          if (live) {
+            const uint32_t s = find_seq(a.seqs, row);
+            e = (int64_t)a.seqs.seq_len[s] - row_end(a.seqs, s) + row + 1;
+          }
+        }
+      }
+      const uint32_t lim = e < 0 ? 0 : e < (int64_t)kend ? (uint32_t)e : kend;
+      const uint32_t all_see = e0 < 0 ? 0 : e0 < (int64_t)kend ? (uint32_t)e0 : kend;
+      float mx = -INFINITY, l = 0.0f;  // the maximum that O and l are taken relative to, in powers of two
+
+      for (uint32_t kt = w.kt0; kt < w.kt1; ++kt) {
+        const uint32_t k0 = p.from + kt * S::KT;
+        ok = mbar_wait(&s_full[x], s_phase, nullptr) && !abort_flag;
+        ok = __all_sync(FULL, ok);
+        if (!ok) break;
+        s_phase ^= 1;
+        tc_fence_after();
+        if (busy) {
+          uint32_t r[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, r[c]);
+          tmem_wait_ld();
+          if (flip) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i) r[c][i] ^= 0x80000000u;
+          }
+          if (k0 + S::KT > all_see) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (k0 + 32 * c + i >= lim) r[c][i] = 0xFF800000u;
+          }
+          float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) t[c] = fmaxf(t[c], __uint_as_float(r[c][i]));
+          const float top = fmaxf(mx, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * sc);
+          // a row whose maximum has grown a lot rescales (all rows of the warp then take their own)
+          if (__any_sync(FULL, top > mx + GROWN || mx == -INFINITY)) {
+            const float f = ex2(mx - (top == -INFINITY ? 0.0f : top));  // 0 from -inf
+            l *= f;
+            mx = top;
+            if (kt > w.kt0) {
+#pragma unroll
+              for (int c = 0; c < HD / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(to + 32 * c, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_st32(to + 32 * c, o);
+              }
+            }
+          }
+          const float ref = mx == -INFINITY ? 0.0f : mx - SHIFT;
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t pk[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const int c = 2 * h + i / 16, j = 2 * (i % 16);
+              const float u = ex2(fmaf(__uint_as_float(r[c][j]), sc, -ref));
+              const float v = ex2(fmaf(__uint_as_float(r[c][j + 1]), sc, -ref));
+              sum[i & 1] += u;
+              sum[2 + (i & 1)] += v;
+              pk[i] = pack2<T>(u, v);
+            }
+            tmem_st32(ts + 32 * h, pk);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[x]);
+      }
+      if (!ok) break;
+
+      // ---- the item's end ----
+      ok = mbar_wait(&o_full[x], o_phase, nullptr) && !abort_flag;
+      ok = __all_sync(FULL, ok);
+      if (!ok) break;
+      o_phase ^= 1;
+      tc_fence_after();
+      if (busy) {
+        const bool whole = w.blocks() == 1, direct = whole && !p.joined;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        float* part = whole ? p.rowpart + ((uint64_t)row * a.n_heads + head) * PART<HD>
+                            : p.slots + ((uint64_t)(2 * blockIdx.x + (w.kt0 == 0 ? 1 : 0)) * TC_TILE + tok * p.group + gh) * PART<HD>;
+        O* out = static_cast<O*>(a.out) + (uint64_t)row * a.out_stride + (uint64_t)head * HD;
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(to + 32 * c, o);
+          tmem_wait_ld();
+          if (live) {
+            if (direct) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
+              if constexpr (sizeof(O) == 2) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                  uint4 v;
+                  v.x = pack2<O>(__uint_as_float(o[i]), __uint_as_float(o[i + 1]));
+                  v.y = pack2<O>(__uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+                  v.z = pack2<O>(__uint_as_float(o[i + 4]), __uint_as_float(o[i + 5]));
+                  v.w = pack2<O>(__uint_as_float(o[i + 6]), __uint_as_float(o[i + 7]));
+                  *reinterpret_cast<uint4*>(out + 32 * c + i) = v;
+                }
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4)
+                  *reinterpret_cast<uint4*>(out + 32 * c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<uint4*>(part + 32 * c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            }
+          }
+        }
+        if (live) {
+          if (!direct) part[HD] = mx - SHIFT, part[HD + 1] = l;
+          else if (a.lse) a.lse[(uint64_t)row * a.n_heads + head] = l == 0.0f ? -INFINITY : (mx - SHIFT + log2f(l)) * LN2;
+        }
+      }
+      tc_fence_before();  // O has been read before the next item's first product, which waits for its weights
+    } while (w.next());
+    if (!ok) abort_flag = 1;
+  }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (!idle && warp == 8) tmem_dealloc(tmem, TMEM_COLS);
+  grid_dep_wait();  // the launch before has ended when this one has
+}
+
+bool encode_rows(CUtensorMap* m, const Pass& p) {
+  const EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const uint32_t hd = p.a.pages.head_size;
+  const cuuint64_t dims[3] = {hd, p.a.n_heads, p.a.seqs.n_rows};
+  const cuuint64_t strides[2] = {hd * 2ull, p.a.q_stride * 2};
+  const cuuint32_t box[3] = {64, p.group, 128 / p.group}, estr[3] = {1, 1, 1};
+  return fn(m, p.dtype == DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+            const_cast<void*>(p.a.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, typename O, int HD>
+cudaError_t launch(const Pass& p, const LaunchCfg& lc) {
+  using S = TcShape<T, HD>;
+  static std::atomic<uint64_t> ready{0};
+  const cudaError_t e = allow_smem(ready, attend_tc_kernel<T, O, HD>, S::SMEM);
+  if (e != cudaSuccess) return e;
+  const uint32_t ps = 1u << p.a.pages.page_shift, tokens = ps < (uint32_t)S::KT ? ps : (uint32_t)S::KT;
+  CUtensorMap mk, mv, mq;
+  if (!encode_pages(&mk, p.a.pages, p.a.pages.k, p.dtype, tokens) ||
+      !encode_pages(&mv, p.a.pages, p.a.pages.v, p.dtype, tokens) || !encode_rows(&mq, p))
+    return cudaErrorInvalidValue;
+  return launch_kernel(attend_tc_kernel<T, O, HD>, dim3(p.grid), dim3(S::THREADS), S::SMEM, lc, mk, mv, mq, p);
+}
+template <typename T, typename O>
+cudaError_t launch_hd(const Pass& p, const LaunchCfg& lc) {
+  return p.a.pages.head_size == 128 ? launch<T, O, 128>(p, lc) : launch<T, O, 64>(p, lc);
+}
+
+}  // namespace
+
+cudaError_t attend_tc(const Pass& p, bool out_f32, const LaunchCfg& lc) {
+  if (p.dtype == DT_F16) return out_f32 ? launch_hd<__half, float>(p, lc) : launch_hd<__half, __half>(p, lc);
+  return out_f32 ? launch_hd<__nv_bfloat16, float>(p, lc) : launch_hd<__nv_bfloat16, __nv_bfloat16>(p, lc);
+}
+
+}  // namespace k
+}  // namespace yl
