@@ -270,6 +270,18 @@ def test_large_scores(yl, torch_cuda):
         within(lse, wlse, lb, "lse")
 
 
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+def test_scales(yl, torch_cuda, scale):
+    """A negative scale, and one of 0 (every visible key alike)."""
+    for t in DTYPES.values():
+        g = ref.Geometry(20, 4, 1, 64, page=16, lens=[200, 90, 0], rows=[1, 70, 1])
+        q, (k, v) = queries(g, t), g.pool(t)
+        out, lse = attend(yl, g, q.cuda(), k.cuda(), v.cuda(), scale)
+        want, wlse, ob, lb = ref.attention(g, q, k, v, scale)
+        within(out, want, ob + (want.abs() + ob) * ref.half_step(t) + 2.0**-25 * (t == torch.float16), "out")
+        within(lse, wlse, lb, "lse")
+
+
 def test_cache_beyond_32_bits(yl, torch_cuda):
     """Pages whose elements lie beyond 2^32 (a view with a large page stride over one allocation)."""
     hd, kv, page = 64, 1, 8

@@ -358,41 +358,64 @@ class DType(enum.IntEnum):
 ROPE_GGUF, ROPE_LLAMA3 = 0, 1
 
 
-def _dtype(t) -> int:
-    """yl_dtype of a torch tensor."""
-    d = _DTYPES.get(str(t.dtype))
-    if d is None:
-        raise TypeError(f"no yl_dtype for {t.dtype}")
+_torch = None  # set at the first serving call, with the table below
+_dtypes: dict = {}
+
+
+def _load_torch():
+    global _torch
+    import torch
+    _dtypes.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    _torch = torch
+    return torch
+
+
+def _here(what: str, *tensors) -> int:
+    """The current device, on which the tensors have to be (raw addresses and None pass)."""
+    dev = (_torch or _load_torch()).cuda.current_device()
+    for t in tensors:
+        if t is not None and not isinstance(t, int) and t.get_device() != dev:
+            raise ValueError(f"{what}: every tensor must be on the current CUDA device")
+    return dev
+
+
+def _dtype(t, what: str, want: Optional[int] = None) -> int:
+    d = _dtypes.get(t.dtype)
+    if d is None or (want is not None and d != want):
+        raise TypeError(f"{what} must be {'float32, float16 or bfloat16' if want is None else DType(want).name}, "
+                        f"got {t.dtype}")
     return d
 
 
-_DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
-
-
-def _expect(t, what: str, dtype: str, numel: int):
-    """`t`, checked to be a contiguous tensor of the current device that holds numel values (raw addresses pass)."""
+def _flat(t, what: str, dtype, numel: int):
+    """Address of a contiguous tensor of the type that holds numel values (raw addresses and None pass)."""
     if t is None or isinstance(t, int):
         return t
-    if str(t.dtype) not in dtype:
+    if t.dtype != dtype:
         raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
-    if not t.is_contiguous() or t.numel() < numel:
+    if t.numel() < numel or not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous and hold {numel} values, got shape {tuple(t.shape)}")
-    return _here(t, what)
-
-
-def _here(t, what: str):
-    import torch
-    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"{what} must be on the current CUDA device")
-    return t
+    return t.data_ptr()
 
 
 def _row_stride(t, what: str, width: int, n_rows: int) -> int:
-    """Elements between rows of a tensor of at least n_rows rows ([rows, width], or [rows, heads, head_size])."""
-    inner = t[0].numel() if t.dim() > 1 and t.shape[0] else 0
-    if t.dim() < 2 or inner != width or t.shape[0] < n_rows or (n_rows and not t[0].is_contiguous()):
-        raise ValueError(f"{what} must hold {n_rows} rows of {width} consecutive values, got shape {tuple(t.shape)}")
-    return t.stride(0) if t.shape[0] > 1 else width
+    """Elements between the rows of a tensor [rows, width] or [rows, heads, head_size], rows consecutive inside."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 2:
+        ok = shape[1] == width and (stride[1] == 1 or width == 1)
+    else:
+        ok = len(shape) == 3 and shape[1] * shape[2] == width and stride[2] == 1 and (stride[1] == shape[2] or shape[1] == 1)
+    if not ok or shape[0] < n_rows:
+        raise ValueError(f"{what} must hold {n_rows} rows of {width} consecutive values, got shape {tuple(shape)}, "
+                         f"strides {stride}")
+    return stride[0] if shape[0] > 1 else width
+
+
+def _raw_stream(stream, dev: int) -> int:
+    """cudaStream_t of `stream` (torch's current stream where it is None)."""
+    if stream is None:
+        return _torch._C._cuda_getCurrentRawStream(dev)
+    return stream if isinstance(stream, int) else stream.cuda_stream
 
 
 class KvPages:
@@ -400,6 +423,7 @@ class KvPages:
 
     def __init__(self, c: KvPagesC, keep=None):
         self.c = c
+        self.ref = C.byref(c)
         self._keep = keep
 
     @classmethod
@@ -414,11 +438,10 @@ class KvPages:
         consecutive; transposed and sliced tensors are fine)."""
         if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.stride(3) != 1:
             raise ValueError("k and v must be [n_pages, page_size, n_kv_heads, head_size], alike, last axis consecutive")
-        _here(k, "k")
-        _here(v, "v")
+        _here("pages", k, v)
         n, ps, h, hd = k.shape
         sp, st, sh, _ = (max(x, hd) for x in k.stride())
-        return cls(KvPagesC(_dtype(k), 0, n, ps, h, hd, sp, st, sh, k.data_ptr(), v.data_ptr()), (k, v))
+        return cls(KvPagesC(_dtype(k, "pages"), 0, n, ps, h, hd, sp, st, sh, k.data_ptr(), v.data_ptr()), (k, v))
 
     def free(self) -> None:
         if self.c.owned and self.c.k:
@@ -437,16 +460,15 @@ class SeqBatch:
 
     def __init__(self, row_start, seq_len, page_table, n_rows: int, shared_len: int = 0, status=None):
         n = seq_len.numel()
-        ints = ("torch.int32", "torch.uint32")
-        _expect(row_start, "row_start", ints, n + 1)
-        _expect(seq_len, "seq_len", ints, n)
+        _here("batch", row_start, seq_len, page_table, status)
         if page_table.dim() != 2 or page_table.shape[0] != n:
             raise ValueError("page_table must be [n_seqs, slots]")
-        _expect(page_table, "page_table", ints, n * page_table.shape[1])
-        _expect(status, "status", ints, 1)
+        i32 = _torch.int32
         self._keep = (row_start, seq_len, page_table, status)
-        self.c = SeqBatchC(n, n_rows, page_table.shape[1], shared_len, _ptr(row_start), _ptr(seq_len),
-                           _ptr(page_table), _ptr(status))
+        self.c = SeqBatchC(n, n_rows, page_table.shape[1], shared_len, _flat(row_start, "row_start", i32, n + 1),
+                           _flat(seq_len, "seq_len", i32, n), _flat(page_table, "page_table", i32, page_table.numel()),
+                           _flat(status, "status", i32, 1))
+        self.ref = C.byref(self.c)
 
 
 def paged_append(qkv, pages: KvPages, batch: SeqBatch, n_heads: int, rope_cs=None, rope_mode: int = ROPE_GGUF,
@@ -454,28 +476,29 @@ def paged_append(qkv, pages: KvPages, batch: SeqBatch, n_heads: int, rope_cs=Non
     """Rotates the new rows' queries and keys and writes keys and values to their pages (yl_paged_append). qkv: f32
     rows [q | k | v]; q_out: rows of rotated queries in the cache's type, or None; rope_cs: [len, head_size/2, 2]
     (or an address from Transformer.rope_table, with rope_len), or None for no rotation."""
-    p = pages.c
-    n = batch.c.n_rows
-    if _dtype(qkv) != DType.F32:
-        raise TypeError("qkv must be float32")
-    if q_out is not None and _dtype(q_out) != p.dtype:
-        raise TypeError("q_out must have the cache's type")
-    if rope_cs is not None and not isinstance(rope_cs, int):
-        _expect(rope_cs, "rope_cs", ("torch.float32",), rope_cs.shape[0] * p.head_size)
-        rope_len = rope_cs.shape[0] if rope_len is None else min(rope_len, rope_cs.shape[0])
-    _here(qkv, "qkv")
+    p, n = pages.c, batch.c.n_rows
+    hd = p.head_size
+    dev = _here("paged_append", qkv, q_out, rope_cs)
+    _dtype(qkv, "qkv", DType.F32)
+    q_ptr = q_stride = 0
     if q_out is not None:
-        _here(q_out, "q_out")
-    _check(_lib.yl_paged_append(
-        _ptr(q_out), 0 if q_out is None else _row_stride(q_out, "q_out", n_heads * p.head_size, n), _ptr(qkv),
-        _row_stride(qkv, "qkv", (n_heads + 2 * p.n_kv_heads) * p.head_size, n), C.byref(p), C.byref(batch.c), n_heads,
-        _ptr(rope_cs), rope_len or 0, rope_mode, _stream(stream)))
+        _dtype(q_out, "q_out", p.dtype)
+        q_ptr, q_stride = q_out.data_ptr(), _row_stride(q_out, "q_out", n_heads * hd, n)
+    if rope_cs is not None and not isinstance(rope_cs, int):
+        rows = rope_cs.shape[0]
+        rope_len = rows if rope_len is None else min(rope_len, rows)
+        rope_cs = _flat(rope_cs, "rope_cs", _torch.float32, rows * hd)
+    rc = _lib.yl_paged_append(q_ptr, q_stride, qkv.data_ptr(),
+                              _row_stride(qkv, "qkv", (n_heads + 2 * p.n_kv_heads) * hd, n), pages.ref, batch.ref,
+                              n_heads, rope_cs, rope_len or 0, rope_mode, _raw_stream(stream, dev))
+    if rc:
+        _check(rc)
 
 
 def paged_attention_workspace(pages: KvPages, batch: SeqBatch, n_heads: int) -> int:
     """Bytes of device workspace paged_attention needs for a batch of these counts."""
     n = C.c_uint64()
-    _check(_lib.yl_paged_attention_workspace(C.byref(pages.c), C.byref(batch.c), n_heads, C.byref(n)))
+    _check(_lib.yl_paged_attention_workspace(pages.ref, batch.ref, n_heads, C.byref(n)))
     return n.value
 
 
@@ -484,19 +507,17 @@ def paged_attention(output, q, pages: KvPages, batch: SeqBatch, n_heads: int, at
     """Causal attention of the batch's rows over the paged cache (yl_paged_attention). q: rows of the cache's type,
     output: rows of that type or f32 ([rows, n_heads, head_size] or flat); lse: f32 [rows, n_heads] or None;
     workspace: a uint8 tensor of at least paged_attention_workspace bytes."""
-    p = pages.c
-    n = batch.c.n_rows
-    if _dtype(q) != p.dtype:
-        raise TypeError("q must have the cache's type")
-    _expect(lse, "lse", ("torch.float32",), n * n_heads)
-    _here(q, "q")
-    _here(output, "output")
-    _here(workspace, "workspace")
+    p, n = pages.c, batch.c.n_rows
     width = n_heads * p.head_size
-    _check(_lib.yl_paged_attention(
-        output.data_ptr(), _row_stride(output, "output", width, n), _dtype(output), _ptr(lse), q.data_ptr(),
-        _row_stride(q, "q", width, n), C.byref(p), C.byref(batch.c), n_heads, attn_scale, workspace.data_ptr(),
-        workspace.numel() * workspace.element_size(), _stream(stream)))
+    dev = _here("paged_attention", output, q, workspace, lse)
+    _dtype(q, "q", p.dtype)
+    rc = _lib.yl_paged_attention(
+        output.data_ptr(), _row_stride(output, "output", width, n), _dtype(output, "output"),
+        _flat(lse, "lse", _torch.float32, n * n_heads), q.data_ptr(), _row_stride(q, "q", width, n), pages.ref,
+        batch.ref, n_heads, attn_scale, _flat(workspace, "workspace", _torch.uint8, 1), workspace.numel(),
+        _raw_stream(stream, dev))
+    if rc:
+        _check(rc)
 
 
 def token_logprobs(logits, tokens=None, logprobs=None, entropy=None, top_ids=None, top_logprobs=None,
@@ -504,20 +525,18 @@ def token_logprobs(logits, tokens=None, logprobs=None, entropy=None, top_ids=Non
     """Log probabilities of the given tokens, entropies and most likely tokens of rows of logits [rows, vocab]
     (yl_token_logprobs). Device tensors: tokens int32 [rows], logprobs and entropy f32 [rows], top_ids int32 and
     top_logprobs f32 [rows, k]; each of the three groups may be left out."""
-    if logits.dim() != 2 or logits.stride(1) != 1 and logits.shape[1] > 1:
-        raise ValueError("logits must be [rows, vocab] with consecutive values in a row")
+    if logits.dim() != 2:
+        raise ValueError("logits must be [rows, vocab]")
     n, vocab = logits.shape
     k = 0 if top_ids is None else top_ids.shape[-1]
-    f, i = ("torch.float32",), ("torch.int32",)
-    _here(logits, "logits")
-    _expect(tokens, "tokens", i, n)
-    _expect(logprobs, "logprobs", f, n)
-    _expect(entropy, "entropy", f, n)
-    _expect(top_ids, "top_ids", i, n * k)
-    _expect(top_logprobs, "top_logprobs", f, n * k)
-    _check(_lib.yl_token_logprobs(logits.data_ptr(), _dtype(logits), logits.stride(0) if n > 1 else vocab, n, vocab,
-                                  _ptr(tokens), _ptr(logprobs), _ptr(entropy), k, _ptr(top_ids), _ptr(top_logprobs),
-                                  _stream(stream)))
+    dev = _here("token_logprobs", logits, tokens, logprobs, entropy, top_ids, top_logprobs)
+    f, i = _torch.float32, _torch.int32
+    rc = _lib.yl_token_logprobs(
+        logits.data_ptr(), _dtype(logits, "logits"), _row_stride(logits, "logits", vocab, n), n, vocab,
+        _flat(tokens, "tokens", i, n), _flat(logprobs, "logprobs", f, n), _flat(entropy, "entropy", f, n), k,
+        _flat(top_ids, "top_ids", i, n * k), _flat(top_logprobs, "top_logprobs", f, n * k), _raw_stream(stream, dev))
+    if rc:
+        _check(rc)
 
 
 # -------------------------------------------------- transformer.rs ---

@@ -28,10 +28,12 @@
 // the tile's keys and join at the item's end. Decoding has 1..16 rows per
 // item and is bound by reading the cache, so WK = 4; from 33 rows on WK = 1.
 // f32 operands are split into two tf32 numbers and multiplied as hi*hi + hi*lo
-// + lo*hi (2^-21 relative); 16-bit ones are exact, and the softmax weights are
+// + lo*hi (2^-22 relative); 16-bit ones are exact, and the softmax weights are
 // rounded to their type for the second product (the sum l takes them
 // unrounded), f16 weights at 2^10 times their value so that small ones do not
 // fall below f16's range.
+#include <cmath>
+
 #include "paged_attention.cuh"
 
 namespace yl {
@@ -80,10 +82,10 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo: hi the nearest tf32, lo exact in f32 (the MMA drops its last bits, 2^-21 of x)
+// x = hi + lo in tf32, off by at most 2^-23 of x (each part rounded to 11 bits)
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-  lo = __float_as_uint(x - __uint_as_float(hi));
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -192,7 +194,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
     // ---- consumers ----
     Walk<S> w(p, tpt, start);
     const uint32_t wm = warp / WK, wk = warp % WK, g = lane >> 2, t4 = lane & 3;
-    const float scale2 = a.scale * LOG2E;
+    const uint32_t flip = p.flip ? (S::F32 ? 0x80000000u : 0x80008000u) : 0;  // sign bits of q
     constexpr int NB = S::WKEYS / 8, OB = HD / 8;
     uint32_t n = 0;
     bool ok = true;
@@ -234,6 +236,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
             v = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) +
                                                  (uint64_t)(w.r.row0 + w.t + m / p.group) * a.q_stride +
                                                  (uint64_t)(w.head * p.group + m % p.group) * HD + 4 * c);
+          if (flip) v = make_float4(-v.x, -v.y, -v.z, -v.w);
           *reinterpret_cast<float4*>(qs + m * S::QP + 4 * c) = v;
         }
         named_bar_sync(1, 32 * S::NW);
@@ -244,8 +247,8 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
                                                                 (uint64_t)row[i] * a.q_stride + (uint64_t)head[i] * HD);
 #pragma unroll
           for (int s = 0; s < HD / 16; ++s) {
-            qf[s][i] = live[i] ? q[8 * s + t4] : 0;
-            qf[s][2 + i] = live[i] ? q[8 * s + 4 + t4] : 0;
+            qf[s][i] = live[i] ? q[8 * s + t4] ^ flip : 0;
+            qf[s][2 + i] = live[i] ? q[8 * s + 4 + t4] ^ flip : 0;
           }
         }
       }
@@ -267,6 +270,14 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
 #pragma unroll
           for (int j = 0; j < NB; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
           if constexpr (S::F32) {
+// The tensor cores drop what falls below an accumulator's last bit, so
+            // long chains lose digits: two accumulators for the large products
+            // and one for the small ones, added at the end.
+            float s1[NB][4], sl[NB][4];
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) s1[j][c] = sl[j][c] = 0.0f;
 #pragma unroll 2
             for (int ks = 0; ks < HD / 16; ++ks) {  // 16 elements: two k-steps of 8
               uint32_t ah[2][4], al[2][4];
@@ -287,12 +298,16 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
                   uint32_t bh[2], bl[2];
                   split(__uint_as_float(r[2 * h]), bh[0], bl[0]);
                   split(__uint_as_float(r[2 * h + 1]), bh[1], bl[1]);
-                  mma_tf32(s[j], al[h], bh[0], bh[1]);
-                  mma_tf32(s[j], ah[h], bl[0], bl[1]);
-                  mma_tf32(s[j], ah[h], bh[0], bh[1]);
+                  mma_tf32(sl[j], al[h], bh[0], bh[1]);
+                  mma_tf32(sl[j], ah[h], bl[0], bl[1]);
+                  mma_tf32(h ? s1[j] : s[j], ah[h], bh[0], bh[1]);
                 }
               }
             }
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) s[j][c] = (s[j][c] + s1[j][c]) + sl[j][c];
           } else {
 #pragma unroll
             for (int ks = 0; ks < HD / 16; ++ks)
@@ -316,7 +331,6 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
           for (int j = 0; j < NB; ++j)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              s[j][c] *= scale2;
               if (mask && (int32_t)(k0 + wk * S::WKEYS + 8 * j + 2 * t4 + (c & 1)) >= lim[c >> 1]) s[j][c] = -INFINITY;
               top[c >> 1] = fmaxf(top[c >> 1], s[j][c]);
             }
@@ -324,7 +338,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
           for (int i = 0; i < 2; ++i) {
             top[i] = fmaxf(top[i], __shfl_xor_sync(FULL, top[i], 1));
             top[i] = fmaxf(top[i], __shfl_xor_sync(FULL, top[i], 2));
-            const float mn = fmaxf(m[i], top[i]);
+            const float mn = fmaxf(m[i], top[i] * p.sc);
             const float ref = mn == -INFINITY ? 0.0f : mn - SHIFT;
             corr[i] = ex2(m[i] - (mn == -INFINITY ? 0.0f : mn));  // 0 from -inf
             m[i] = mn;
@@ -333,7 +347,10 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
             for (int j = 0; j < NB; ++j)
 #pragma unroll
               for (int c = 2 * i; c < 2 * i + 2; ++c) {
-                s[j][c] = ex2(s[j][c] - ref);
+                // the product with the factor is exact before the maximum is taken off
+                float d = fmaf(s[j][c], p.sc, -ref);
+                if (S::F32) d = fmaf(fmaxf(s[j][c], -1e30f), p.sc_lo, d);  // (-inf stays in d alone)
+                s[j][c] = ex2(d);
                 sum += s[j][c];
               }
             l[i] = l[i] * corr[i] + sum;
@@ -378,9 +395,12 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
                 uint32_t vh[2], vl[2];
                 split(lds(base + at<S>(key, c) + e), vh[0], vl[0]);
                 split(lds(base + at<S>(key + 1, c) + e), vh[1], vl[1]);
-                mma_tf32(o[d], pl, vh[0], vh[1]);
-                mma_tf32(o[d], ph, vl[0], vl[1]);
-                mma_tf32(o[d], ph, vh[0], vh[1]);
+                float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // (added with rounding, see above)
+                mma_tf32(t, pl, vh[0], vh[1]);
+                mma_tf32(t, ph, vl[0], vl[1]);
+                mma_tf32(t, ph, vh[0], vh[1]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[d][c] += t[c];
               }
             }
           } else {
@@ -642,6 +662,10 @@ cudaError_t launch(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
     Pass p{};
     p.a = a;
     p.dtype = dtype;
+    const double sc = std::fabs((double)a.scale) * 1.4426950408889634;
+    p.sc = sc < 1.2e-38 ? 1.2e-38f : (float)sc;  // not 0: times -inf it stays -inf
+    p.sc_lo = std::isfinite(p.sc) ? (float)(sc - (double)p.sc) : 0.0f;
+    p.flip = a.scale < 0.0f;
     p.grid = blocks_of(pl.bm[i]);
     p.prefix = i;
     p.from = pl.shared && !i ? a.seqs.shared_len : 0;

@@ -10,7 +10,7 @@
 namespace yl {
 namespace k {
 
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LN2 = 0.6931471805599453f;
 constexpr int STATUS_TIMEOUT = -7;  // YL_ERR_TIMEOUT
 
 // One launch: over the sequences' own keys (from `from` on), or over the
@@ -18,6 +18,10 @@ constexpr int STATUS_TIMEOUT = -7;  // YL_ERR_TIMEOUT
 struct Pass {
   PagedAttnArgs a;
   int dtype;
+  // scores in powers of two are |scale| log2(e) (a product with q, negated where
+  // the scale is negative), as the sum of two f32
+  float sc, sc_lo;
+  uint32_t flip;
   uint32_t from, prefix;  // first key; 1: the prefix pass (keys 0 .. shared_len)
   uint32_t group, min_chunk;
   uint32_t grid;   // blocks

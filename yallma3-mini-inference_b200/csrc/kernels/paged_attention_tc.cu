@@ -293,8 +293,7 @@ __global__ void __launch_bounds__(384, 1)
     const uint32_t x = warp >> 2, quarter = (warp & 3) << 21;  // lane 32 * (warp % 4) in the address's upper half
     const uint32_t ts = tmem + TMEM_S + 128 * x + quarter, to = tmem + TMEM_O + 128 * x + quarter;
     const uint32_t m = 32 * (warp & 3) + lane;
-    const bool flip = a.scale < 0.0f;
-    const float sc = fabsf(a.scale) * LOG2E;
+    const float sc = p.sc;
     uint32_t s_phase = 0, o_phase = 0;
     bool ok = true;
     do {
@@ -338,7 +337,7 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, r[c]);
           tmem_wait_ld();
-          if (flip) {
+          if (p.flip) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
