@@ -49,32 +49,57 @@ struct TcShape {
 };
 constexpr uint32_t TMEM_S = 0, TMEM_O = 256, TMEM_COLS = 512;  // per row tile: 128 columns of each
 
-// V [key][element]: rows of 128 bytes run along N, 8-key groups 1024 bytes apart, 64-element columns COL apart.
-__device__ __forceinline__ uint64_t smem_desc_n(uint32_t saddr, uint32_t col_bytes) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(col_bytes >> 4) << 16) | (64ull << 32) | (1ull << 46) |
-         (2ull << 61);
+// Shared-memory descriptors of 128-byte-swizzled tiles, as (upper, lower) words:
+// the lower holds the address (in 16 bytes) and can be advanced by adding to it.
+// Q, K: rows of 128 bytes along the summed axis, 8-row groups 1024 bytes apart.
+// V [key][element]: rows of 128 bytes along N, 8-key groups 1024 bytes apart,
+// 64-element columns COL apart.
+constexpr uint32_t DESC_HI = 64u | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_n(uint32_t saddr, uint32_t col_bytes) {
+  return (saddr >> 4) | ((col_bytes >> 4) << 16);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(DESC_HI)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(DESC_HI)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " YL_V32 ";" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
-               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-               "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-               "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-               "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
-               : "memory");
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes != 0;
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // 3-D tiled load: (element, head, row).
@@ -134,9 +159,9 @@ __global__ void __launch_bounds__(384, 1)
   tc_fence_after();
   const uint32_t tmem = idle ? 0 : tmem_slot;
 
-  // 384 threads at 168 registers are launched; 256 x 208 + 128 x 80 fit in them
+  // 384 threads at 168 registers are launched; 256 x 200 + 128 x 104 are as many
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
   if (!idle && warp == 9) {
     // ---- loads ----
     Walk<S> w(p, tpt, start);
@@ -212,35 +237,51 @@ __global__ void __launch_bounds__(384, 1)
       tc_fence_after();
       return ok;
     };
-    auto qk = [&](uint32_t x, uint32_t buf) {
-      if (lane == 0) {
-        const uint32_t q = q_smem + x * S::TILE, kb = ring + buf * S::TILE;
+    // An MMA takes its descriptors from uniform registers. Issued by a lane that
+    // elect.sync names, from values that come out of a shuffle, eight cost 64
+    // cycles each, what the tensor cores need; by a lane picked with lane == 0
+    // they cost 130.
+    const uint32_t ut = __shfl_sync(FULL, tmem, 0);
+    const uint32_t uq = __shfl_sync(FULL, desc_k(q_smem), 0);
+    auto qk = [&](auto xc, uint32_t buf) {
+      constexpr uint32_t x = decltype(xc)::value;
+      const uint32_t kb = __shfl_sync(FULL, desc_k(ring + buf * S::TILE), 0);
+      if (elect_one()) {
 #pragma unroll
         for (uint32_t s = 0; s < HD / 16; ++s) {
-          const uint32_t off = (s >> 2) * S::COL + (s & 3) * 32;
-          mma_ss(tmem + TMEM_S + 128 * x, smem_desc_sw128(q + off), smem_desc_sw128(kb + off), S::IDESC_S, s > 0);
+          const uint32_t off = ((s >> 2) * S::COL + (s & 3) * 32) >> 4;
+          mma_ss(ut + TMEM_S + 128 * x, uq + x * (S::TILE >> 4) + off, kb + off, S::IDESC_S, s > 0);
         }
         tc_commit(&s_full[x]);
       }
+      __syncwarp();
     };
-    auto pv = [&](uint32_t x, uint32_t buf, bool first, bool last) {
-      if (lane == 0) {
-        const uint32_t vb = ring + buf * S::TILE;
+    auto pv = [&](auto xc, uint32_t buf, bool first, bool last) {
+      constexpr uint32_t x = decltype(xc)::value;
+      const uint32_t vb = __shfl_sync(FULL, desc_n(ring + buf * S::TILE, S::COL), 0);
+      const uint32_t keep = __shfl_sync(FULL, first ? 0u : 1u, 0);
+      if (elect_one()) {
 #pragma unroll
         for (uint32_t s = 0; s < S::KT / 16; ++s)
-          mma_ts(tmem + TMEM_O + 128 * x, tmem + TMEM_S + 128 * x + 8 * s, smem_desc_n(vb + s * 16 * 128, S::COL),
-                 S::IDESC_O, !first || s > 0);
+          mma_ts(ut + TMEM_O + 128 * x, ut + TMEM_S + 128 * x + 8 * s, vb + s * (16 * 128 >> 4), S::IDESC_O,
+                 s > 0 ? 1u : keep);
         if (last) tc_commit(&o_full[x]);
       }
+      __syncwarp();
+    };
+    constexpr std::integral_constant<uint32_t, 0> first_tile{};
+    constexpr std::integral_constant<uint32_t, 1> second_tile{};
+    auto commit = [&](uint64_t* bar) {
+      if (elect_one()) tc_commit(bar);
+      __syncwarp();
     };
     do {
       const uint32_t kend = w.kend(), tiles = w.tokens() > tok_tile ? 2 : 1, nt = w.kt1 - w.kt0;
       if (!wait(&q_full, items & 1) || !wait(&full[n % S::NBUF], (n / S::NBUF) & 1)) break;
-      for (uint32_t x = 0; x < tiles; ++x) qk(x, n % S::NBUF);
-      if (lane == 0) {
-        tc_commit(&empty[n % S::NBUF]);
-        if (nt == 1) tc_commit(&q_empty);
-      }
+      qk(first_tile, n % S::NBUF);
+      if (tiles == 2) qk(second_tile, n % S::NBUF);
+      commit(&empty[n % S::NBUF]);
+      if (nt == 1) commit(&q_empty);
       for (uint32_t i = 0; i < nt && ok; ++i) {
         const uint32_t v = n + 1, kn = n + 2, k0 = p.from + (w.kt0 + i) * S::KT;
         const bool more = i + 1 < nt;
@@ -256,21 +297,22 @@ __global__ void __launch_bounds__(384, 1)
           fence_proxy_async();
           __syncwarp();
         }
-        for (uint32_t x = 0; x < tiles; ++x) {
-          if (!wait(&p_full[x], p_phase[x])) break;
-          p_phase[x] ^= 1;
-          pv(x, v % S::NBUF, i == 0, !more);
-          if (more) {
-            if (x == 0 && !wait(&full[kn % S::NBUF], (kn / S::NBUF) & 1)) break;
-            qk(x, kn % S::NBUF);
-          }
+        if (!wait(&p_full[0], p_phase[0])) break;
+        p_phase[0] ^= 1;
+        pv(first_tile, v % S::NBUF, i == 0, !more);
+        if (more) {
+          if (!wait(&full[kn % S::NBUF], (kn / S::NBUF) & 1)) break;
+          qk(first_tile, kn % S::NBUF);
         }
-        if (!ok) break;
-        if (lane == 0) {
-          tc_commit(&empty[v % S::NBUF]);
-          if (more) tc_commit(&empty[kn % S::NBUF]);
-          if (i + 2 == nt) tc_commit(&q_empty);
+        if (tiles == 2) {
+          if (!wait(&p_full[1], p_phase[1])) break;
+          p_phase[1] ^= 1;
+          pv(second_tile, v % S::NBUF, i == 0, !more);
+          if (more) qk(second_tile, kn % S::NBUF);
         }
+        commit(&empty[v % S::NBUF]);
+        if (more) commit(&empty[kn % S::NBUF]);
+        if (i + 2 == nt) commit(&q_empty);
         n += 2;
       }
       ++items;
@@ -279,14 +321,12 @@ __global__ void __launch_bounds__(384, 1)
       abort_flag = 1;
       if (lane == 0 && a.seqs.status) *a.seqs.status = STATUS_TIMEOUT;
     }
-    if (lane == 0) {
-      tc_commit(&drain);  // every MMA has completed when this flips
-      mbar_wait(&drain, 0, nullptr);
-    }
+    commit(&drain);  // every MMA has completed when this flips
+    mbar_wait(&drain, 0, nullptr);
     __syncwarp();
   }
   } else {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
   if (!idle) {
     // ---- softmax: one thread per row ----
     Walk<S> w(p, tpt, start);
@@ -337,57 +377,57 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, r[c]);
           tmem_wait_ld();
-          if (p.flip) {
+          if (__builtin_expect(p.flip != 0, 0)) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
               for (int i = 0; i < 32; ++i) r[c][i] ^= 0x80000000u;
           }
-          if (k0 + S::KT > all_see) {
+          if (__any_sync(FULL, k0 + S::KT > all_see)) {
+            const uint32_t left = lim > k0 ? lim - k0 : 0;  // visible keys of the tile
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (k0 + 32 * c + i >= lim) r[c][i] = 0xFF800000u;
+                if (32u * c + i >= left) r[c][i] = 0xFF800000u;
           }
           float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
+          for (int i = 0; i < 32; i += 2)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) t[c] = fmaxf(t[c], __uint_as_float(r[c][i]));
-          const float top = fmaxf(mx, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * sc);
+            for (int c = 0; c < 4; ++c) t[c] = max3(t[c], __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1]));
+          const float top = fmaxf(mx, max3(fmaxf(t[0], t[1]), t[2], t[3]) * sc);
           // a row whose maximum has grown a lot rescales (all rows of the warp then take their own)
           if (__any_sync(FULL, top > mx + GROWN || mx == -INFINITY)) {
             const float f = ex2(mx - (top == -INFINITY ? 0.0f : top));  // 0 from -inf
             l *= f;
             mx = top;
             if (kt > w.kt0) {
-#pragma unroll
-              for (int c = 0; c < HD / 32; ++c) {
-                uint32_t o[32];
-                tmem_ld32(to + 32 * c, o);
+#pragma unroll 1
+              for (int c = 0; c < HD / 16; ++c) {  // (few registers are left beside the row of S)
+                uint32_t o[16];
+                tmem_ld16(to + 16 * c, o);
                 tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                tmem_st32(to + 32 * c, o);
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_st16(to + 16 * c, o);
               }
             }
           }
           const float ref = mx == -INFINITY ? 0.0f : mx - SHIFT;
           float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t pk[32];
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[16];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int c = 2 * h + i / 16, j = 2 * (i % 16);
-              const float u = ex2(fmaf(__uint_as_float(r[c][j]), sc, -ref));
-              const float v = ex2(fmaf(__uint_as_float(r[c][j + 1]), sc, -ref));
+            for (int i = 0; i < 16; ++i) {
+              const float u = ex2(fmaf(__uint_as_float(r[c][2 * i]), sc, -ref));
+              const float v = ex2(fmaf(__uint_as_float(r[c][2 * i + 1]), sc, -ref));
               sum[i & 1] += u;
               sum[2 + (i & 1)] += v;
               pk[i] = pack2<T>(u, v);
             }
-            tmem_st32(ts + 32 * h, pk);
+            tmem_st16(ts + 16 * c, pk);
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tmem_wait_st();
