@@ -162,6 +162,7 @@ int attention(void* output, uint64_t out_stride, int out_dtype, float* lse, cons
   if (!workspace || (uintptr_t)workspace % 256) return fail(YL_ERR_ARG, "workspace must be 256-byte aligned");
   if (workspace_bytes < need) return fail(YL_ERR_ARG, "workspace smaller than yl_paged_attention_workspace says");
   if (batch->n_rows == 0) return YL_OK;
+  if ((uint64_t)batch->n_rows * n_heads > 0x7FFFFFFFull) return fail(YL_ERR_ARG, "more than 2^31-1 rows x heads");
   a.out = output;
   a.out_stride = out_stride;
   a.lse = lse;

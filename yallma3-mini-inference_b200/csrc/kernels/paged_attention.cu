@@ -125,6 +125,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
   float* join = reinterpret_cast<float*>(smem + S::NBUF * BUF + S::Q_BYTES);
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t tpt = S::BM / p.group;
+  uint4 goes_on = make_uint4(0, 0, 0, 0);  // (warp 0) the item that goes on in the next block
 
   if (threadIdx.x == 0) {
     for (int b = 0; b < S::NBUF; ++b) {
@@ -432,10 +433,14 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
       }
       const uint32_t blocks = w.blocks(), first = w.first_block();
       const bool whole = blocks == 1;
-      if (w.kt0 == 0 && warp == 0)
-        for (uint32_t t = lane; t < ntok; t += 32)
-          p.desc[(uint64_t)(w.r.row0 + w.t + t) * a.pages.n_kv_heads + w.head] =
-              make_uint2(first, whole ? t : blocks << 16 | t);
+      if (w.kt0 == 0 && warp == 0) {
+        if (p.joined)
+          for (uint32_t t = lane; t < ntok; t += 32)
+            p.desc[(uint64_t)(w.r.row0 + w.t + t) * a.pages.n_kv_heads + w.head] =
+                make_uint2(first, whole ? t : blocks << 16 | t);
+        else if (!whole)
+          goes_on = make_uint4(w.r.row0 + w.t, ntok, w.head, blocks);
+      }
       float* const slot = p.slots + (uint64_t)(2 * blockIdx.x + (w.kt0 == 0 ? 1 : 0)) * S::BM * PART<HD>;
       auto part = [&](uint32_t mrow, uint32_t r, uint32_t h) {
         return whole ? p.rowpart + ((uint64_t)r * a.n_heads + h) * PART<HD> : slot + mrow * PART<HD>;
@@ -517,6 +522,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
       if (lane == 0 && a.seqs.status) *a.seqs.status = STATUS_TIMEOUT;
     }
   }
+  if (threadIdx.x == 0) p.cut[blockIdx.x] = goes_on;
   __syncthreads();
   grid_dep_wait();  // the launch before has ended when this one has
 }
@@ -526,73 +532,139 @@ struct JoinArgs {
   PagedAttnArgs a;
   uint32_t group, n_passes;
   struct {
+    const uint4* cut;
     const uint2* desc;
     const float* slots;
     const float* rowpart;
     uint32_t grid, bm;
   } pass[2];
-  int joined;
 };
 
-// One warp per (row, query head): lanes hold HD/32 neighbours each.
-template <typename O, int HD>
-__global__ void __launch_bounds__(256) join_kernel(JoinArgs j) {
+// Joins n parts of one (row, query head) and writes it out; part(i) is where
+// the i-th lies. `each` warps take every each-th part and meet in shared
+// memory (all of the block's threads then call this together); lanes hold
+// HD/32 neighbours.
+template <typename O, int HD, typename F>
+__device__ __forceinline__ void join_row(const PagedAttnArgs& a, uint32_t row, uint32_t head, uint32_t n, F&& part,
+                                         uint32_t first, uint32_t each, float (*meet)[PART<HD>]) {
   constexpr int PER = HD / 32;
   const uint32_t lane = threadIdx.x & 31;
-  const uint64_t id = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const PagedAttnArgs& a = j.a;
-  const uint64_t row = id / a.n_heads;
-  const uint32_t head = (uint32_t)(id % a.n_heads);
-  grid_dep_wait();
-  if (row < row_begin(a.seqs, 0) || row >= row_begin(a.seqs, a.seqs.n_seqs)) return;
   float m = -INFINITY, l = 0.0f, o[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) o[i] = 0.0f;
-  for (uint32_t ps = 0; ps < j.n_passes; ++ps) {
-    const uint2 d = j.pass[ps].desc[row * a.pages.n_kv_heads + head / j.group];
-    const uint32_t blocks = d.y >> 16, mr = (d.y & 0xFFFFu) * j.group + head % j.group;
-    uint32_t n = blocks ? blocks : 1;
-    if (!blocks && !j.joined) return;  // written by its one block
-    if (blocks && ((uint64_t)d.x + blocks > j.pass[ps].grid || mr >= j.pass[ps].bm)) return;
-    auto part = [&](uint32_t i) -> const float* {
-      if (!blocks) return j.pass[ps].rowpart + (row * a.n_heads + head) * PART<HD>;
-      const uint64_t slot = i == 0 ? 2ull * d.x + 1 : 2ull * (d.x + i);
-      return j.pass[ps].slots + (slot * j.pass[ps].bm + mr) * PART<HD>;
-    };
-    for (uint32_t i0 = 0; i0 < n; i0 += 32) {
-      const uint32_t c = min(32u, n - i0);
-      float pm = -INFINITY, pl = 0.0f;
-      if (lane < c) {
-        const float* q = part(i0 + lane);
-        pm = q[HD], pl = q[HD + 1];
-      }
-      const float top = fmaxf(m, warp_max(pm)), ref = top == -INFINITY ? 0.0f : top;
-      const float f0 = ex2(m - ref), f = ex2(pm - ref);
-      l = l * f0 + warp_sum(f * pl);
+  for (int e = 0; e < PER; ++e) o[e] = 0.0f;
+  constexpr uint32_t U = 4;  // parts in flight
+  for (uint32_t i0 = first; i0 < n; i0 += U * each) {
+    float pm[U], pl[U], po[U][PER];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) o[i] *= f0;
-      m = top;
-#pragma unroll 4
-      for (uint32_t i = 0; i < c; ++i) {
-        const float fi = __shfl_sync(FULL, f, i);
-        const float2* q = reinterpret_cast<const float2*>(part(i0 + i) + PER * lane);
+    for (uint32_t u = 0; u < U; ++u) {
+      pm[u] = -INFINITY, pl[u] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < PER / 2; ++e) {
-          const float2 v = q[e];
-          o[2 * e] += fi * v.x, o[2 * e + 1] += fi * v.y;
-        }
+      for (int e = 0; e < PER; ++e) po[u][e] = 0.0f;
+      if (i0 + u * each < n) {
+        const float* q = part(i0 + u * each);
+        const float2 ml = *reinterpret_cast<const float2*>(q + HD);
+        pm[u] = ml.x, pl[u] = ml.y;
+#pragma unroll
+        for (int e = 0; e < PER; e += 2)
+          *reinterpret_cast<float2*>(&po[u][e]) = *reinterpret_cast<const float2*>(q + PER * lane + e);
       }
+    }
+    const float top = fmaxf(m, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]))), ref = top == -INFINITY ? 0.0f : top;
+    const float f0 = ex2(m - ref);
+    m = top;
+    l *= f0;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o[e] *= f0;
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      const float f = ex2(pm[u] - ref);
+      l += f * pl[u];
+#pragma unroll
+      for (int e = 0; e < PER; ++e) o[e] += f * po[u][e];
+    }
+  }
+  if (each > 1) {
+    __syncthreads();  // the row before has been read
+#pragma unroll
+    for (int e = 0; e < PER; ++e) meet[first][PER * lane + e] = o[e];
+    if (lane == 0) meet[first][HD] = m, meet[first][HD + 1] = l;
+    __syncthreads();
+    if (first) return;
+    float top = m;
+    for (uint32_t w = 1; w < each; ++w) top = fmaxf(top, meet[w][HD]);
+    const float ref = top == -INFINITY ? 0.0f : top, f0 = ex2(m - ref);
+    m = top;
+    l *= f0;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o[e] *= f0;
+    for (uint32_t w = 1; w < each; ++w) {
+      const float f = ex2(meet[w][HD] - ref);
+      l += f * meet[w][HD + 1];
+#pragma unroll
+      for (int e = 0; e < PER; ++e) o[e] += f * meet[w][PER * lane + e];
     }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  O* out = static_cast<O*>(a.out) + row * a.out_stride + (uint64_t)head * HD + PER * lane;
+  O* out = static_cast<O*>(a.out) + (uint64_t)row * a.out_stride + (uint64_t)head * HD + PER * lane;
 #pragma unroll
-  for (int e = 0; e < PER / 2; ++e) {
-    const float x = o[2 * e] * inv, y = o[2 * e + 1] * inv;
-    if constexpr (sizeof(O) == 4) reinterpret_cast<float2*>(out)[e] = make_float2(x, y);
-    else reinterpret_cast<uint32_t*>(out)[e] = pack2<O>(x, y);
+  for (int e = 0; e < PER; e += 2) {
+    if constexpr (sizeof(O) == 4) *reinterpret_cast<float2*>(out + e) = make_float2(o[e] * inv, o[e + 1] * inv);
+    else *reinterpret_cast<uint32_t*>(out + e) = pack2<O>(o[e] * inv, o[e + 1] * inv);
   }
-  if (lane == 0 && a.lse) a.lse[row * a.n_heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+  if (lane == 0 && a.lse) a.lse[(uint64_t)row * a.n_heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
+// One pass: block x takes the item that begins in the pass's block x and goes
+// on in the next; its rows go round the grid's second dimension, eight at a
+// time with a warp each, or, where many blocks share them, one at a time.
+template <typename O, int HD>
+__global__ void __launch_bounds__(256) join_cut_kernel(JoinArgs j) {
+  __shared__ float meet[8][PART<HD>];
+  grid_dep_wait();
+  const PagedAttnArgs& a = j.a;
+  const auto& ps = j.pass[0];
+  const uint4 c = ps.cut[blockIdx.x];  // {first row, tokens, head, blocks}
+  const uint32_t rows = c.y * j.group, n = c.w, warp = threadIdx.x >> 5;
+  auto each_part = [&](uint32_t mr) {
+    return [&, mr](uint32_t i) -> const float* {
+      const uint64_t slot = i == 0 ? 2ull * blockIdx.x + 1 : 2ull * (blockIdx.x + i);
+      return ps.slots + (slot * ps.bm + mr) * PART<HD>;
+    };
+  };
+  if (n > 8) {
+    for (uint32_t mr = blockIdx.y; mr < rows; mr += gridDim.y)
+      join_row<O, HD>(a, c.x + mr / j.group, c.z * j.group + mr % j.group, n, each_part(mr), warp, 8, meet);
+  } else {
+    for (uint32_t mr = blockIdx.y * 8 + warp; mr < rows; mr += gridDim.y * 8)
+      join_row<O, HD>(a, c.x + mr / j.group, c.z * j.group + mr % j.group, n, each_part(mr), 0, 1, meet);
+  }
+}
+
+// Prefix and own parts: four warps per (row, query head).
+template <typename O, int HD>
+__global__ void __launch_bounds__(128) join_rows_kernel(JoinArgs j) {
+  __shared__ float meet[4][PART<HD>];
+  const PagedAttnArgs& a = j.a;
+  const uint32_t row = blockIdx.x / a.n_heads, head = blockIdx.x % a.n_heads;
+  grid_dep_wait();
+  if (row < row_begin(a.seqs, 0) || row >= row_begin(a.seqs, a.seqs.n_seqs)) return;
+  uint2 d[2];
+  uint32_t n[2];
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    d[p] = j.pass[p].desc[(uint64_t)row * a.pages.n_kv_heads + head / j.group];
+    n[p] = d[p].y >> 16 ? d[p].y >> 16 : 1;
+    // (row ranges that overlap or leave gaps: nothing outside the workspace is read)
+    if (d[p].y >> 16 && ((uint64_t)d[p].x + n[p] > j.pass[p].grid || (d[p].y & 0xFFFFu) >= j.pass[p].bm / j.group)) return;
+  }
+  auto part = [&](uint32_t i) -> const float* {
+    const int p = i < n[0] ? 0 : 1;
+    const uint32_t k = p ? i - n[0] : i;
+    if (!(d[p].y >> 16)) return j.pass[p].rowpart + ((uint64_t)row * a.n_heads + head) * PART<HD>;
+    const uint64_t slot = k == 0 ? 2ull * d[p].x + 1 : 2ull * (d[p].x + k);
+    return j.pass[p].slots + (slot * j.pass[p].bm + (d[p].y & 0xFFFFu) * j.group + head % j.group) * PART<HD>;
+  };
+  join_row<O, HD>(a, row, head, n[0] + n[1], part, threadIdx.x >> 5, 4, meet);
 }
 
 // ---- host --------------------------------------------------------------------
@@ -607,7 +679,7 @@ uint32_t blocks_of(uint32_t bm) { return bm == TC_TILE ? 148 : 2 * 148; }
 struct Plan {
   bool shared;        // a prefix pass of its own
   uint32_t bm[2];     // row tiles of the sequences' pass, and of the prefix pass
-  uint64_t desc[2], slots[2], rowpart[2], bytes;  // workspace offsets
+  uint64_t cut[2], desc[2], slots[2], rowpart[2], bytes;  // workspace offsets
 };
 Plan plan_of(const Pages& p, const Seqs& s, int dtype, uint32_t n_heads) {
   const uint64_t group = n_heads / p.n_kv_heads, hd = p.head_size;
@@ -625,7 +697,8 @@ Plan plan_of(const Pages& p, const Seqs& s, int dtype, uint32_t n_heads) {
     return o;
   };
   for (int i = 0; i < (pl.shared ? 2 : 1); ++i) {
-    pl.desc[i] = take((uint64_t)s.n_rows * p.n_kv_heads * 8);
+    pl.cut[i] = take(16ull * blocks_of(pl.bm[i]));
+    pl.desc[i] = pl.shared ? take((uint64_t)s.n_rows * p.n_kv_heads * 8) : 0;
     pl.slots[i] = take(2ull * blocks_of(pl.bm[i]) * pl.bm[i] * (hd + 4) * 4);
     pl.rowpart[i] = pl.shared ? take((uint64_t)s.n_rows * n_heads * (hd + 4) * 4) : 0;
   }
@@ -655,7 +728,6 @@ cudaError_t launch(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
   j.a = a;
   j.group = a.n_heads / a.pages.n_kv_heads;
   j.n_passes = pl.shared ? 2 : 1;
-  j.joined = pl.shared;
   LaunchCfg lc;
   lc.stream = stream;
   for (int i = pl.shared ? 1 : 0; i >= 0; --i) {  // the prefix first
@@ -671,10 +743,13 @@ cudaError_t launch(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
     p.from = pl.shared && !i ? a.seqs.shared_len : 0;
     p.group = j.group;
     p.min_chunk = 2;
+    p.item_cost = pl.bm[i] == TC_TILE ? 2 : 1;
     p.joined = pl.shared;
+    p.cut = reinterpret_cast<uint4*>(ws + pl.cut[i]);
     p.desc = reinterpret_cast<uint2*>(ws + pl.desc[i]);
     p.slots = reinterpret_cast<float*>(ws + pl.slots[i]);
     p.rowpart = reinterpret_cast<float*>(ws + pl.rowpart[i]);
+    j.pass[i].cut = p.cut;
     j.pass[i].desc = p.desc;
     j.pass[i].slots = p.slots;
     j.pass[i].rowpart = p.rowpart;
@@ -687,8 +762,10 @@ cudaError_t launch(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     lc.pdl = true;
   }
-  const uint64_t warps = (uint64_t)a.seqs.n_rows * a.n_heads;
-  return launch_kernel(join_kernel<O, HD>, dim3((uint32_t)((warps + 7) / 8)), dim3(256), 0, lc, j);
+  if (pl.shared)
+    return launch_kernel(join_rows_kernel<O, HD>, dim3(a.seqs.n_rows * a.n_heads), dim3(128), 0, lc, j);
+  return launch_kernel(join_cut_kernel<O, HD>, dim3(blocks_of(pl.bm[0]), pl.bm[0] == TC_TILE ? 32 : 4), dim3(256), 0, lc,
+                       j);
 }
 
 template <typename T, typename O>

@@ -25,8 +25,10 @@ struct Pass {
   uint32_t from, prefix;  // first key; 1: the prefix pass (keys 0 .. shared_len)
   uint32_t group, min_chunk;
   uint32_t grid;   // blocks
+  uint32_t item_cost;  // an item's own cost in key tiles (queries, first tile, output), when the line is cut
   int joined;      // every item leaves its part in the workspace
-  uint2* desc;     // [n_rows][n_kv_heads] {first block, blocks << 16 | token in the tile}
+  uint4* cut;      // [grid]: the item that begins in a block and goes on in the next {first row, tokens, head, blocks}
+  uint2* desc;     // joined: [n_rows][n_kv_heads] {first block, blocks << 16 | token in the tile}
   float* slots;    // [2 * grid][BM][HD + 4]: a part is O, m (in powers of two), l
   float* rowpart;  // [n_rows][n_heads][HD + 4]: items of one block, where every item leaves its part
 };
@@ -100,24 +102,25 @@ __device__ __forceinline__ uint32_t keys_end(const Pass& p, const Rows& r, uint3
   const int64_t e = r.pos0 + (t < r.n ? t : r.n);
   return e <= 0 ? 0 : e < (int64_t)r.limit ? (uint32_t)e : r.limit;
 }
-// Key tiles of the row tile that ends at token t (one where it sees no key).
+// Key tiles of the row tile that ends at token t (one where it sees no key). On
+// the line it takes item_cost units more, before its first tile.
 template <typename S>
 __device__ __forceinline__ uint32_t tiles_of(const Pass& p, const Rows& r, uint32_t t) {
   const uint32_t e = keys_end(p, r, t);
   return e > p.from + S::KT ? (e - p.from + S::KT - 1) / S::KT : 1;
 }
 template <typename S>
-__device__ __forceinline__ uint64_t tiles_per_head(const Pass& p, const Rows& r, uint32_t tpt) {
+__device__ __forceinline__ uint64_t units_per_head(const Pass& p, const Rows& r, uint32_t tpt) {
   uint64_t n = 0;
-  if (p.prefix) return (uint64_t)((r.n + tpt - 1) / tpt) * tiles_of<S>(p, r, r.n);
-  for (uint32_t t = 0; t < r.n; t += tpt) n += tiles_of<S>(p, r, t + tpt);
+  if (p.prefix) return (uint64_t)((r.n + tpt - 1) / tpt) * (tiles_of<S>(p, r, r.n) + p.item_cost);
+  for (uint32_t t = 0; t < r.n; t += tpt) n += tiles_of<S>(p, r, t + tpt) + p.item_cost;
   return n;
 }
 
 // Where a block's piece of the line begins.
 struct Start {
-  uint64_t begin, end, chunk;  // in key tiles
-  uint32_t seq, head, t, kt;   // sequence, head, first token of the row tile, key tile
+  uint64_t begin, end, chunk;  // on the line
+  uint32_t seq, head, t;       // sequence, head, first token of the row tile
   uint64_t g0;                 // where the item begins on the line
   int masked;                  // prefix pass: some row does not see all of the prefix
 };
@@ -141,7 +144,7 @@ __device__ void find_start(const Pass& p, uint32_t tpt, Start* out, uint64_t* sc
   }
   // exclusive sums of the sequences' tiles, a block's width at a time; the
   // second time over, the piece's place is looked for
-  uint64_t total = 0, begin = 0;
+  uint64_t total = 0, begin = 0, end = 0;
   for (int round = 0; round < 2; ++round) {
     uint64_t base = 0;
     for (uint32_t c = 0; c < n; c += S::THREADS) {
@@ -150,7 +153,7 @@ __device__ void find_start(const Pass& p, uint32_t tpt, Start* out, uint64_t* sc
       uint64_t per_head = 0;
       if (i < n) {
         r = rows_of(p, i);
-        per_head = tiles_per_head<S>(p, r, tpt);
+        per_head = units_per_head<S>(p, r, tpt);
       }
       const uint64_t mine = per_head * heads;
       uint64_t inc = mine;
@@ -173,17 +176,16 @@ __device__ void find_start(const Pass& p, uint32_t tpt, Start* out, uint64_t* sc
         const uint64_t h = off / per_head;
         off -= h * per_head;
         g0 += h * per_head;
-        uint32_t t = 0, nt = tiles_of<S>(p, r, tpt);
-        while (off >= nt) {
-          off -= nt;
-          g0 += nt;
+        uint32_t t = 0, units = tiles_of<S>(p, r, tpt) + p.item_cost;
+        while (off >= units) {
+          off -= units;
+          g0 += units;
           t += tpt;
-          nt = tiles_of<S>(p, r, t + tpt);
+          units = tiles_of<S>(p, r, t + tpt) + p.item_cost;
         }
-        out->seq = i;
+        if (end > g0 + p.item_cost) out->seq = i;  // else the piece ends before the item's first tile
         out->head = (uint32_t)h;
         out->t = t;
-        out->kt = (uint32_t)off;
         out->g0 = g0;
       }
       base += sum;
@@ -193,10 +195,11 @@ __device__ void find_start(const Pass& p, uint32_t tpt, Start* out, uint64_t* sc
       uint64_t chunk = (total + gridDim.x - 1) / gridDim.x;
       if (chunk < p.min_chunk) chunk = p.min_chunk;
       begin = chunk * blockIdx.x;
+      end = begin + chunk < total ? begin + chunk : total;
       if (tid == 0) {
         out->chunk = chunk;
         out->begin = begin;
-        out->end = begin + chunk < total ? begin + chunk : total;
+        out->end = end;
       }
       if (begin >= total) break;  // nothing for this block: seq stays unset
     }
@@ -206,31 +209,32 @@ __device__ void find_start(const Pass& p, uint32_t tpt, Start* out, uint64_t* sc
   __syncthreads();
 }
 
-// Walks a block's piece: one step per item, the same in every warp.
+// Walks a block's piece: one step per item that has key tiles in it, the same
+// in every warp.
 template <typename S>
 struct Walk {
   const Pass& p;
   const uint32_t tpt;
-  uint64_t at, end, chunk, g0;
+  uint64_t begin, end, chunk, g0;
   uint32_t seq, head, t, kt0, kt1, nt;
   Rows r;
 
   __device__ Walk(const Pass& pass, uint32_t tokens, const Start& s)
-      : p(pass), tpt(tokens), at(s.begin), end(s.end), chunk(s.chunk), g0(s.g0), seq(s.seq), head(s.head), t(s.t),
-        kt0(s.kt) {
+      : p(pass), tpt(tokens), begin(s.begin), end(s.end), chunk(s.chunk), g0(s.g0), seq(s.seq), head(s.head), t(s.t) {
     r = rows_of(p, seq);
-    piece();
-  }
-  __device__ void piece() {
     nt = tiles_of<S>(p, r, t + tpt);
-    const uint64_t left = end - at;
-    kt1 = nt - kt0 < left ? nt : kt0 + (uint32_t)left;
+    cut();
+  }
+  // The item's key tiles within the piece: units [g0 + item_cost, + nt).
+  __device__ bool cut() {
+    const uint64_t first = g0 + p.item_cost;
+    kt0 = begin > first ? (uint32_t)(begin - first) : 0;
+    kt1 = end > first ? (uint32_t)(end - first < nt ? end - first : nt) : 0;
+    return kt0 < kt1;
   }
   __device__ bool next() {
-    at += kt1 - kt0;
-    if (at >= end) return false;
-    g0 += nt;
-    kt0 = 0;
+    g0 += nt + p.item_cost;
+    if (g0 >= end) return false;
     t += tpt;
     if (t >= r.n) {
       t = 0;
@@ -242,14 +246,14 @@ struct Walk {
         } while (r.n == 0);
       }
     }
-    piece();
-    return true;
+    nt = tiles_of<S>(p, r, t + tpt);
+    return cut();
   }
   __device__ uint32_t tokens() const { return r.n - t < tpt ? r.n - t : tpt; }
   __device__ uint32_t kend() const { return keys_end(p, r, t + tpt); }
-  // Whole in one block, or the blocks it lies in.
-  __device__ uint32_t first_block() const { return (uint32_t)(g0 / chunk); }
-  __device__ uint32_t blocks() const { return (uint32_t)((g0 + nt - 1) / chunk) - first_block() + 1; }
+  // The blocks that the item's key tiles lie in.
+  __device__ uint32_t first_block() const { return (uint32_t)((g0 + p.item_cost) / chunk); }
+  __device__ uint32_t blocks() const { return (uint32_t)((g0 + p.item_cost + nt - 1) / chunk) - first_block() + 1; }
 };
 
 // Sequence of a row by bisection (rows inside the prefix only).

@@ -80,6 +80,14 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(yes));
   return yes != 0;
 }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " YL_V32 ";" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+               "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+               "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+               "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -87,14 +95,51 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-      "[%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "mov.b64 rc, {%6, %7};\n\tfma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "add.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+// 2^x for x up to 127 without the special-function unit, which gives 16 results
+// per clock and SM and would bound the softmax: x = n + f, |f| <= 1/2, 2^f by a
+// polynomial fitted to it by least squares of the relative error on Chebyshev
+// nodes (2^-22, as ex2.approx), times 2^n. Below -126 it stays at 2^-126, next
+// to which every weight is 0; NaN stays NaN.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  constexpr float C0 = 1.00000012f, C1 = 0.693146944f, C2 = 0.240221217f, C3 = 0.0555074252f, C4 = 0.00967545994f,
+                  C5 = 0.0013266971f;
+  constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are n
+  x = make_float2(max_nan(x.x, -126.0f), max_nan(x.y, -126.0f));
+  const float2 t = add2(x, make_float2(MAGIC, MAGIC));
+  const float2 n = add2(t, make_float2(-MAGIC, -MAGIC));
+  const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
+  float2 y = make_float2(C5, C5);
+  y = fma2(y, f, make_float2(C4, C4));
+  y = fma2(y, f, make_float2(C3, C3));
+  y = fma2(y, f, make_float2(C2, C2));
+  y = fma2(y, f, make_float2(C1, C1));
+  y = fma2(y, f, make_float2(C0, C0));
+  // n in the exponent's place: (bits of t) << 23 drops what MAGIC put above n
+  const float px = __uint_as_float((__float_as_uint(t.x) << 23) + 0x3F800000u);
+  const float py = __uint_as_float((__float_as_uint(t.y) << 23) + 0x3F800000u);
+  return make_float2(y.x * px, y.y * py);
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -130,6 +175,7 @@ __global__ void __launch_bounds__(384, 1)
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t tok_tile = 128 / p.group, tpt = 2 * tok_tile;
   const PagedAttnArgs& a = p.a;
+  uint4 goes_on = make_uint4(0, 0, 0, 0);  // (warp 0) the item that goes on in the next block
 
   if (threadIdx.x == 0) {
     for (int b = 0; b < S::NBUF; ++b) {
@@ -203,7 +249,7 @@ __global__ void __launch_bounds__(384, 1)
         for (uint32_t kv = 0; kv < 2; ++kv, ++n) {
           const uint32_t b = n % S::NBUF;
           if (n >= (uint32_t)S::NBUF) {
-            ok = mbar_wait(&empty[b], (n / S::NBUF - 1) & 1, nullptr) && !abort_flag;
+            ok = mbar_wait(&empty[b], (n / S::NBUF - 1) & 1, nullptr);
             ok = __all_sync(FULL, ok);
             if (!ok) break;
           }
@@ -232,48 +278,40 @@ __global__ void __launch_bounds__(384, 1)
     uint32_t n = 0, items = 0, p_phase[2] = {0, 0};
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      ok = ok && mbar_wait(bar, parity, nullptr) && !abort_flag;
-      ok = __all_sync(FULL, ok);
+      ok = __all_sync(FULL, mbar_wait(bar, parity, nullptr));
       tc_fence_after();
       return ok;
     };
-    // An MMA takes its descriptors from uniform registers. Issued by a lane that
-    // elect.sync names, from values that come out of a shuffle, eight cost 64
-    // cycles each, what the tensor cores need; by a lane picked with lane == 0
-    // they cost 130.
-    const uint32_t ut = __shfl_sync(FULL, tmem, 0);
-    const uint32_t uq = __shfl_sync(FULL, desc_k(q_smem), 0);
+    // Issued by the lane that elect.sync names (not one picked by its number):
+    // only then an MMA's descriptors go to its uniform registers directly, and
+    // it costs the 64 cycles that the tensor cores need, not 130.
     auto qk = [&](auto xc, uint32_t buf) {
       constexpr uint32_t x = decltype(xc)::value;
-      const uint32_t kb = __shfl_sync(FULL, desc_k(ring + buf * S::TILE), 0);
       if (elect_one()) {
+        const uint32_t q = desc_k(q_smem + x * S::TILE), kb = desc_k(ring + buf * S::TILE);
 #pragma unroll
         for (uint32_t s = 0; s < HD / 16; ++s) {
           const uint32_t off = ((s >> 2) * S::COL + (s & 3) * 32) >> 4;
-          mma_ss(ut + TMEM_S + 128 * x, uq + x * (S::TILE >> 4) + off, kb + off, S::IDESC_S, s > 0);
+          mma_ss(tmem + TMEM_S + 128 * x, q + off, kb + off, S::IDESC_S, s > 0);
         }
         tc_commit(&s_full[x]);
       }
-      __syncwarp();
     };
     auto pv = [&](auto xc, uint32_t buf, bool first, bool last) {
       constexpr uint32_t x = decltype(xc)::value;
-      const uint32_t vb = __shfl_sync(FULL, desc_n(ring + buf * S::TILE, S::COL), 0);
-      const uint32_t keep = __shfl_sync(FULL, first ? 0u : 1u, 0);
       if (elect_one()) {
+        const uint32_t vb = desc_n(ring + buf * S::TILE, S::COL);
 #pragma unroll
         for (uint32_t s = 0; s < S::KT / 16; ++s)
-          mma_ts(ut + TMEM_O + 128 * x, ut + TMEM_S + 128 * x + 8 * s, vb + s * (16 * 128 >> 4), S::IDESC_O,
-                 s > 0 ? 1u : keep);
+          mma_ts(tmem + TMEM_O + 128 * x, tmem + TMEM_S + 128 * x + 8 * s, vb + s * (16 * 128 >> 4), S::IDESC_O,
+                 s > 0 || !first);
         if (last) tc_commit(&o_full[x]);
       }
-      __syncwarp();
     };
     constexpr std::integral_constant<uint32_t, 0> first_tile{};
     constexpr std::integral_constant<uint32_t, 1> second_tile{};
     auto commit = [&](uint64_t* bar) {
       if (elect_one()) tc_commit(bar);
-      __syncwarp();
     };
     do {
       const uint32_t kend = w.kend(), tiles = w.tokens() > tok_tile ? 2 : 1, nt = w.kt1 - w.kt0;
@@ -341,9 +379,12 @@ __global__ void __launch_bounds__(384, 1)
       const uint32_t tok = m / p.group + t0, gh = m % p.group;
       if (warp == 0 && w.kt0 == 0) {
         const uint32_t first = w.first_block(), blocks = w.blocks();
-        for (uint32_t t = lane; t < all; t += 32)
-          p.desc[(uint64_t)(w.r.row0 + w.t + t) * a.pages.n_kv_heads + w.head] =
-              make_uint2(first, blocks == 1 ? t : blocks << 16 | t);
+        if (p.joined)
+          for (uint32_t t = lane; t < all; t += 32)
+            p.desc[(uint64_t)(w.r.row0 + w.t + t) * a.pages.n_kv_heads + w.head] =
+                make_uint2(first, blocks == 1 ? t : blocks << 16 | t);
+        else if (blocks > 1)
+          goes_on = make_uint4(w.r.row0 + w.t, all, w.head, blocks);
       }
       if (all <= t0) continue;  // this row tile has no rows (no barrier of it moves)
       const bool live = m < tok_tile * p.group && tok < all;
@@ -367,69 +408,86 @@ __global__ void __launch_bounds__(384, 1)
 
       for (uint32_t kt = w.kt0; kt < w.kt1; ++kt) {
         const uint32_t k0 = p.from + kt * S::KT;
-        ok = mbar_wait(&s_full[x], s_phase, nullptr) && !abort_flag;
+        ok = mbar_wait(&s_full[x], s_phase, nullptr);
         ok = __all_sync(FULL, ok);
         if (!ok) break;
         s_phase ^= 1;
         tc_fence_after();
         if (busy) {
           uint32_t r[4][32];
+          auto load = [&] {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, r[c]);
-          tmem_wait_ld();
-          if (__builtin_expect(p.flip != 0, 0)) {
+            for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, r[c]);
+            tmem_wait_ld();
+            if (__builtin_expect(p.flip != 0, 0)) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+              for (int c = 0; c < 4; ++c)
 #pragma unroll
-              for (int i = 0; i < 32; ++i) r[c][i] ^= 0x80000000u;
+                for (int i = 0; i < 32; ++i) r[c][i] ^= 0x80000000u;
+            }
+            if (__any_sync(FULL, k0 + S::KT > all_see)) {
+              const uint32_t left = lim > k0 ? lim - k0 : 0;  // visible keys of the tile
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (32u * c + i >= left) r[c][i] = 0xFF800000u;
+            }
+          };
+          load();
+          // Weights and the tile's maximum in one go, relative to the maximum so
+          // far; if that turns out to have grown by more than GROWN in a row of
+          // the warp, which is rare after an item's first tile, O and l are
+          // rescaled and the weights taken again.
+          uint32_t pk[4][16];
+          float2 sum[4];
+          float t[4];
+          auto weights = [&](float ref) {
+            const float2 sc2 = make_float2(sc, sc), ref2 = make_float2(-ref, -ref);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sum[c] = make_float2(0.0f, 0.0f), t[c] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const float2 s2 = make_float2(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1]));
+                const float2 e = fma2(s2, sc2, ref2);
+                const float2 w2 = (i + c) % 4 == 3 ? exp2_fma(e) : make_float2(ex2(e.x), ex2(e.y));
+                t[c] = max3(t[c], s2.x, s2.y);
+                sum[c] = add2(sum[c], w2);
+                pk[c][i] = pack2<T>(w2.x, w2.y);
+              }
+          };
+          if (kt == w.kt0) {  // no maximum yet: the tile's first
+#pragma unroll
+            for (int c = 0; c < 4; ++c) t[c] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 32; i += 2)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) t[c] = max3(t[c], __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1]));
+            mx = max3(fmaxf(t[0], t[1]), t[2], t[3]) * sc;
           }
-          if (__any_sync(FULL, k0 + S::KT > all_see)) {
-            const uint32_t left = lim > k0 ? lim - k0 : 0;  // visible keys of the tile
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (32u * c + i >= left) r[c][i] = 0xFF800000u;
-          }
-          float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int i = 0; i < 32; i += 2)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) t[c] = max3(t[c], __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1]));
+          weights(mx == -INFINITY ? 0.0f : mx - SHIFT);
           const float top = fmaxf(mx, max3(fmaxf(t[0], t[1]), t[2], t[3]) * sc);
-          // a row whose maximum has grown a lot rescales (all rows of the warp then take their own)
-          if (__any_sync(FULL, top > mx + GROWN || mx == -INFINITY)) {
+          if (__any_sync(FULL, top > mx + GROWN)) {
             const float f = ex2(mx - (top == -INFINITY ? 0.0f : top));  // 0 from -inf
             l *= f;
             mx = top;
-            if (kt > w.kt0) {
 #pragma unroll 1
-              for (int c = 0; c < HD / 16; ++c) {  // (few registers are left beside the row of S)
-                uint32_t o[16];
-                tmem_ld16(to + 16 * c, o);
-                tmem_wait_ld();
+            for (int c = 0; c < HD / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(to + 32 * c, o);
+              tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                tmem_st16(to + 16 * c, o);
-              }
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st32(to + 32 * c, o);
             }
+            load();  // (the row and its weights together are more than a thread's registers)
+            weights(mx == -INFINITY ? 0.0f : mx - SHIFT);
           }
-          const float ref = mx == -INFINITY ? 0.0f : mx - SHIFT;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float u = ex2(fmaf(__uint_as_float(r[c][2 * i]), sc, -ref));
-              const float v = ex2(fmaf(__uint_as_float(r[c][2 * i + 1]), sc, -ref));
-              sum[i & 1] += u;
-              sum[2 + (i & 1)] += v;
-              pk[i] = pack2<T>(u, v);
-            }
-            tmem_st16(ts + 16 * c, pk);
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          for (int c = 0; c < 4; ++c) tmem_st16(ts + 16 * c, pk[c]);
+          l += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) + ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
           tmem_wait_st();
         }
         tc_fence_before();
@@ -439,14 +497,14 @@ __global__ void __launch_bounds__(384, 1)
       if (!ok) break;
 
       // ---- the item's end ----
-      ok = mbar_wait(&o_full[x], o_phase, nullptr) && !abort_flag;
+      ok = mbar_wait(&o_full[x], o_phase, nullptr);
       ok = __all_sync(FULL, ok);
       if (!ok) break;
       o_phase ^= 1;
       tc_fence_after();
       if (busy) {
         const bool whole = w.blocks() == 1, direct = whole && !p.joined;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = mx == -INFINITY && l == l ? 0.0f : 1.0f / l;
         float* part = whole ? p.rowpart + ((uint64_t)row * a.n_heads + head) * PART<HD>
                             : p.slots + ((uint64_t)(2 * blockIdx.x + (w.kt0 == 0 ? 1 : 0)) * TC_TILE + tok * p.group + gh) * PART<HD>;
         O* out = static_cast<O*>(a.out) + (uint64_t)row * a.out_stride + (uint64_t)head * HD;
@@ -483,13 +541,14 @@ __global__ void __launch_bounds__(384, 1)
         }
         if (live) {
           if (!direct) part[HD] = mx - SHIFT, part[HD + 1] = l;
-          else if (a.lse) a.lse[(uint64_t)row * a.n_heads + head] = l == 0.0f ? -INFINITY : (mx - SHIFT + log2f(l)) * LN2;
+          else if (a.lse) a.lse[(uint64_t)row * a.n_heads + head] = mx == -INFINITY && l == l ? -INFINITY : (mx - SHIFT + log2f(l)) * LN2;
         }
       }
       tc_fence_before();  // O has been read before the next item's first product, which waits for its weights
     } while (w.next());
     if (!ok) abort_flag = 1;
   }
+  if (threadIdx.x == 0) p.cut[blockIdx.x] = goes_on;
   }
   tc_fence_before();
   __syncthreads();
