@@ -1,14 +1,16 @@
 // Log probabilities of given tokens, entropy and the most likely tokens of
 // rows of logits, in one pass over each row.
 //
-// With m = max x, taken at index i*: S' = sum over i != i* of exp(x_i - m) and
-// W = sum of exp(x_i - m) (x_i - m) give
-//   lse = m + log1p(S'),  logprob(t) = x_t - lse,  entropy = log1p(S') - W / (1 + S').
-// Keeping the largest term out of S' keeps the digits of log probabilities
-// near 0. Partial (m, S', W) join as
-//   m1 >= m2, d = m2 - m1:  S' = S1 + e^d (1 + S2),  W = W1 + e^d (W2 + d (1 + S2)).
+// With m = max x: S = sum of exp(x_i - m) and W = sum of exp(x_i - m) (x_i - m) give
+//   logprob(t) = (x_t - m) - log S,  entropy = log S - W / S.
+// Partial (m, S, W) join as
+//   m1 >= m2, d = m2 - m1:  S = S1 + e^d S2,  W = W1 + e^d (W2 + d S2).
+// S is 1 + S', S' the sum without the largest term, and log S = log1p(S'). Where
+// S' is small (a nearly certain token), S - 1 has lost its digits: such a row's
+// S' is summed again without that term, from L2, so that log probabilities near
+// 0 keep theirs.
 //
-// Most likely tokens: every thread keeps the largest of the values it reads.
+// Most likely tokens: every thread knows the largest of the values it reads.
 // The k-th largest of the threads' maxima bounds the k-th largest value from
 // below, and only the k threads at or above it can hold one of the k largest,
 // so only their values (a few per cent of the row) are read a second time.
@@ -32,7 +34,7 @@ using namespace yl::dev;
 
 namespace {
 
-constexpr uint32_t LP_THREADS = 512;
+constexpr uint32_t LP_THREADS = 256;
 constexpr uint32_t LP_WARPS = LP_THREADS / 32;
 constexpr uint32_t LP_CAND = 1024;  // candidates ranked at once
 
@@ -47,23 +49,33 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t key_index(uint64_t key) { return 0xFFFFFFFFu - (uint32_t)key; }
 
-// Differences to the maximum are taken no lower: exp is 0 there in f32, and a
-// product with it is 0 too, where -inf, or the lowest f32 times a sum, would
-// give NaN.
-constexpr float FLOOR = -200.0f;
+// Exponents (in powers of two) are taken no lower in a product with their
+// power: that is 0 in f32 there, and so is the product, where -inf, or the
+// lowest f32, would give NaN.
+constexpr float FLOOR = -256.0f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// m; S = sum of 2^d and W = sum of 2^d d, d = (x - m) log2(e). The difference is
+// taken first: x log2(e) may be beyond f32 where x is a mask of the lowest value.
 struct Part {
   float m, s, w;
 };
 __device__ __forceinline__ Part join(Part a, Part b) {
-  if (b.m > a.m) {
-    const Part t = a;
-    a = b;
-    b = t;
-  }
-  if (b.m == -INFINITY) return a;  // no value (a NaN sum stays with a, see below)
-  const float d = fmaxf(b.m - a.m, FLOOR), f = __expf(d);
-  return {a.m, a.s + f * (1.0f + b.s), a.w + f * (b.w + d * (1.0f + b.s))};
+  const float m = fmaxf(a.m, b.m), r = m == -INFINITY ? 0.0f : m;
+  const float da = fmaxf((a.m - r) * LOG2E, FLOOR), db = fmaxf((b.m - r) * LOG2E, FLOOR);
+  const float fa = ex2(da), fb = ex2(db);
+  return {m, fa * a.s + fb * b.s, fa * (a.w + da * a.s) + fb * (b.w + db * b.s)};
 }
 __device__ __forceinline__ Part warp_join(Part p) {
 #pragma unroll
@@ -71,7 +83,6 @@ __device__ __forceinline__ Part warp_join(Part p) {
     p = join(p, Part{__shfl_xor_sync(FULL, p.m, o), __shfl_xor_sync(FULL, p.s, o), __shfl_xor_sync(FULL, p.w, o)});
   return p;
 }
-
 // Sorts a warp's 32 keys, largest in lane 0 (bitonic network).
 __device__ __forceinline__ uint64_t warp_sort_desc(uint64_t v, uint32_t lane) {
 #pragma unroll
@@ -149,53 +160,68 @@ struct LpShared {
   uint64_t red[LP_WARPS];
   uint32_t n_group, n_cand;
   Part whole;
+  float rest[LP_WARPS], whole_rest;
   uint64_t top[32];  // this block's largest keys, in order
 };
 
-// A thread's running (m, S', W) and the index of m.
+// A thread's running (m, S, W), and which of its batches of values had m.
 struct Run {
   float m = -INFINITY, s = 0.0f, w = 0.0f;
-  uint32_t idx = 0xFFFFFFFFu;
+  uint32_t batch = 0;
 
-  // N consecutive values, the first at index `first`.
-  template <uint32_t N>
-  __device__ __forceinline__ void add(const float (&v)[N], uint32_t first) {
-    float top = v[0];
+  template <uint32_t N, bool W>
+  __device__ __forceinline__ void add(const float (&v)[N], uint32_t number) {
+    float top[2] = {v[0], -INFINITY};
 #pragma unroll
-    for (uint32_t i = 1; i < N; ++i) top = fmaxf(top, v[i]);
-    if (idx == 0xFFFFFFFFu) idx = first;  // the lowest index stands for a part of nothing but -inf
-    if (top > m) {
-      uint32_t at = 0;
-#pragma unroll
-      for (uint32_t i = N; i-- > 0;)
-        if (v[i] == top) at = i;
-      if (m != -INFINITY) {
-        const float d = fmaxf(m - top, FLOOR), f = __expf(d);
-        w = f * (w + d * (1.0f + s));
-        s = f * (1.0f + s);
-      }
-      m = top;
-      idx = first + at;
-#pragma unroll
-      for (uint32_t i = 0; i < N; ++i) {
-        const float d = v[i] - top, e = i == at ? 0.0f : __expf(d);
-        s += e;
-        w = fmaf(e, fmaxf(d, FLOOR), w);
-      }
+    for (uint32_t i = 1; i < N; i += 2) top[(i / 2) & 1] = i + 1 < N ? max3(top[(i / 2) & 1], v[i], v[i + 1]) : fmaxf(top[(i / 2) & 1], v[i]);
+    const float mn = max3(m, top[0], top[1]), r = mn == -INFINITY ? 0.0f : mn;
+    if (mn > m) {
+      batch = number;
+      const float d0 = fmaxf((m - r) * LOG2E, FLOOR), f = ex2(d0);
+      if (W) w = f * (w + d0 * s);
+      s *= f;
+      m = mn;
+    }
+    if constexpr (N == 1) {
+      const float d = (v[0] - r) * LOG2E, e = ex2(d);
+      s += e;
+      if (W) w = fmaf(e, fmaxf(d, FLOOR), w);
     } else {
-      const float ref = m == -INFINITY ? 0.0f : m;
+      const float2 l2 = make_float2(LOG2E, LOG2E), r2 = make_float2(-r, -r);
+      float2 es = make_float2(0.0f, 0.0f), ws = es;
 #pragma unroll
-      for (uint32_t i = 0; i < N; ++i) {
-        const float d = v[i] - ref, e = __expf(d);
-        s += e;
-        w = fmaf(e, fmaxf(d, FLOOR), w);
+      for (uint32_t i = 0; i < N; i += 2) {
+        const float2 d = mul2(add2(make_float2(v[i], v[i + 1]), r2), l2), e = make_float2(ex2(d.x), ex2(d.y));
+        es = add2(es, e);
+        if (W) ws = fma2(e, make_float2(fmaxf(d.x, FLOOR), fmaxf(d.y, FLOOR)), ws);
       }
+      s += es.x + es.y;
+      if (W) w += ws.x + ws.y;
     }
   }
 };
 
+// S' of a block's part of the row: the sum without the values equal to m (the
+// caller knows that there is one).
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(LogprobArgs a) {
+__device__ float sum_without(const Row<T>& part, float m) {
+  float s = 0.0f;
+  const uint32_t tid = threadIdx.x;
+  auto add = [&](float v) { s += v == m ? 0.0f : ex2((v - m) * LOG2E); };
+  if (tid < part.head) add(to_f32(part.x[part.begin + tid]));
+  for (uint32_t v = tid; v < part.vecs; v += LP_THREADS) {
+    float o[Row<T>::PER];
+    part.load(v, o);
+#pragma unroll
+    for (uint32_t i = 0; i < Row<T>::PER; ++i) add(o[i]);
+  }
+  if (part.vec_index(part.vecs) + tid < part.end) add(to_f32(part.x[part.vec_index(part.vecs) + tid]));
+  return s;
+}
+
+// W: the entropy is asked for.
+template <typename T, bool W>
+__global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(LogprobArgs a) {
   __shared__ LpShared sh;
   const cg::cluster_group cluster = cg::this_cluster();
   const uint32_t C = cluster.num_blocks(), rank = cluster.block_rank();
@@ -212,40 +238,53 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(LogprobArgs a) {
   const uint32_t each = (a.vocab + C - 1) / C;
   const uint32_t b = min(rank * each, a.vocab), e = min(b + each, a.vocab);
   const Row<T> part(x, b, e);
-  constexpr uint32_t PER = Row<T>::PER;
+  constexpr uint32_t PER = Row<T>::PER, U = 2;  // 32 bytes in flight per thread, a batch
 
   Run r;
+  const uint32_t batches = part.vecs > tid ? (part.vecs - tid + LP_THREADS - 1) / LP_THREADS : 0;  // of one load each
+  const uint32_t tail = part.vec_index(part.vecs) + tid;
   if (tid < part.head) {
     const float v[1] = {to_f32(x[part.begin + tid])};
-    r.add(v, part.begin + tid);
+    r.template add<1, W>(v, 0xFFFFFFFEu);
   }
-  constexpr uint32_t U = 64 / 16;  // 64 bytes in flight per thread
-  uint32_t v = tid;
-  for (; v + (U - 1) * LP_THREADS < part.vecs; v += U * LP_THREADS) {
-    float o[U][PER];
+  uint32_t n = 0;
+  for (; n + U <= batches; n += U) {
+    float o[U * PER];
 #pragma unroll
-    for (uint32_t u = 0; u < U; ++u) part.load(v + u * LP_THREADS, o[u]);
-#pragma unroll
-    for (uint32_t u = 0; u < U; ++u) r.add(o[u], part.vec_index(v + u * LP_THREADS));
+    for (uint32_t u = 0; u < U; ++u) part.load(tid + (n + u) * LP_THREADS, *reinterpret_cast<float(*)[PER]>(o + u * PER));
+    r.template add<U * PER, W>(o, n);
   }
-  for (; v < part.vecs; v += LP_THREADS) {
+  for (; n < batches; ++n) {
     float o[PER];
-    part.load(v, o);
-    r.add(o, part.vec_index(v));
+    part.load(tid + n * LP_THREADS, o);
+    r.template add<PER, W>(o, n);
   }
-  const uint32_t tail = part.vec_index(part.vecs) + tid;
   if (tail < e) {
     const float o[1] = {to_f32(x[tail])};
-    r.add(o, tail);
+    r.template add<1, W>(o, 0xFFFFFFFFu);
   }
-  // a part without a value keeps m = -inf; a NaN among them left a NaN sum
+  // a NaN left its mark in the sum alone
   const bool nan = isnan(r.s);
   if (nan) r.m = INFINITY;
   const Part p = warp_join(Part{r.m, r.s, r.w});
   if (lane == 0) sh.part[warp] = p;
 
   if (a.top_k) {
-    const uint64_t mine = r.idx == 0xFFFFFFFFu || nan ? 0ull : key_of(r.m, r.idx);
+    // where the thread's largest value lies: the first of its batch that equals it
+    // (a part of nothing but -inf: its first value)
+    uint32_t idx = 0xFFFFFFFFu;
+    if (tid < part.head && (r.batch == 0xFFFFFFFEu || r.m == -INFINITY)) idx = part.begin + tid;
+    else if (batches && (r.batch < 0xFFFFFFFEu || r.m == -INFINITY)) {
+      const uint32_t n0 = r.m == -INFINITY ? 0 : r.batch, n1 = min(n0 + (n0 + U <= batches && n0 % U == 0 ? U : 1u), batches);
+      for (uint32_t k = n0; k < n1 && idx == 0xFFFFFFFFu; ++k) {
+        float o[PER];
+        part.load(tid + k * LP_THREADS, o);
+#pragma unroll
+        for (uint32_t i = PER; i-- > 0;)
+          if (o[i] == r.m) idx = part.vec_index(tid + k * LP_THREADS) + i;
+      }
+    } else if (tail < e) idx = tail;
+    const uint64_t mine = idx == 0xFFFFFFFFu || nan ? 0ull : key_of(r.m, idx);
     sh.list[warp][lane] = warp_sort_desc(mine, lane);
     if (tid == 0) sh.n_group = sh.n_cand = 0;
     join_lists(sh.list, LP_WARPS, warp, lane);
@@ -302,26 +341,43 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(LogprobArgs a) {
     const Part q = warp_join(lane < LP_WARPS ? sh.part[lane] : Part{-INFINITY, 0.0f, 0.0f});
     if (lane == 0) sh.whole = q;
   }
-  // ---- join the cluster's blocks ----
+  // ---- join the cluster's blocks: every block has the row's (m, S, W) ----
   if (C > 1) cluster.sync();
   else __syncthreads();
-  if (rank == 0) {
-    if (warp < C && a.top_k) {
-      const LpShared* other = C > 1 ? cluster.map_shared_rank(&sh, warp) : &sh;
-      sh.list[warp][lane] = other->top[lane];
+  Part q = {-INFINITY, 0.0f, 0.0f};
+  if (lane < C) q = C > 1 ? cluster.map_shared_rank(&sh, lane)->whole : sh.whole;
+  q = warp_join(q);
+  // NaN, +inf, or nothing above -inf: no distribution
+  const bool none = isnan(q.s) || fabsf(q.m) == INFINITY;
+  float rest = q.s - 1.0f;  // S'
+  if (!none && rest < 0.0078125f) {
+    // nearly certain: 2^-24 of 1 is more than 2^-17 of S'
+    float s = sum_without(part, q.m);
+    s = warp_sum(s);
+    if (lane == 0) sh.rest[warp] = s;
+    __syncthreads();
+    if (tid == 0) {
+      float t = 0.0f;
+      for (uint32_t w = 0; w < LP_WARPS; ++w) t += sh.rest[w];
+      sh.whole_rest = t;
     }
-    Part q = {-INFINITY, 0.0f, 0.0f};
-    if (warp == 0 && lane < C) q = C > 1 ? cluster.map_shared_rank(&sh, lane)->whole : sh.whole;
-    if (a.top_k) join_lists(sh.list, C, warp, lane);
+    if (C > 1) cluster.sync();
+    else __syncthreads();
+    rest = 0.0f;
+    if (lane < C) rest = C > 1 ? cluster.map_shared_rank(&sh, lane)->whole_rest : sh.whole_rest;
+    rest = warp_sum(rest);
+  }
+  if (rank == 0) {
+    if (a.top_k) {
+      if (warp < C) sh.list[warp][lane] = C > 1 ? cluster.map_shared_rank(&sh, warp)->top[lane] : sh.top[lane];
+      join_lists(sh.list, C, warp, lane);
+    }
     if (warp == 0) {
-      q = warp_join(q);
-      // NaN, +inf, or nothing above -inf: no distribution
-      const bool none = isnan(q.s) || fabsf(q.m) == INFINITY;
       const float nanf_ = __int_as_float(0x7FC00000);
-      const float log_sum = log1pf(q.s);
+      const float log_sum = log1pf(rest);
       if (lane == 0) {
         if (a.tokens) a.logprobs[row] = none || token < 0 ? nanf_ : (xt - q.m) - log_sum;
-        if (a.entropy) a.entropy[row] = none ? nanf_ : log_sum - q.w / (1.0f + q.s);
+        if (W) a.entropy[row] = none ? nanf_ : log_sum - q.w * LN2 / (1.0f + rest);
       }
       if (lane < a.top_k) {
         const uint64_t key = sh.list[0][lane];
@@ -330,15 +386,15 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(LogprobArgs a) {
       }
     }
   }
-  if (C > 1) cluster.sync();  // the other blocks' shared memory stays until it has been read
+  if (C > 1) cluster.sync();  // the blocks' shared memory stays until all have read it
 }
 
-template <typename T>
-cudaError_t launch(const LogprobArgs& a, cudaStream_t stream) {
-  // blocks per row: enough to have two on every SM, while each still reads
+template <typename T, bool W>
+cudaError_t launch_w(const LogprobArgs& a, cudaStream_t stream) {
+  // blocks per row: enough to have one on every SM, while each still reads
   // 4096 values or more
   uint32_t c = 1;
-  while (c < 8 && (uint64_t)a.n_rows * c < 2 * 148 && a.vocab / (2 * c) >= 4096) c *= 2;
+  while (c < 8 && (uint64_t)a.n_rows * c < 148 && a.vocab / (2 * c) >= 4096) c *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.n_rows * c);
   cfg.blockDim = dim3(LP_THREADS);
@@ -349,7 +405,12 @@ cudaError_t launch(const LogprobArgs& a, cudaStream_t stream) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, a);
+  return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, W>, a);
+}
+
+template <typename T>
+cudaError_t launch(const LogprobArgs& a, cudaStream_t stream) {
+  return a.entropy ? launch_w<T, true>(a, stream) : launch_w<T, false>(a, stream);
 }
 
 }  // namespace
