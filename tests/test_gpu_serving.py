@@ -231,13 +231,19 @@ def test_garbage_behind_the_sequences(yl, torch_cuda, dtype, bad):
 
 def test_not_finite_keys_reach_their_readers_only(yl, torch_cuda):
     """NaN in one sequence's cache stays in that sequence."""
-    g = ref.Geometry(12, 4, 2, 64, page=16, lens=[40, 50, 60], rows=[1, 1, 1])
-    for t in DTYPES.values():
-        q, (k, v) = queries(g, t).cuda(), (x.cuda() for x in g.pool(t))
-        clean, _ = attend(yl, g, q, k, v, 0.125)
-        k[int(g.table[1, 0]), 3] = math.nan
-        got, lse = attend(yl, g, q, k, v, 0.125)
-        assert torch.equal(got[[0, 2]], clean[[0, 2]]) and got[1].isnan().all() and lse[1].isnan().all()
+    for rows in ([1, 1, 1], [20, 30, 40]):
+        g = ref.Geometry(12, 4, 2, 64, page=16, lens=[40, 50, 60], rows=rows)
+        mine = slice(rows[0], rows[0] + rows[1])
+        others = [i for i in range(sum(rows)) if i not in range(mine.start, mine.stop)]
+        for t in DTYPES.values():
+            for bits in (0x7FFFFFFF, 0x7FC00000, -1):  # all ones, as arithmetic makes it, and torch's, and a negative one
+                q, (k, v) = queries(g, t).cuda(), (x.cuda() for x in g.pool(t))
+                clean, _ = attend(yl, g, q, k, v, 0.125)
+                ints = torch.int32 if t == torch.float32 else torch.int16
+                k.view(ints)[int(g.table[1, 0]), 3] = bits if t == torch.float32 else (bits >> 16 if bits > 0 else -1)
+                assert k[int(g.table[1, 0]), 3].isnan().all()
+                got, lse = attend(yl, g, q, k, v, 0.125)
+                assert torch.equal(got[others], clean[others]) and got[mine].isnan().all() and lse[mine].isnan().all()
 
 
 def test_bad_pages_and_missing_slots(yl, torch_cuda):

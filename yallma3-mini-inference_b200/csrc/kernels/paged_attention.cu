@@ -28,7 +28,7 @@
 // the tile's keys and join at the item's end. Decoding has 1..16 rows per
 // item and is bound by reading the cache, so WK = 4; from 33 rows on WK = 1.
 // f32 operands are split into two tf32 numbers and multiplied as hi*hi + hi*lo
-// + lo*hi (2^-22 relative); 16-bit ones are exact, and the softmax weights are
+// + lo*hi (2^-21 relative); 16-bit ones are exact, and the softmax weights are
 // rounded to their type for the second product (the sum l takes them
 // unrounded), f16 weights at 2^10 times their value so that small ones do not
 // fall below f16's range.
@@ -82,10 +82,13 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo in tf32, off by at most 2^-23 of x (each part rounded to 11 bits)
+// x = hi + lo in tf32, off by at most 2^-21 of x: hi is x rounded to 11 bits
+// (in integers; cvt.rna.tf32 takes as long as an MMA), lo the exact rest, of
+// which the MMA reads the upper 11 bits. A NaN whose hi would overflow to 0
+// stays a NaN in lo.
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+  hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -127,6 +130,10 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
   const uint32_t tpt = S::BM / p.group;
   uint4 goes_on = make_uint4(0, 0, 0, 0);  // (warp 0) the item that goes on in the next block
 
+  if (threadIdx.x == 32 * S::NW) {
+    prefetch_map(&map_k);
+    prefetch_map(&map_v);
+  }
   if (threadIdx.x == 0) {
     for (int b = 0; b < S::NBUF; ++b) {
       mbar_init(&full[b], 1);
@@ -673,11 +680,15 @@ uint32_t tile_rows(uint64_t rows, int dtype) {
   if (dtype != DT_F32 && rows > 32) return TC_TILE;
   return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
-uint32_t blocks_of(uint32_t bm) { return bm == TC_TILE ? 148 : 2 * 148; }
+// Two blocks per SM; two passes that both leave room for the other get one each
+// and run side by side.
+uint32_t blocks_of(uint32_t bm, bool beside) { return bm == TC_TILE || beside ? 148 : 2 * 148; }
+
 
 // What a call launches, by its counts alone.
 struct Plan {
   bool shared;        // a prefix pass of its own
+  bool beside;        // the two passes run side by side
   uint32_t bm[2];     // row tiles of the sequences' pass, and of the prefix pass
   uint64_t cut[2], desc[2], slots[2], rowpart[2], bytes;  // workspace offsets
 };
@@ -690,6 +701,7 @@ Plan plan_of(const Pages& p, const Seqs& s, int dtype, uint32_t n_heads) {
   pl.shared = s.shared_len && s.n_seqs > 1 && each <= 32;
   pl.bm[0] = tile_rows(each, dtype);
   pl.bm[1] = tile_rows((uint64_t)s.n_rows * group, dtype);
+  pl.beside = pl.shared && pl.bm[0] != TC_TILE && pl.bm[1] != TC_TILE;
   uint64_t at = 0;
   auto take = [&](uint64_t n) {
     const uint64_t o = at;
@@ -697,9 +709,9 @@ Plan plan_of(const Pages& p, const Seqs& s, int dtype, uint32_t n_heads) {
     return o;
   };
   for (int i = 0; i < (pl.shared ? 2 : 1); ++i) {
-    pl.cut[i] = take(16ull * blocks_of(pl.bm[i]));
+    pl.cut[i] = take(16ull * blocks_of(pl.bm[i], pl.beside));
     pl.desc[i] = pl.shared ? take((uint64_t)s.n_rows * p.n_kv_heads * 8) : 0;
-    pl.slots[i] = take(2ull * blocks_of(pl.bm[i]) * pl.bm[i] * (hd + 4) * 4);
+    pl.slots[i] = take(2ull * blocks_of(pl.bm[i], pl.beside) * pl.bm[i] * (hd + 4) * 4);
     pl.rowpart[i] = pl.shared ? take((uint64_t)s.n_rows * n_heads * (hd + 4) * 4) : 0;
   }
   pl.bytes = at;
@@ -738,11 +750,11 @@ cudaError_t launch(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
     p.sc = sc < 1.2e-38 ? 1.2e-38f : (float)sc;  // not 0: times -inf it stays -inf
     p.sc_lo = std::isfinite(p.sc) ? (float)(sc - (double)p.sc) : 0.0f;
     p.flip = a.scale < 0.0f;
-    p.grid = blocks_of(pl.bm[i]);
+    p.grid = blocks_of(pl.bm[i], pl.beside);
     p.prefix = i;
     p.from = pl.shared && !i ? a.seqs.shared_len : 0;
     p.group = j.group;
-    p.min_chunk = 2;
+    p.min_chunk = dtype == DT_F32 ? 1 : 2;  // (an f32 tile takes as long as joining its part)
     p.item_cost = pl.bm[i] == TC_TILE ? 2 : 1;
     p.joined = pl.shared;
     p.cut = reinterpret_cast<uint4*>(ws + pl.cut[i]);
@@ -764,7 +776,7 @@ cudaError_t launch(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
   }
   if (pl.shared)
     return launch_kernel(join_rows_kernel<O, HD>, dim3(a.seqs.n_rows * a.n_heads), dim3(128), 0, lc, j);
-  return launch_kernel(join_cut_kernel<O, HD>, dim3(blocks_of(pl.bm[0]), pl.bm[0] == TC_TILE ? 32 : 4), dim3(256), 0, lc,
+  return launch_kernel(join_cut_kernel<O, HD>, dim3(blocks_of(pl.bm[0], pl.beside), pl.bm[0] == TC_TILE ? 32 : 4), dim3(256), 0, lc,
                        j);
 }
 

@@ -71,6 +71,9 @@ __device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, u
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(tok), "r"(page), "r"(smem_u32(bar))
       : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // ---- work ------------------------------------------------------------------
 // A sequence as a pass sees it.
@@ -125,55 +128,72 @@ struct Start {
   int masked;                  // prefix pass: some row does not see all of the prefix
 };
 
+__device__ __forceinline__ uint64_t div_up(uint64_t a, uint32_t b) {
+  return a < 0xFFFF0000u ? ((uint32_t)a + b - 1) / b : (a + b - 1) / b;
+}
+__device__ __forceinline__ uint32_t div_small(uint64_t a, uint64_t b) {
+  return (uint32_t)((a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b);
+}
+
+// All threads. The sequences' units are summed a block's width at a time; where
+// one width holds them all, as it mostly does, they are looked at once.
 template <typename S>
 __device__ void find_start(const Pass& p, uint32_t tpt, Start* out, uint64_t* scratch) {
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t n = p.prefix ? 1 : p.a.seqs.n_seqs;
-  const uint32_t heads = p.a.pages.n_kv_heads;
   constexpr uint32_t NWARPS = S::THREADS / 32;
-  __shared__ int any_masked;
-  if (tid == 0) any_masked = 0, out->seq = 0xFFFFFFFFu;
-  __syncthreads();
-  if (p.prefix) {  // rows inside the prefix
-    bool m = false;
+  Rows r{};
+  uint64_t per_head = 0, mine = 0, first = 0;  // this thread's sequence of the width: units, and where they begin
+  auto width = [&](uint32_t c, uint64_t base) -> uint64_t {
+    const uint32_t i = c + tid;
+    per_head = 0;
+    if (i < n) {
+      r = rows_of(p, i);
+      per_head = units_per_head<S>(p, r, tpt);
+    }
+    mine = per_head * p.a.pages.n_kv_heads;
+    uint64_t inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t v = __shfl_up_sync(FULL, inc, o);
+      if ((int)lane >= o) inc += v;
+    }
+    if (lane == 31) scratch[warp] = inc;
+    __syncthreads();
+    uint64_t before = base, sum = 0;
+    for (uint32_t w = 0; w < NWARPS; ++w) {
+      if (w < warp) before += scratch[w];
+      sum += scratch[w];
+    }
+    first = before + inc - mine;
+    return sum;
+  };
+  bool masked = false;
+  if (p.prefix)  // rows inside the prefix
     for (uint32_t i = tid; i < p.a.seqs.n_seqs; i += S::THREADS) {
       const uint32_t rn = row_end(p.a.seqs, i) - row_begin(p.a.seqs, i);
-      m |= rn && (int64_t)p.a.seqs.seq_len[i] - rn + 1 < (int64_t)p.a.seqs.shared_len;
+      masked |= rn && (int64_t)p.a.seqs.seq_len[i] - rn + 1 < (int64_t)p.a.seqs.shared_len;
     }
-    if (m) any_masked = 1;
+  if (tid == 0) out->seq = 0xFFFFFFFFu;
+  uint64_t total = width(0, 0);
+  for (uint32_t c = S::THREADS; c < n; c += S::THREADS) {
+    __syncthreads();
+    total += width(c, 0);
   }
-  // exclusive sums of the sequences' tiles, a block's width at a time; the
-  // second time over, the piece's place is looked for
-  uint64_t total = 0, begin = 0, end = 0;
-  for (int round = 0; round < 2; ++round) {
+  uint64_t chunk = div_up(total, gridDim.x);
+  if (chunk < p.min_chunk) chunk = p.min_chunk;
+  const uint64_t begin = chunk * blockIdx.x, end = begin + chunk < total ? begin + chunk : total;
+  if (tid == 0) out->chunk = chunk, out->begin = begin, out->end = end;
+  if (begin < total) {
     uint64_t base = 0;
     for (uint32_t c = 0; c < n; c += S::THREADS) {
-      const uint32_t i = c + tid;
-      Rows r{};
-      uint64_t per_head = 0;
-      if (i < n) {
-        r = rows_of(p, i);
-        per_head = units_per_head<S>(p, r, tpt);
+      if (n > S::THREADS) {
+        __syncthreads();
+        base += width(c, base);
       }
-      const uint64_t mine = per_head * heads;
-      uint64_t inc = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t v = __shfl_up_sync(FULL, inc, o);
-        if ((int)lane >= o) inc += v;
-      }
-      __syncthreads();
-      if (lane == 31) scratch[warp] = inc;
-      __syncthreads();
-      uint64_t before = base, sum = 0;
-      for (uint32_t w = 0; w < NWARPS; ++w) {
-        if (w < warp) before += scratch[w];
-        sum += scratch[w];
-      }
-      const uint64_t first = before + inc - mine;
-      if (round == 1 && begin >= first && begin < first + mine) {
+      if (begin >= first && begin < first + mine) {
         uint64_t off = begin - first, g0 = first;
-        const uint64_t h = off / per_head;
+        const uint32_t h = div_small(off, per_head);
         off -= h * per_head;
         g0 += h * per_head;
         uint32_t t = 0, units = tiles_of<S>(p, r, tpt) + p.item_cost;
@@ -183,30 +203,15 @@ __device__ void find_start(const Pass& p, uint32_t tpt, Start* out, uint64_t* sc
           t += tpt;
           units = tiles_of<S>(p, r, t + tpt) + p.item_cost;
         }
-        if (end > g0 + p.item_cost) out->seq = i;  // else the piece ends before the item's first tile
-        out->head = (uint32_t)h;
+        if (end > g0 + p.item_cost) out->seq = c + tid;  // else the piece ends before the item's first tile
+        out->head = h;
         out->t = t;
         out->g0 = g0;
       }
-      base += sum;
-    }
-    if (round == 0) {
-      total = base;
-      uint64_t chunk = (total + gridDim.x - 1) / gridDim.x;
-      if (chunk < p.min_chunk) chunk = p.min_chunk;
-      begin = chunk * blockIdx.x;
-      end = begin + chunk < total ? begin + chunk : total;
-      if (tid == 0) {
-        out->chunk = chunk;
-        out->begin = begin;
-        out->end = end;
-      }
-      if (begin >= total) break;  // nothing for this block: seq stays unset
     }
   }
-  __syncthreads();
-  if (tid == 0) out->masked = any_masked;
-  __syncthreads();
+  // (also the barrier that makes *out visible)
+  out->masked = __syncthreads_or(masked);
 }
 
 // Walks a block's piece: one step per item that has key tiles in it, the same
@@ -252,8 +257,8 @@ struct Walk {
   __device__ uint32_t tokens() const { return r.n - t < tpt ? r.n - t : tpt; }
   __device__ uint32_t kend() const { return keys_end(p, r, t + tpt); }
   // The blocks that the item's key tiles lie in.
-  __device__ uint32_t first_block() const { return (uint32_t)((g0 + p.item_cost) / chunk); }
-  __device__ uint32_t blocks() const { return (uint32_t)((g0 + p.item_cost + nt - 1) / chunk) - first_block() + 1; }
+  __device__ uint32_t first_block() const { return div_small(g0 + p.item_cost, chunk); }
+  __device__ uint32_t blocks() const { return div_small(g0 + p.item_cost + nt - 1, chunk) - first_block() + 1; }
 };
 
 // Sequence of a row by bisection (rows inside the prefix only).

@@ -160,6 +160,11 @@ __global__ void __launch_bounds__(384, 1)
   const PagedAttnArgs& a = p.a;
   uint4 goes_on = make_uint4(0, 0, 0, 0);  // (warp 0) the item that goes on in the next block
 
+  if (threadIdx.x == 32 * 9) {
+    prefetch_map(&map_q);
+    prefetch_map(&map_k);
+    prefetch_map(&map_v);
+  }
   if (threadIdx.x == 0) {
     for (int b = 0; b < S::NBUF; ++b) {
       mbar_init(&full[b], 1);
