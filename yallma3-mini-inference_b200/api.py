@@ -358,63 +358,65 @@ class DType(enum.IntEnum):
 ROPE_GGUF, ROPE_LLAMA3 = 0, 1
 
 
-_torch = None  # set at the first serving call, with the table below
+_torch = None  # set at the first serving call, with what the calls below take from it
 _dtypes: dict = {}
+_f32 = _i32 = _u8 = _device = _stream_of = None
 
 
 def _load_torch():
-    global _torch
+    global _torch, _f32, _i32, _u8, _device, _stream_of
     import torch
     _dtypes.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    _f32, _i32, _u8 = torch.float32, torch.int32, torch.uint8
+    torch.cuda.init()
+    _device, _stream_of = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
     _torch = torch
-    return torch
 
 
-def _here(what: str, *tensors) -> int:
-    """The current device, on which the tensors have to be (raw addresses and None pass)."""
-    dev = (_torch or _load_torch()).cuda.current_device()
-    for t in tensors:
-        if t is not None and not isinstance(t, int) and t.get_device() != dev:
-            raise ValueError(f"{what}: every tensor must be on the current CUDA device")
-    return dev
-
-
-def _dtype(t, what: str, want: Optional[int] = None) -> int:
+def _dtype(t, what: str) -> int:
     d = _dtypes.get(t.dtype)
-    if d is None or (want is not None and d != want):
-        raise TypeError(f"{what} must be {'float32, float16 or bfloat16' if want is None else DType(want).name}, "
-                        f"got {t.dtype}")
+    if d is None:
+        raise TypeError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
     return d
 
 
-def _flat(t, what: str, dtype, numel: int):
-    """Address of a contiguous tensor of the type that holds numel values (raw addresses and None pass)."""
+def _flat(t, what: str, dtype, numel: int, dev: int):
+    """Address of a contiguous tensor of the type on the device that holds numel values (None and addresses pass)."""
     if t is None or isinstance(t, int):
         return t
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
     if t.numel() < numel or not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous and hold {numel} values, got shape {tuple(t.shape)}")
+    if t.get_device() != dev:
+        raise ValueError(f"{what} must be on the current CUDA device")
     return t.data_ptr()
 
 
-def _row_stride(t, what: str, width: int, n_rows: int) -> int:
-    """Elements between the rows of a tensor [rows, width] or [rows, heads, head_size], rows consecutive inside."""
+def _row_stride(t, what: str, width: int, n_rows: int, dev: int) -> int:
+    """Elements between the rows of a tensor [rows, width] or [rows, heads, head_size] on the device, rows
+    consecutive inside."""
     shape, stride = t.shape, t.stride()
     if len(shape) == 2:
-        ok = shape[1] == width and (stride[1] == 1 or width == 1)
+        rows, w = shape
+        ok = w == width and (stride[1] == 1 or w == 1)
+    elif len(shape) == 3:
+        rows, h, hd = shape
+        ok = h * hd == width and stride[2] == 1 and (stride[1] == hd or h == 1)
     else:
-        ok = len(shape) == 3 and shape[1] * shape[2] == width and stride[2] == 1 and (stride[1] == shape[2] or shape[1] == 1)
-    if not ok or shape[0] < n_rows:
+        ok = False
+    if not ok or rows < n_rows:
         raise ValueError(f"{what} must hold {n_rows} rows of {width} consecutive values, got shape {tuple(shape)}, "
                          f"strides {stride}")
-    return stride[0] if shape[0] > 1 else width
+    if t.get_device() != dev:
+        raise ValueError(f"{what} must be on the current CUDA device")
+    return stride[0] if rows > 1 else width
 
 
 def _raw_stream(stream, dev: int) -> int:
     """cudaStream_t of `stream` (torch's current stream where it is None)."""
     if stream is None:
-        return _torch._C._cuda_getCurrentRawStream(dev)
+        return _stream_of(dev)
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
@@ -424,6 +426,7 @@ class KvPages:
     def __init__(self, c: KvPagesC, keep=None):
         self.c = c
         self.ref = C.byref(c)
+        self.dtype, self.n_kv_heads, self.head_size = c.dtype, c.n_kv_heads, c.head_size
         self._keep = keep
 
     @classmethod
@@ -438,14 +441,17 @@ class KvPages:
         consecutive; transposed and sliced tensors are fine)."""
         if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.stride(3) != 1:
             raise ValueError("k and v must be [n_pages, page_size, n_kv_heads, head_size], alike, last axis consecutive")
-        _here("pages", k, v)
+        if _torch is None:
+            _load_torch()
+        if k.get_device() != _device() or v.get_device() != _device():
+            raise ValueError("k and v must be on the current CUDA device")
         n, ps, h, hd = k.shape
         sp, st, sh, _ = (max(x, hd) for x in k.stride())
         return cls(KvPagesC(_dtype(k, "pages"), 0, n, ps, h, hd, sp, st, sh, k.data_ptr(), v.data_ptr()), (k, v))
 
     def free(self) -> None:
         if self.c.owned and self.c.k:
-            _lib.yl_kv_pages_free(C.byref(self.c))
+            _lib.yl_kv_pages_free(self.ref)
 
     def __del__(self):
         try:
@@ -459,15 +465,17 @@ class SeqBatch:
     page_table [n_seqs, slots]; status: one int32, set to -6 (YL_ERR_RANGE) for a bad page or position."""
 
     def __init__(self, row_start, seq_len, page_table, n_rows: int, shared_len: int = 0, status=None):
-        n = seq_len.numel()
-        _here("batch", row_start, seq_len, page_table, status)
+        if _torch is None:
+            _load_torch()
+        n, dev = seq_len.numel(), _device()
         if page_table.dim() != 2 or page_table.shape[0] != n:
             raise ValueError("page_table must be [n_seqs, slots]")
-        i32 = _torch.int32
         self._keep = (row_start, seq_len, page_table, status)
-        self.c = SeqBatchC(n, n_rows, page_table.shape[1], shared_len, _flat(row_start, "row_start", i32, n + 1),
-                           _flat(seq_len, "seq_len", i32, n), _flat(page_table, "page_table", i32, page_table.numel()),
-                           _flat(status, "status", i32, 1))
+        self.n_rows = n_rows
+        self.c = SeqBatchC(n, n_rows, page_table.shape[1], shared_len,
+                           _flat(row_start, "row_start", _i32, n + 1, dev), _flat(seq_len, "seq_len", _i32, n, dev),
+                           _flat(page_table, "page_table", _i32, page_table.numel(), dev),
+                           _flat(status, "status", _i32, 1, dev))
         self.ref = C.byref(self.c)
 
 
@@ -476,21 +484,21 @@ def paged_append(qkv, pages: KvPages, batch: SeqBatch, n_heads: int, rope_cs=Non
     """Rotates the new rows' queries and keys and writes keys and values to their pages (yl_paged_append). qkv: f32
     rows [q | k | v]; q_out: rows of rotated queries in the cache's type, or None; rope_cs: [len, head_size/2, 2]
     (or an address from Transformer.rope_table, with rope_len), or None for no rotation."""
-    p, n = pages.c, batch.c.n_rows
-    hd = p.head_size
-    dev = _here("paged_append", qkv, q_out, rope_cs)
-    _dtype(qkv, "qkv", DType.F32)
+    n, hd, dev = batch.n_rows, pages.head_size, _device()
+    if qkv.dtype is not _f32:
+        raise TypeError(f"qkv must be float32, got {qkv.dtype}")
     q_ptr = q_stride = 0
     if q_out is not None:
-        _dtype(q_out, "q_out", p.dtype)
-        q_ptr, q_stride = q_out.data_ptr(), _row_stride(q_out, "q_out", n_heads * hd, n)
+        if _dtypes.get(q_out.dtype) != pages.dtype:
+            raise TypeError(f"q_out must have the cache's type, got {q_out.dtype}")
+        q_ptr, q_stride = q_out.data_ptr(), _row_stride(q_out, "q_out", n_heads * hd, n, dev)
     if rope_cs is not None and not isinstance(rope_cs, int):
         rows = rope_cs.shape[0]
         rope_len = rows if rope_len is None else min(rope_len, rows)
-        rope_cs = _flat(rope_cs, "rope_cs", _torch.float32, rows * hd)
+        rope_cs = _flat(rope_cs, "rope_cs", _f32, rows * hd, dev)
     rc = _lib.yl_paged_append(q_ptr, q_stride, qkv.data_ptr(),
-                              _row_stride(qkv, "qkv", (n_heads + 2 * p.n_kv_heads) * hd, n), pages.ref, batch.ref,
-                              n_heads, rope_cs, rope_len or 0, rope_mode, _raw_stream(stream, dev))
+                              _row_stride(qkv, "qkv", (n_heads + 2 * pages.n_kv_heads) * hd, n, dev), pages.ref,
+                              batch.ref, n_heads, rope_cs, rope_len or 0, rope_mode, _raw_stream(stream, dev))
     if rc:
         _check(rc)
 
@@ -507,14 +515,14 @@ def paged_attention(output, q, pages: KvPages, batch: SeqBatch, n_heads: int, at
     """Causal attention of the batch's rows over the paged cache (yl_paged_attention). q: rows of the cache's type,
     output: rows of that type or f32 ([rows, n_heads, head_size] or flat); lse: f32 [rows, n_heads] or None;
     workspace: a uint8 tensor of at least paged_attention_workspace bytes."""
-    p, n = pages.c, batch.c.n_rows
-    width = n_heads * p.head_size
-    dev = _here("paged_attention", output, q, workspace, lse)
-    _dtype(q, "q", p.dtype)
+    n, dev = batch.n_rows, _device()
+    width = n_heads * pages.head_size
+    if _dtypes.get(q.dtype) != pages.dtype:
+        raise TypeError(f"q must have the cache's type, got {q.dtype}")
     rc = _lib.yl_paged_attention(
-        output.data_ptr(), _row_stride(output, "output", width, n), _dtype(output, "output"),
-        _flat(lse, "lse", _torch.float32, n * n_heads), q.data_ptr(), _row_stride(q, "q", width, n), pages.ref,
-        batch.ref, n_heads, attn_scale, _flat(workspace, "workspace", _torch.uint8, 1), workspace.numel(),
+        output.data_ptr(), _row_stride(output, "output", width, n, dev), _dtype(output, "output"),
+        _flat(lse, "lse", _f32, n * n_heads, dev), q.data_ptr(), _row_stride(q, "q", width, n, dev), pages.ref,
+        batch.ref, n_heads, attn_scale, _flat(workspace, "workspace", _u8, 1, dev), workspace.numel(),
         _raw_stream(stream, dev))
     if rc:
         _check(rc)
@@ -525,16 +533,15 @@ def token_logprobs(logits, tokens=None, logprobs=None, entropy=None, top_ids=Non
     """Log probabilities of the given tokens, entropies and most likely tokens of rows of logits [rows, vocab]
     (yl_token_logprobs). Device tensors: tokens int32 [rows], logprobs and entropy f32 [rows], top_ids int32 and
     top_logprobs f32 [rows, k]; each of the three groups may be left out."""
-    if logits.dim() != 2:
-        raise ValueError("logits must be [rows, vocab]")
+    if _torch is None:
+        _load_torch()
     n, vocab = logits.shape
-    k = 0 if top_ids is None else top_ids.shape[-1]
-    dev = _here("token_logprobs", logits, tokens, logprobs, entropy, top_ids, top_logprobs)
-    f, i = _torch.float32, _torch.int32
+    k, dev = 0 if top_ids is None else top_ids.shape[-1], _device()
     rc = _lib.yl_token_logprobs(
-        logits.data_ptr(), _dtype(logits, "logits"), _row_stride(logits, "logits", vocab, n), n, vocab,
-        _flat(tokens, "tokens", i, n), _flat(logprobs, "logprobs", f, n), _flat(entropy, "entropy", f, n), k,
-        _flat(top_ids, "top_ids", i, n * k), _flat(top_logprobs, "top_logprobs", f, n * k), _raw_stream(stream, dev))
+        logits.data_ptr(), _dtype(logits, "logits"), _row_stride(logits, "logits", vocab, n, dev), n, vocab,
+        _flat(tokens, "tokens", _i32, n, dev), _flat(logprobs, "logprobs", _f32, n, dev),
+        _flat(entropy, "entropy", _f32, n, dev), k, _flat(top_ids, "top_ids", _i32, n * k, dev),
+        _flat(top_logprobs, "top_logprobs", _f32, n * k, dev), _raw_stream(stream, dev))
     if rc:
         _check(rc)
 
