@@ -711,8 +711,8 @@ Plan plan_of(const Pages& p, const Seqs& s, int dtype, uint32_t n_heads) {
   for (int i = 0; i < (pl.shared ? 2 : 1); ++i) {
     pl.cut[i] = take(16ull * blocks_of(pl.bm[i], pl.beside));
     pl.desc[i] = pl.shared ? take((uint64_t)s.n_rows * p.n_kv_heads * 8) : 0;
-    pl.slots[i] = take(2ull * blocks_of(pl.bm[i], pl.beside) * pl.bm[i] * (hd + 4) * 4);
-    pl.rowpart[i] = pl.shared ? take((uint64_t)s.n_rows * n_heads * (hd + 4) * 4) : 0;
+    pl.slots[i] = take(2ull * blocks_of(pl.bm[i], pl.beside) * pl.bm[i] * (hd + 8) * 4);
+    pl.rowpart[i] = pl.shared ? take((uint64_t)s.n_rows * n_heads * (hd + 8) * 4) : 0;
   }
   pl.bytes = at;
   return pl;

@@ -29,12 +29,12 @@ struct Pass {
   int joined;      // every item leaves its part in the workspace
   uint4* cut;      // [grid]: the item that begins in a block and goes on in the next {first row, tokens, head, blocks}
   uint2* desc;     // joined: [n_rows][n_kv_heads] {first block, blocks << 16 | token in the tile}
-  float* slots;    // [2 * grid][BM][HD + 4]: a part is O, m (in powers of two), l
-  float* rowpart;  // [n_rows][n_heads][HD + 4]: items of one block, where every item leaves its part
+  float* slots;    // [2 * grid][BM][HD + 8]: a part is O, m (in powers of two), l
+  float* rowpart;  // [n_rows][n_heads][HD + 8]: items of one block, where every item leaves its part
 };
 
 template <int HD>
-constexpr uint32_t PART = HD + 4;  // floats of a part, a multiple of 16 bytes
+constexpr uint32_t PART = HD + 8;  // floats of a part, a multiple of 32 bytes
 constexpr uint32_t TC_TILE = 256;  // rows of an item of attend_tc
 
 // The pass on the 5th-generation tensor cores: items of up to TC_TILE rows,
@@ -112,11 +112,32 @@ __device__ __forceinline__ uint32_t tiles_of(const Pass& p, const Rows& r, uint3
   const uint32_t e = keys_end(p, r, t);
   return e > p.from + S::KT ? (e - p.from + S::KT - 1) / S::KT : 1;
 }
+__device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+  return v;
+}
+__device__ __forceinline__ Rows rows_from_lane(const Rows& r, int src) {
+  return Rows{__shfl_sync(FULL, r.row0, src), __shfl_sync(FULL, r.n, src), __shfl_sync(FULL, r.pos0, src),
+              __shfl_sync(FULL, r.limit, src)};
+}
+// Units of a sequence on the line, per head; every lane its own sequence. Those
+// of many row tiles (long prompts) are counted by the whole warp, in turn.
 template <typename S>
-__device__ __forceinline__ uint64_t units_per_head(const Pass& p, const Rows& r, uint32_t tpt) {
+__device__ __forceinline__ uint64_t units_per_head(const Pass& p, const Rows& r, uint32_t tpt, uint32_t lane) {
+  const uint32_t tiles = (r.n + tpt - 1) / tpt;
+  if (p.prefix) return (uint64_t)tiles * (tiles_of<S>(p, r, r.n) + p.item_cost);
   uint64_t n = 0;
-  if (p.prefix) return (uint64_t)((r.n + tpt - 1) / tpt) * (tiles_of<S>(p, r, r.n) + p.item_cost);
-  for (uint32_t t = 0; t < r.n; t += tpt) n += tiles_of<S>(p, r, t + tpt) + p.item_cost;
+  if (tiles <= 4)
+    for (uint32_t t = 0; t < r.n; t += tpt) n += tiles_of<S>(p, r, t + tpt) + p.item_cost;
+  for (uint32_t many = __ballot_sync(FULL, tiles > 4); many; many &= many - 1) {
+    const int src = __ffs(many) - 1;
+    const Rows w = rows_from_lane(r, src);
+    uint64_t part = 0;
+    for (uint32_t t = lane * tpt; t < w.n; t += 32 * tpt) part += tiles_of<S>(p, w, t + tpt) + p.item_cost;
+    part = warp_sum_u64(part);
+    if ((int)lane == src) n = part;
+  }
   return n;
 }
 
@@ -146,11 +167,8 @@ __device__ void find_start(const Pass& p, uint32_t tpt, Start* out, uint64_t* sc
   uint64_t per_head = 0, mine = 0, first = 0;  // this thread's sequence of the width: units, and where they begin
   auto width = [&](uint32_t c, uint64_t base) -> uint64_t {
     const uint32_t i = c + tid;
-    per_head = 0;
-    if (i < n) {
-      r = rows_of(p, i);
-      per_head = units_per_head<S>(p, r, tpt);
-    }
+    r = i < n ? rows_of(p, i) : Rows{};
+    per_head = units_per_head<S>(p, r, tpt, lane);
     mine = per_head * p.a.pages.n_kv_heads;
     uint64_t inc = mine;
 #pragma unroll
@@ -191,22 +209,49 @@ __device__ void find_start(const Pass& p, uint32_t tpt, Start* out, uint64_t* sc
         __syncthreads();
         base += width(c, base);
       }
-      if (begin >= first && begin < first + mine) {
-        uint64_t off = begin - first, g0 = first;
-        const uint32_t h = div_small(off, per_head);
-        off -= h * per_head;
-        g0 += h * per_head;
-        uint32_t t = 0, units = tiles_of<S>(p, r, tpt) + p.item_cost;
-        while (off >= units) {
-          off -= units;
-          g0 += units;
-          t += tpt;
-          units = tiles_of<S>(p, r, t + tpt) + p.item_cost;
+      const uint32_t here = __ballot_sync(FULL, begin >= first && begin < first + mine);
+      if (here) {  // in one of this warp's sequences: all lanes look for the row tile
+        const int src = __ffs(here) - 1;
+        const Rows w = rows_from_lane(r, src);
+        const uint64_t each = __shfl_sync(FULL, per_head, src);
+        uint64_t g0 = __shfl_sync(FULL, first, src), off = begin - g0;
+        const uint32_t h = div_small(off, each);
+        off -= h * each;
+        g0 += h * each;
+        uint32_t t = 0;
+        if (p.prefix) {
+          const uint32_t units = tiles_of<S>(p, w, w.n) + p.item_cost, k = div_small(off, units);
+          t = k * tpt;
+          g0 += (uint64_t)k * units;
+        } else {
+          while (t < w.n) {  // 32 row tiles at a time
+            const uint32_t mt = t + lane * tpt;
+            const uint32_t units = mt < w.n ? tiles_of<S>(p, w, mt + tpt) + p.item_cost : 0;
+            uint64_t upto = units;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const uint64_t v = __shfl_up_sync(FULL, upto, o);
+              if ((int)lane >= o) upto += v;
+            }
+            const uint32_t in = __ballot_sync(FULL, upto > off);
+            if (in) {
+              const int k = __ffs(in) - 1;
+              t += k * tpt;
+              g0 += __shfl_sync(FULL, upto - units, k);
+              break;
+            }
+            const uint64_t all = __shfl_sync(FULL, upto, 31);
+            off -= all;
+            g0 += all;
+            t += 32 * tpt;
+          }
         }
-        if (end > g0 + p.item_cost) out->seq = c + tid;  // else the piece ends before the item's first tile
-        out->head = h;
-        out->t = t;
-        out->g0 = g0;
+        if (lane == 0) {
+          if (end > g0 + p.item_cost) out->seq = c + warp * 32 + src;  // else the piece ends before the item's first tile
+          out->head = h;
+          out->t = t;
+          out->g0 = g0;
+        }
       }
     }
   }

@@ -95,6 +95,19 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
       : "memory");
 }
+// Waits for the loads before; the registers pass through, so that nothing reads them earlier.
+#define YL_RW32(p) "+r"(p[0]), "+r"(p[1]), "+r"(p[2]), "+r"(p[3]), "+r"(p[4]), "+r"(p[5]), "+r"(p[6]), "+r"(p[7]), \
+                   "+r"(p[8]), "+r"(p[9]), "+r"(p[10]), "+r"(p[11]), "+r"(p[12]), "+r"(p[13]), "+r"(p[14]),       \
+                   "+r"(p[15]), "+r"(p[16]), "+r"(p[17]), "+r"(p[18]), "+r"(p[19]), "+r"(p[20]), "+r"(p[21]),     \
+                   "+r"(p[22]), "+r"(p[23]), "+r"(p[24]), "+r"(p[25]), "+r"(p[26]), "+r"(p[27]), "+r"(p[28]),     \
+                   "+r"(p[29]), "+r"(p[30]), "+r"(p[31])
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&a)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : YL_RW32(a)::"memory");
+}
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&a)[32], uint32_t (&b)[32]) {
+  tmem_wait_ld(a);
+  asm volatile("" : YL_RW32(b)::"memory");
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
@@ -130,6 +143,17 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 32 bytes in one store (a thread writes its row: fewer of them, fewer trips), or two where 16 bytes is the alignment.
+__device__ __forceinline__ void store32(void* to, const uint32_t* v, bool wide) {
+  if (wide)
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+  else {
+    static_cast<uint4*>(to)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    static_cast<uint4*>(to)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+  }
+}
 // 3-D tiled load: (element, head, row).
 __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t head, uint32_t row,
                                          uint64_t* bar) {
@@ -406,7 +430,8 @@ __global__ void __launch_bounds__(384, 1)
           auto load = [&] {
 #pragma unroll
             for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, r[c]);
-            tmem_wait_ld();
+            tmem_wait_ld(r[0], r[1]);
+            tmem_wait_ld(r[2], r[3]);
             if (__builtin_expect(p.flip != 0, 0)) {
 #pragma unroll
               for (int c = 0; c < 4; ++c)
@@ -465,7 +490,7 @@ __global__ void __launch_bounds__(384, 1)
             for (int c = 0; c < HD / 32; ++c) {
               uint32_t o[32];
               tmem_ld32(to + 32 * c, o);
-              tmem_wait_ld();
+              tmem_wait_ld(o);
 #pragma unroll
               for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
               tmem_st32(to + 32 * c, o);
@@ -496,34 +521,29 @@ __global__ void __launch_bounds__(384, 1)
         float* part = whole ? p.rowpart + ((uint64_t)row * a.n_heads + head) * PART<HD>
                             : p.slots + ((uint64_t)(2 * blockIdx.x + (w.kt0 == 0 ? 1 : 0)) * TC_TILE + tok * p.group + gh) * PART<HD>;
         O* out = static_cast<O*>(a.out) + (uint64_t)row * a.out_stride + (uint64_t)head * HD;
+        const bool wide = (reinterpret_cast<uintptr_t>(a.out) | (a.out_stride * sizeof(O))) % 32 == 0;
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t o[32];
           tmem_ld32(to + 32 * c, o);
-          tmem_wait_ld();
+          tmem_wait_ld(o);
           if (live) {
             if (direct) {
 #pragma unroll
               for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
               if constexpr (sizeof(O) == 2) {
+                uint32_t v[16];
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                  uint4 v;
-                  v.x = pack2<O>(__uint_as_float(o[i]), __uint_as_float(o[i + 1]));
-                  v.y = pack2<O>(__uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
-                  v.z = pack2<O>(__uint_as_float(o[i + 4]), __uint_as_float(o[i + 5]));
-                  v.w = pack2<O>(__uint_as_float(o[i + 6]), __uint_as_float(o[i + 7]));
-                  *reinterpret_cast<uint4*>(out + 32 * c + i) = v;
-                }
+                for (int i = 0; i < 16; ++i) v[i] = pack2<O>(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+#pragma unroll
+                for (int i = 0; i < 16; i += 8) store32(out + 32 * c + 2 * i, v + i, wide);
               } else {
 #pragma unroll
-                for (int i = 0; i < 32; i += 4)
-                  *reinterpret_cast<uint4*>(out + 32 * c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                for (int i = 0; i < 32; i += 8) store32(out + 32 * c + i, o + i, wide);
               }
             } else {
 #pragma unroll
-              for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<uint4*>(part + 32 * c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              for (int i = 0; i < 32; i += 8) store32(part + 32 * c + i, o + i, true);
             }
           }
         }
