@@ -223,7 +223,7 @@ __device__ void find_start(const Pass& p, uint32_t tpt, Start* out, uint64_t* sc
           const uint32_t units = tiles_of<S>(p, w, w.n) + p.item_cost, k = div_small(off, units);
           t = k * tpt;
           g0 += (uint64_t)k * units;
-        } else {
+        } else if (w.n > tpt) {
           while (t < w.n) {  // 32 row tiles at a time
             const uint32_t mt = t + lane * tpt;
             const uint32_t units = mt < w.n ? tiles_of<S>(p, w, mt + tpt) + p.item_cost : 0;

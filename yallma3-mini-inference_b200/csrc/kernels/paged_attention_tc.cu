@@ -20,9 +20,11 @@
 // the tile before, so O is at rest while its rows are rescaled.
 //
 // Warps: 0-3 softmax of the first row tile, 4-7 of the second (warp w reads
-// tensor-memory lanes 32 (w % 4) ..), 8 issues the MMAs, 9 loads Q (a box of
-// group heads x tokens), and keys and values page by page, 10 and 11 only hand
-// their registers to the softmax warps (a row of S is 128 registers).
+// tensor-memory lanes 32 (w % 4) ..), 8 and 10 issue the MMAs of the first and
+// the second (one's waiting is hidden behind the other's MMAs; the tensor cores
+// hold only a few in advance), 9 loads Q (a box of group heads x tokens), and keys
+// and values page by page, 11 only hands its registers to the softmax warps, for
+// which a row of S is 128 registers.
 #include "paged_attention.cuh"
 
 namespace yl {
@@ -174,7 +176,7 @@ __global__ void __launch_bounds__(384, 1)
   extern __shared__ uint8_t raw[];
   __shared__ Start start;
   __shared__ uint64_t scratch[16];
-  __shared__ __align__(8) uint64_t full[S::NBUF], empty[S::NBUF], q_full, q_empty, s_full[2], p_full[2], o_full[2], drain;
+  __shared__ __align__(8) uint64_t full[S::NBUF], empty[S::NBUF], q_full, q_empty, s_full[2], p_full[2], o_full[2], turn[2], drain[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -192,12 +194,13 @@ __global__ void __launch_bounds__(384, 1)
   if (threadIdx.x == 0) {
     for (int b = 0; b < S::NBUF; ++b) {
       mbar_init(&full[b], 1);
-      mbar_init(&empty[b], 1);
+      mbar_init(&empty[b], 2);
     }
     mbar_init(&q_full, 1);
-    mbar_init(&q_empty, 1);
-    mbar_init(&drain, 1);
+    mbar_init(&q_empty, 2);
     for (int x = 0; x < 2; ++x) {
+      mbar_init(&drain[x], 1);
+      mbar_init(&turn[x], 1);
       mbar_init(&s_full[x], 1);
       mbar_init(&p_full[x], 4);
       mbar_init(&o_full[x], 1);
@@ -284,21 +287,22 @@ __global__ void __launch_bounds__(384, 1)
       }
       __syncwarp();
     }
-  } else if (!idle && warp == 8) {
-    // ---- MMAs: one lane issues; all wait, and clear what lies behind the last key ----
+  } else if (!idle && warp != 11) {
+    // ---- MMAs of one row tile: an elected lane issues; all wait, and clear what lies behind the last key ----
     Walk<S> w(p, tpt, start);
-    uint32_t n = 0, items = 0, p_phase[2] = {0, 0};
+    const uint32_t x = warp == 8 ? 0 : 1;
+    uint32_t n = 0, items = 0, p_phase = 0, turns = 0;
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       ok = __all_sync(FULL, mbar_wait(bar, parity, nullptr));
       tc_fence_after();
       return ok;
     };
+    auto wait_full = [&](uint32_t i) { return wait(&full[i % S::NBUF], (i / S::NBUF) & 1); };
     // Issued by the lane that elect.sync names (not one picked by its number):
     // only then an MMA's descriptors go to its uniform registers directly, and
     // it costs the 64 cycles that the tensor cores need, not 130.
-    auto qk = [&](auto xc, uint32_t buf) {
-      constexpr uint32_t x = decltype(xc)::value;
+    auto qk = [&](uint32_t buf) {
       if (elect_one()) {
         const uint32_t q = desc_k(q_smem + x * S::TILE), kb = desc_k(ring + buf * S::TILE);
 #pragma unroll
@@ -309,8 +313,7 @@ __global__ void __launch_bounds__(384, 1)
         tc_commit(&s_full[x]);
       }
     };
-    auto pv = [&](auto xc, uint32_t buf, bool first, bool last) {
-      constexpr uint32_t x = decltype(xc)::value;
+    auto pv = [&](uint32_t buf, bool first, bool last) {
       if (elect_one()) {
         const uint32_t vb = desc_n(ring + buf * S::TILE, S::COL);
 #pragma unroll
@@ -320,24 +323,28 @@ __global__ void __launch_bounds__(384, 1)
         if (last) tc_commit(&o_full[x]);
       }
     };
-    constexpr std::integral_constant<uint32_t, 0> first_tile{};
-    constexpr std::integral_constant<uint32_t, 1> second_tile{};
-    auto commit = [&](uint64_t* bar) {
-      if (elect_one()) tc_commit(bar);
+    // a buffer is free when both row tiles' MMAs are through with it; a tile without rows has none
+    auto release = [&](uint64_t* bar, bool mine) {
+      if (elect_one()) {
+        if (mine) tc_commit(bar);
+        else mbar_arrive(bar);
+      }
     };
     do {
-      const uint32_t kend = w.kend(), tiles = w.tokens() > tok_tile ? 2 : 1, nt = w.kt1 - w.kt0;
-      if (!wait(&q_full, items & 1) || !wait(&full[n % S::NBUF], (n / S::NBUF) & 1)) break;
-      qk(first_tile, n % S::NBUF);
-      if (tiles == 2) qk(second_tile, n % S::NBUF);
-      commit(&empty[n % S::NBUF]);
-      if (nt == 1) commit(&q_empty);
-      for (uint32_t i = 0; i < nt && ok; ++i) {
+      const uint32_t kend = w.kend(), nt = w.kt1 - w.kt0;
+      const bool mine = x == 0 || w.tokens() > tok_tile;
+      if (mine && !wait(&q_full, items & 1)) break;
+      if (!wait_full(n)) break;
+      if (mine) qk(n % S::NBUF);
+      release(&empty[n % S::NBUF], mine);
+      if (nt == 1) release(&q_empty, mine);
+      for (uint32_t i = 0; i < nt; ++i) {
         const uint32_t v = n + 1, kn = n + 2, k0 = p.from + (w.kt0 + i) * S::KT;
         const bool more = i + 1 < nt;
-        if (!wait(&full[v % S::NBUF], (v / S::NBUF) & 1)) break;
-        if (k0 + S::KT > kend) {
+        if (!wait_full(v)) break;
+        if (mine && k0 + S::KT > kend) {
           // values behind the last visible key may be anything: their weight is 0, and 0 times NaN is not
+          // (both warps write the same zeros, each before its own products)
           uint8_t* vb = smem + (2 + v % S::NBUF) * S::TILE;
           const uint32_t from = kend > k0 ? kend - k0 : 0;
           for (uint32_t u = lane; u < (S::KT - from) * 8 * S::NH; u += 32) {
@@ -347,32 +354,33 @@ __global__ void __launch_bounds__(384, 1)
           fence_proxy_async();
           __syncwarp();
         }
-        if (!wait(&p_full[0], p_phase[0])) break;
-        p_phase[0] ^= 1;
-        pv(first_tile, v % S::NBUF, i == 0, !more);
-        if (more) {
-          if (!wait(&full[kn % S::NBUF], (kn / S::NBUF) & 1)) break;
-          qk(first_tile, kn % S::NBUF);
+        if (more && !wait_full(kn)) break;
+        if (mine && !wait(&p_full[x], p_phase)) break;
+        // The row tiles' MMAs alternate, each tile's at one go: mixed, both
+        // tiles' S would be there at the same time, both softmaxes would run
+        // together, and the tensor cores would wait for both (565 us, not 5xx).
+        if ((x == 1 || turns > 0) && !wait(&turn[x], (turns - 1 + x) & 1)) break;
+        ++turns;
+        if (mine) {
+          p_phase ^= 1;
+          pv(v % S::NBUF, i == 0, !more);
+          if (more) qk(kn % S::NBUF);
         }
-        if (tiles == 2) {
-          if (!wait(&p_full[1], p_phase[1])) break;
-          p_phase[1] ^= 1;
-          pv(second_tile, v % S::NBUF, i == 0, !more);
-          if (more) qk(second_tile, kn % S::NBUF);
-        }
-        commit(&empty[v % S::NBUF]);
-        if (more) commit(&empty[kn % S::NBUF]);
-        if (i + 2 == nt) commit(&q_empty);
+        if (elect_one()) mbar_arrive(&turn[x ^ 1]);
+        release(&empty[v % S::NBUF], mine);
+        if (more) release(&empty[kn % S::NBUF], mine);
+        if (i + 2 == nt) release(&q_empty, mine);
         n += 2;
       }
+      if (!ok) break;
       ++items;
-    } while (ok && w.next());
+    } while (w.next());
     if (!ok) {
       abort_flag = 1;
       if (lane == 0 && a.seqs.status) *a.seqs.status = STATUS_TIMEOUT;
     }
-    commit(&drain);  // every MMA has completed when this flips
-    mbar_wait(&drain, 0, nullptr);
+    if (elect_one()) tc_commit(&drain[x]);  // every MMA of this warp has completed when this flips
+    mbar_wait(&drain[x], 0, nullptr);
     __syncwarp();
   }
   } else {
