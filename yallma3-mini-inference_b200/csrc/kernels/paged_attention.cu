@@ -379,6 +379,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
         if (busy) {
           if (k0 + S::KT > kend) {
             // values behind the last visible key may be anything: their weight is 0, and 0 times NaN is not
+#pragma unroll 1
             for (uint32_t u = lane; u < (uint32_t)S::WKEYS * S::NH * 8; u += 32) {
               const uint32_t key = wk * S::WKEYS + u / (S::NH * 8), c = u % (S::NH * 8);
               if (k0 + key >= kend)
@@ -438,13 +439,13 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
         l[i] += __shfl_xor_sync(FULL, l[i], 1);
         l[i] += __shfl_xor_sync(FULL, l[i], 2);
       }
-      const uint32_t blocks = w.blocks(), first = w.first_block();
-      const bool whole = blocks == 1;
+      const bool whole = w.whole();
       if (w.kt0 == 0 && warp == 0) {
+        const uint32_t blocks = whole ? 0 : w.blocks();
         if (p.joined)
+#pragma unroll 1
           for (uint32_t t = lane; t < ntok; t += 32)
-            p.desc[(uint64_t)(w.r.row0 + w.t + t) * a.pages.n_kv_heads + w.head] =
-                make_uint2(first, whole ? t : blocks << 16 | t);
+            p.desc[(uint64_t)(w.r.row0 + w.t + t) * a.pages.n_kv_heads + w.head] = make_uint2(blockIdx.x, blocks << 16 | t);
         else if (!whole)
           goes_on = make_uint4(w.r.row0 + w.t, ntok, w.head, blocks);
       }
@@ -468,6 +469,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
           }
         }
         named_bar_sync(1, 32 * S::NW);
+#pragma unroll 1
         for (uint32_t u = threadIdx.x; u < nrow * (HD / 4); u += 32 * S::NW) {
           const uint32_t mr = u / (HD / 4), c = u % (HD / 4), w0 = mr / 16 * WK, rr = mr % 16;
           float top = -INFINITY, sum = 0.0f;

@@ -129,11 +129,13 @@ __device__ __forceinline__ uint64_t units_per_head(const Pass& p, const Rows& r,
   if (p.prefix) return (uint64_t)tiles * (tiles_of<S>(p, r, r.n) + p.item_cost);
   uint64_t n = 0;
   if (tiles <= 4)
+#pragma unroll 1
     for (uint32_t t = 0; t < r.n; t += tpt) n += tiles_of<S>(p, r, t + tpt) + p.item_cost;
   for (uint32_t many = __ballot_sync(FULL, tiles > 4); many; many &= many - 1) {
     const int src = __ffs(many) - 1;
     const Rows w = rows_from_lane(r, src);
     uint64_t part = 0;
+#pragma unroll 1
     for (uint32_t t = lane * tpt; t < w.n; t += 32 * tpt) part += tiles_of<S>(p, w, t + tpt) + p.item_cost;
     part = warp_sum_u64(part);
     if ((int)lane == src) n = part;
@@ -149,11 +151,10 @@ struct Start {
   int masked;                  // prefix pass: some row does not see all of the prefix
 };
 
-__device__ __forceinline__ uint64_t div_up(uint64_t a, uint32_t b) {
-  return a < 0xFFFF0000u ? ((uint32_t)a + b - 1) / b : (a + b - 1) / b;
-}
-__device__ __forceinline__ uint32_t div_small(uint64_t a, uint64_t b) {
-  return (uint32_t)((a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b);
+// a / b; 64-bit division is a long piece of code that hardly ever runs.
+__device__ __noinline__ uint64_t div_long(uint64_t a, uint64_t b) { return a / b; }
+__device__ __forceinline__ uint64_t div(uint64_t a, uint64_t b) {
+  return (a | b) >> 32 ? div_long(a, b) : (uint32_t)a / (uint32_t)b;
 }
 
 // All threads. The sequences' units are summed a block's width at a time; where
@@ -198,7 +199,7 @@ __device__ void find_start(const Pass& p, uint32_t tpt, Start* out, uint64_t* sc
     __syncthreads();
     total += width(c, 0);
   }
-  uint64_t chunk = div_up(total, gridDim.x);
+  uint64_t chunk = div(total + gridDim.x - 1, gridDim.x);
   if (chunk < p.min_chunk) chunk = p.min_chunk;
   const uint64_t begin = chunk * blockIdx.x, end = begin + chunk < total ? begin + chunk : total;
   if (tid == 0) out->chunk = chunk, out->begin = begin, out->end = end;
@@ -215,12 +216,12 @@ __device__ void find_start(const Pass& p, uint32_t tpt, Start* out, uint64_t* sc
         const Rows w = rows_from_lane(r, src);
         const uint64_t each = __shfl_sync(FULL, per_head, src);
         uint64_t g0 = __shfl_sync(FULL, first, src), off = begin - g0;
-        const uint32_t h = div_small(off, each);
+        const uint32_t h = (uint32_t)div(off, each);
         off -= h * each;
         g0 += h * each;
         uint32_t t = 0;
         if (p.prefix) {
-          const uint32_t units = tiles_of<S>(p, w, w.n) + p.item_cost, k = div_small(off, units);
+          const uint32_t units = tiles_of<S>(p, w, w.n) + p.item_cost, k = (uint32_t)div(off, units);
           t = k * tpt;
           g0 += (uint64_t)k * units;
         } else if (w.n > tpt) {
@@ -301,9 +302,12 @@ struct Walk {
   }
   __device__ uint32_t tokens() const { return r.n - t < tpt ? r.n - t : tpt; }
   __device__ uint32_t kend() const { return keys_end(p, r, t + tpt); }
-  // The blocks that the item's key tiles lie in.
-  __device__ uint32_t first_block() const { return div_small(g0 + p.item_cost, chunk); }
-  __device__ uint32_t blocks() const { return div_small(g0 + p.item_cost + nt - 1, chunk) - first_block() + 1; }
+  // All of the item lies in this block; else how many blocks it lies in, this
+  // one, where it begins, the first.
+  __device__ bool whole() const { return kt1 - kt0 == nt; }
+  __device__ uint32_t blocks() const {
+    return kt1 == nt ? 1 : 1 + (uint32_t)div(g0 + p.item_cost + nt - end + chunk - 1, chunk);
+  }
 };
 
 // Sequence of a row by bisection (rows inside the prefix only).

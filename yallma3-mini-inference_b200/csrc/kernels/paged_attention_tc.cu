@@ -347,6 +347,7 @@ __global__ void __launch_bounds__(384, 1)
           // (both warps write the same zeros, each before its own products)
           uint8_t* vb = smem + (2 + v % S::NBUF) * S::TILE;
           const uint32_t from = kend > k0 ? kend - k0 : 0;
+#pragma unroll 1
           for (uint32_t u = lane; u < (S::KT - from) * 8 * S::NH; u += 32) {
             const uint32_t c = u / ((S::KT - from) * 8), o = u % ((S::KT - from) * 8);
             *reinterpret_cast<uint4*>(vb + c * S::COL + from * 128 + o * 16) = make_uint4(0, 0, 0, 0);
@@ -398,12 +399,12 @@ __global__ void __launch_bounds__(384, 1)
       const uint32_t all = w.tokens(), t0 = x * tok_tile, kend = w.kend();
       const uint32_t tok = m / p.group + t0, gh = m % p.group;
       if (warp == 0 && w.kt0 == 0) {
-        const uint32_t first = w.first_block(), blocks = w.blocks();
+        const uint32_t blocks = w.whole() ? 0 : w.blocks();
         if (p.joined)
+#pragma unroll 1
           for (uint32_t t = lane; t < all; t += 32)
-            p.desc[(uint64_t)(w.r.row0 + w.t + t) * a.pages.n_kv_heads + w.head] =
-                make_uint2(first, blocks == 1 ? t : blocks << 16 | t);
-        else if (blocks > 1)
+            p.desc[(uint64_t)(w.r.row0 + w.t + t) * a.pages.n_kv_heads + w.head] = make_uint2(blockIdx.x, blocks << 16 | t);
+        else if (blocks)
           goes_on = make_uint4(w.r.row0 + w.t, all, w.head, blocks);
       }
       if (all <= t0) continue;  // this row tile has no rows (no barrier of it moves)
@@ -524,7 +525,7 @@ __global__ void __launch_bounds__(384, 1)
       o_phase ^= 1;
       tc_fence_after();
       if (busy) {
-        const bool whole = w.blocks() == 1, direct = whole && !p.joined;
+        const bool whole = w.whole(), direct = whole && !p.joined;
         const float inv = mx == -INFINITY && l == l ? 0.0f : 1.0f / l;
         float* part = whole ? p.rowpart + ((uint64_t)row * a.n_heads + head) * PART<HD>
                             : p.slots + ((uint64_t)(2 * blockIdx.x + (w.kt0 == 0 ? 1 : 0)) * TC_TILE + tok * p.group + gh) * PART<HD>;
