@@ -113,7 +113,7 @@ __device__ __forceinline__ uint32_t tiles_of(const Pass& p, const Rows& r, uint3
   return e > p.from + S::KT ? (e - p.from + S::KT - 1) / S::KT : 1;
 }
 __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
-#pragma unroll
+#pragma unroll 1
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
   return v;
 }
@@ -157,103 +157,106 @@ __device__ __forceinline__ uint64_t div(uint64_t a, uint64_t b) {
   return (a | b) >> 32 ? div_long(a, b) : (uint32_t)a / (uint32_t)b;
 }
 
-// All threads. The sequences' units are summed a block's width at a time; where
-// one width holds them all, as it mostly does, they are looked at once.
+// All threads. The sequences' units are summed a block's width at a time, once
+// for the total and once more to find the piece's place, which is found at once
+// where one width holds all sequences, as it mostly does. (Rolled loops: this
+// runs once, and a launch between other kernels waits for every instruction.)
 template <typename S>
 __device__ void find_start(const Pass& p, uint32_t tpt, Start* out, uint64_t* scratch) {
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t n = p.prefix ? 1 : p.a.seqs.n_seqs;
   constexpr uint32_t NWARPS = S::THREADS / 32;
-  Rows r{};
-  uint64_t per_head = 0, mine = 0, first = 0;  // this thread's sequence of the width: units, and where they begin
-  auto width = [&](uint32_t c, uint64_t base) -> uint64_t {
-    const uint32_t i = c + tid;
-    r = i < n ? rows_of(p, i) : Rows{};
-    per_head = units_per_head<S>(p, r, tpt, lane);
-    mine = per_head * p.a.pages.n_kv_heads;
-    uint64_t inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t v = __shfl_up_sync(FULL, inc, o);
-      if ((int)lane >= o) inc += v;
-    }
-    if (lane == 31) scratch[warp] = inc;
-    __syncthreads();
-    uint64_t before = base, sum = 0;
-    for (uint32_t w = 0; w < NWARPS; ++w) {
-      if (w < warp) before += scratch[w];
-      sum += scratch[w];
-    }
-    first = before + inc - mine;
-    return sum;
-  };
   bool masked = false;
   if (p.prefix)  // rows inside the prefix
+#pragma unroll 1
     for (uint32_t i = tid; i < p.a.seqs.n_seqs; i += S::THREADS) {
       const uint32_t rn = row_end(p.a.seqs, i) - row_begin(p.a.seqs, i);
       masked |= rn && (int64_t)p.a.seqs.seq_len[i] - rn + 1 < (int64_t)p.a.seqs.shared_len;
     }
   if (tid == 0) out->seq = 0xFFFFFFFFu;
-  uint64_t total = width(0, 0);
-  for (uint32_t c = S::THREADS; c < n; c += S::THREADS) {
-    __syncthreads();
-    total += width(c, 0);
-  }
-  uint64_t chunk = div(total + gridDim.x - 1, gridDim.x);
-  if (chunk < p.min_chunk) chunk = p.min_chunk;
-  const uint64_t begin = chunk * blockIdx.x, end = begin + chunk < total ? begin + chunk : total;
-  if (tid == 0) out->chunk = chunk, out->begin = begin, out->end = end;
-  if (begin < total) {
+  Rows r{};
+  uint64_t per_head = 0, mine = 0, first = 0;  // this thread's sequence of the width: units, and where they begin
+  uint64_t total = 0, begin = 0, end = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
     uint64_t base = 0;
+#pragma unroll 1
     for (uint32_t c = 0; c < n; c += S::THREADS) {
-      if (n > S::THREADS) {
+      if (pass == 0 || n > S::THREADS) {
+        r = c + tid < n ? rows_of(p, c + tid) : Rows{};
+        per_head = units_per_head<S>(p, r, tpt, lane);
+        mine = per_head * p.a.pages.n_kv_heads;
+        uint64_t inc = mine;
+#pragma unroll 1
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint64_t v = __shfl_up_sync(FULL, inc, o);
+          if ((int)lane >= o) inc += v;
+        }
         __syncthreads();
-        base += width(c, base);
+        if (lane == 31) scratch[warp] = inc;
+        __syncthreads();
+        first = base + inc - mine;
+#pragma unroll 1
+        for (uint32_t w = 0; w < NWARPS; ++w) {
+          if (w < warp) first += scratch[w];
+          base += scratch[w];
+        }
       }
+      if (pass == 0) continue;
       const uint32_t here = __ballot_sync(FULL, begin >= first && begin < first + mine);
-      if (here) {  // in one of this warp's sequences: all lanes look for the row tile
-        const int src = __ffs(here) - 1;
-        const Rows w = rows_from_lane(r, src);
-        const uint64_t each = __shfl_sync(FULL, per_head, src);
-        uint64_t g0 = __shfl_sync(FULL, first, src), off = begin - g0;
-        const uint32_t h = (uint32_t)div(off, each);
-        off -= h * each;
-        g0 += h * each;
-        uint32_t t = 0;
-        if (p.prefix) {
-          const uint32_t units = tiles_of<S>(p, w, w.n) + p.item_cost, k = (uint32_t)div(off, units);
-          t = k * tpt;
-          g0 += (uint64_t)k * units;
-        } else if (w.n > tpt) {
-          while (t < w.n) {  // 32 row tiles at a time
-            const uint32_t mt = t + lane * tpt;
-            const uint32_t units = mt < w.n ? tiles_of<S>(p, w, mt + tpt) + p.item_cost : 0;
-            uint64_t upto = units;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const uint64_t v = __shfl_up_sync(FULL, upto, o);
-              if ((int)lane >= o) upto += v;
-            }
-            const uint32_t in = __ballot_sync(FULL, upto > off);
-            if (in) {
-              const int k = __ffs(in) - 1;
-              t += k * tpt;
-              g0 += __shfl_sync(FULL, upto - units, k);
-              break;
-            }
-            const uint64_t all = __shfl_sync(FULL, upto, 31);
-            off -= all;
-            g0 += all;
-            t += 32 * tpt;
+      if (!here) continue;
+      // in one of this warp's sequences: all lanes look for the row tile
+      const int src = __ffs(here) - 1;
+      const Rows w = rows_from_lane(r, src);
+      const uint64_t each = __shfl_sync(FULL, per_head, src);
+      uint64_t g0 = __shfl_sync(FULL, first, src), off = begin - g0;
+      const uint32_t h = (uint32_t)div(off, each);
+      off -= h * each;
+      g0 += h * each;
+      uint32_t t = 0;
+      if (p.prefix) {
+        const uint32_t units = tiles_of<S>(p, w, w.n) + p.item_cost, k = (uint32_t)div(off, units);
+        t = k * tpt;
+        g0 += (uint64_t)k * units;
+      } else if (w.n > tpt) {
+#pragma unroll 1
+        while (t < w.n) {  // 32 row tiles at a time
+          const uint32_t mt = t + lane * tpt;
+          const uint32_t units = mt < w.n ? tiles_of<S>(p, w, mt + tpt) + p.item_cost : 0;
+          uint64_t upto = units;
+#pragma unroll 1
+          for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t v = __shfl_up_sync(FULL, upto, o);
+            if ((int)lane >= o) upto += v;
           }
-        }
-        if (lane == 0) {
-          if (end > g0 + p.item_cost) out->seq = c + warp * 32 + src;  // else the piece ends before the item's first tile
-          out->head = h;
-          out->t = t;
-          out->g0 = g0;
+          const uint32_t in = __ballot_sync(FULL, upto > off);
+          if (in) {
+            const int k = __ffs(in) - 1;
+            t += k * tpt;
+            g0 += __shfl_sync(FULL, upto - units, k);
+            break;
+          }
+          const uint64_t all = __shfl_sync(FULL, upto, 31);
+          off -= all;
+          g0 += all;
+          t += 32 * tpt;
         }
       }
+      if (lane == 0) {
+        if (end > g0 + p.item_cost) out->seq = c + warp * 32 + src;  // else the piece ends before the item's first tile
+        out->head = h;
+        out->t = t;
+        out->g0 = g0;
+      }
+    }
+    if (pass == 0) {
+      total = base;
+      uint64_t chunk = div(total + gridDim.x - 1, gridDim.x);
+      if (chunk < p.min_chunk) chunk = p.min_chunk;
+      begin = chunk * blockIdx.x;
+      end = begin + chunk < total ? begin + chunk : total;
+      if (tid == 0) out->chunk = chunk, out->begin = begin, out->end = end;
+      if (begin >= total) break;  // nothing for this block
     }
   }
   // (also the barrier that makes *out visible)
