@@ -544,8 +544,9 @@ typedef struct yl_seq_batch {
  * rope_mode says (yl_rope_mode); NULL: no rotation. q_out: rotated queries in
  * the cache's type, rows q_stride elements apart; NULL: keys and values only
  * (a row then still holds n_heads query heads, which are skipped). Products
- * and sums in f32, one rounding to the cache's type. Two rows of one call
- * must not have the same slot. */
+ * and sums in f32, one rounding to the cache's type; an f32 cache gets the
+ * bits of a session's own cache. Two rows of one call must not have the same
+ * slot, and no other call may write a slot at the same time. */
 int yl_paged_append(void* q_out, uint64_t q_stride, const float* qkv, uint64_t qkv_stride, const yl_kv_pages* pages,
                     const yl_seq_batch* batch, uint32_t n_heads, const float* rope_cs, uint32_t rope_len,
                     int rope_mode, void* stream);
@@ -560,8 +561,11 @@ int yl_paged_append(void* q_out, uint64_t q_stride, const float* qkv, uint64_t q
  * in f32; products of an f32 cache as three tf32 products (about 2^-21
  * relative); for a 16-bit cache the softmax weights are rounded to its type.
  * Contents of the cache behind a sequence's last position do not matter,
- * infinities and NaN included. The summation order depends on the batch's
- * geometry alone: the same call gives the same bits.
+ * infinities and NaN included. A value that is not finite reaches all rows
+ * that see it, and may reach rows of the same chunk before it (their weight
+ * for it is 0, and 0 times infinity is NaN); in an f32 cache an infinite key
+ * or value gives NaN. The summation order depends on the batch's geometry
+ * alone: the same call gives the same bits.
  * workspace: device memory of at least the bytes yl_paged_attention_workspace
  * gives for a batch of these counts (n_seqs, n_rows, shared_len) and heads,
  * 256-byte aligned, with any contents; not to be shared by calls that may

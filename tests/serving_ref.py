@@ -57,11 +57,11 @@ class Geometry:
         return torch.where(torch.from_numpy(good)[:, None, None], rows, 0.0)
 
 
-def attention(g: Geometry, q, k, v, scale, limit=1 << 31):
+def attention(g: Geometry, q, k, v, scale, limit=1 << 31, only=None):
     """(out, lse, out_bound, lse_bound) in 64 bits. The bounds count, for scores of |terms| sum A: products and sums of
     hd terms, each off by at most two half steps of f32 (a tensor core may truncate) in chains of hd/4 + 16; for the
     softmax: exp of an f32 argument (its rounding: |s| * 2 U32; exp itself: 4 U32) and sums in chains of n/4 + 64; for a
-    16-bit type one half step on every weight. Output rounding is added by the caller."""
+    16-bit type one half step on every weight. Output rounding is added by the caller. only: the rows to compute."""
     n, group = g.n_rows, g.heads // g.kv
     out = torch.zeros(n, g.heads, g.hd, dtype=torch.float64)
     lse = torch.full((n, g.heads), -torch.inf, dtype=torch.float64)
@@ -75,6 +75,8 @@ def attention(g: Geometry, q, k, v, scale, limit=1 << 31):
             if pos < 0:
                 continue
             r, m = int(g.row_start[i]) + t, min(int(pos) + 1, limit)
+            if only is not None and r not in only:
+                continue
             for h in range(g.heads):
                 qq, kk, vv = q[r, h].double(), ks[:m, h // group], vs[:m, h // group]
                 s = kk @ qq * scale

@@ -317,6 +317,288 @@ def test_same_bits_again_and_on_another_stream(yl, torch_cuda):
     torch.cuda.current_stream().wait_stream(side)
 
 
+def check_some_rows(yl, g, dtype, rows, shared=None):
+    q, (k, v), scale = queries(g, dtype), g.pool(dtype), g.hd**-0.5
+    out, lse = attend(yl, g, q.cuda(), k.cuda(), v.cuda(), scale, shared=shared)
+    only = set(int(r) for r in rows)
+    want, wlse, ob, lb = ref.attention(g, q, k, v, scale, only=only)
+    at = sorted(only)
+    within(out[at], want[at], (ob + (want.abs() + ob) * ref.half_step(dtype) + 2.0**-25 * (dtype == torch.float16))[at], "out")
+    within(lse[at], wlse[at], lb[at], "lse")
+    assert out.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_one_long_prompt(yl, torch_cuda, dtype):
+    """More row tiles than a warp counts at a time, key tiles cut among all blocks; rows next to tile borders."""
+    n = 5003
+    g = ref.Geometry(30, 2, 1, 64, page=32, lens=[n], rows=[n])
+    rows = [0, 1, 31, 32, 63, 64, 127, 128, 129, 255, 256, n - 130, n - 129, n - 2, n - 1] + list(
+        np.random.default_rng(0).integers(0, n, 40))
+    check_some_rows(yl, g, DTYPES[dtype], rows)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_many_sequences(yl, torch_cuda, dtype):
+    """More sequences than a block has threads, idle slots among them."""
+    rng = np.random.default_rng(31)
+    lens = rng.integers(1, 90, 700)
+    rows = (rng.random(700) < 0.8).astype(int)
+    g = ref.Geometry(31, 2, 1, 64, page=16, lens=lens, rows=rows, pad_rows=9)
+    check_some_rows(yl, g, DTYPES[dtype], rng.integers(0, int(g.row_start[-1]), 120))
+    lens, rows = lens + 64, rng.integers(0, 4, 700)
+    g = ref.Geometry(32, 4, 2, 64, page=16, lens=lens, rows=rows, shared=64)
+    check_some_rows(yl, g, DTYPES[dtype], rng.integers(0, int(g.row_start[-1]), 120))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_mixed_prompts_and_tokens(yl, torch_cuda, dtype):
+    """One prompt chunk next to single tokens, with and without a shared prefix."""
+    for shared in (0, 128):
+        g = ref.Geometry(33, 6, 2, 128, page=64, lens=[shared + n for n in (400, 1, 17, 90, 300)], rows=[300, 1, 1, 1, 2],
+                         shared=shared)
+        check_some_rows(yl, g, DTYPES[dtype], np.random.default_rng(1).integers(0, 305, 60))
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_geometries(yl, torch_cuda, seed):
+    rng = np.random.default_rng(1000 + seed)
+    pick = lambda *a: a[rng.integers(len(a))]  # noqa: E731
+    kv, group, hd = pick(1, 2, 3), pick(1, 2, 3, 4, 5, 7, 8, 12, 16), pick(64, 128)
+    page, n = pick(8, 16, 32, 64, 128, 256), int(rng.integers(1, 9))
+    shared = pick(0, 0, 1, 2, 5) * page
+    lens = shared + np.array([pick(0, 1, 7, 64, 65, int(rng.integers(1, 400))) for _ in range(n)])
+    rows = [min(int(x) + 2, pick(0, 1, 1, 3, 17, int(rng.integers(1, 100)))) for x in lens]
+    g = ref.Geometry(seed, kv * group, kv, hd, page=page, lens=lens, rows=rows, shared=shared, pad_rows=pick(0, 3))
+    if not g.n_rows:
+        return
+    check_attention(yl, g, pick(*DTYPES.values()), shared=pick(0, shared))
+
+
+def test_row_starts_behind_zero_and_out_of_order(yl, torch_cuda):
+    """Rows before row_start[0] belong to nobody. Starts beyond n_rows or that run backwards stay within the rows."""
+    g = ref.Geometry(34, 4, 2, 64, page=16, lens=[30, 60, 40], rows=[2, 1, 3])
+    for t in DTYPES.values():
+        (k, v) = (x.cuda() for x in g.pool(t))
+        q = queries(g, t)
+        want, _ = attend(yl, g, q.cuda(), k, v, 0.125)
+        shifted = ref.Geometry(34, 4, 2, 64, page=16, lens=[30, 60, 40], rows=[2, 1, 3], pad_rows=4)
+        shifted.table, shifted.row_start = g.table, g.row_start + 4
+        qs = torch.cat([torch.zeros(4, 4, 64, dtype=t), q])
+        got, lse = attend(yl, shifted, qs.cuda(), k, v, 0.125)
+        assert torch.equal(got[4:], want) and (got[:4] == 7.0).all() and (lse[:4] == 7.0).all()
+        for starts in ([0, 5, 2, 6], [9, 9, 9, 9], [0, 2, 100, 0xFFFFFFF0], [6, 4, 2, 0]):
+            shifted.row_start = np.array(starts, np.uint32)
+            attend(yl, shifted, qs.cuda(), k, v, 0.125)
+            yl.paged_append(torch.zeros(10, 8 * 64, device="cuda"), yl.KvPages.of(k.clone(), v.clone()), shifted.device(yl), 4)
+    torch.cuda.synchronize()
+
+
+def test_captured_step_follows_its_arrays(yl, torch_cuda):
+    """Append, attention and log probabilities captured once and replayed while the sequences grow: the arrays' new
+    contents count, and each replay equals the eager calls."""
+    t, hd, heads, kv, vocab = torch.bfloat16, 64, 8, 2, 5000
+    n, page, slots, shared = 5, 16, 12, 32
+    rng = np.random.default_rng(5)
+    table = np.concatenate([np.tile([0, 1], (n, 1)), 2 + rng.permutation(n * (slots - 2)).reshape(n, -1)], 1)
+    arrays = [torch.from_numpy(a.astype(np.int32)).cuda() for a in (np.arange(n + 1), np.full(n, 40), table)]
+    pools = [torch.randn(2 + n * (slots - 2), page, kv, hd, device="cuda").to(t) for _ in range(2)]
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    batch = yl.SeqBatch(*arrays, n, shared_len=shared, status=status)
+    cs = ref.rope_cs(slots * page, hd).cuda()
+    qkv, logits = torch.empty(n, (heads + 2 * kv) * hd, device="cuda"), torch.empty(n, vocab, device="cuda")
+    tokens = torch.zeros(n, dtype=torch.int32, device="cuda")
+
+    def buffers():
+        return dict(q=torch.empty(n, heads, hd, dtype=t, device="cuda"), out=torch.empty(n, heads, hd, dtype=t, device="cuda"),
+                    lse=torch.empty(n, heads, device="cuda"), lp=torch.empty(n, device="cuda"),
+                    ids=torch.empty(n, 4, dtype=torch.int32, device="cuda"), top=torch.empty(n, 4, device="cuda"))
+
+    def step(pages, b, ws):
+        yl.paged_append(qkv, pages, batch, heads, rope_cs=cs, q_out=b["q"])
+        yl.paged_attention(b["out"], b["q"], pages, batch, heads, 0.125, ws, lse=b["lse"])
+        yl.token_logprobs(logits, tokens, b["lp"], top_ids=b["ids"], top_logprobs=b["top"])
+
+    pages = yl.KvPages.of(*pools)
+    size = yl.paged_attention_workspace(pages, batch, heads)
+    ws, ws2 = (torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(2))
+    a, b = buffers(), buffers()
+    qkv.normal_(), logits.normal_()
+    step(pages, a, ws)  # (loads the kernels)
+    twin_pages = yl.KvPages.of(*[x.clone() for x in pools])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(pages, a, ws)
+    for i in range(6):
+        arrays[1].copy_(torch.tensor([33 + i, 40 + 20 * i, 60 + i, 33, 160 + i], dtype=torch.int32))
+        qkv.normal_(), logits.normal_()
+        graph.replay()
+        step(twin_pages, b, ws2)
+        for name in a:
+            assert torch.equal(a[name], b[name]), (i, name)
+    assert status.item() == 0
+    arrays[1][4] = 1000  # beyond the table
+    graph.replay()
+    assert status.item() == -6
+
+
+def test_two_calls_at_once(yl, torch_cuda):
+    """Two streams, a workspace each."""
+    g = ref.Geometry(35, 8, 2, 128, page=16, lens=[900, 3000, 50, 2000], rows=[1, 1, 1, 1])
+    h = ref.Geometry(36, 8, 2, 128, page=16, lens=[900, 700], rows=[300, 500])
+    ops = []
+    for x in (g, h):
+        q, (k, v) = queries(x, torch.float16).cuda(), (y.cuda() for y in x.pool(torch.float16))
+        ops.append((x, q, k, v, attend(yl, x, q, k, v, 0.1)[0]))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ops]
+    got = [[], []]
+    for _ in range(10):
+        for i, (s, (x, q, k, v, _)) in enumerate(zip(streams, ops)):
+            with torch.cuda.stream(s):
+                got[i].append(attend(yl, x, q, k, v, 0.1)[0])
+    torch.cuda.synchronize()
+    for i, (_, _, _, _, want) in enumerate(ops):
+        assert all(torch.equal(o, want) for o in got[i])
+
+
+def test_python_refusals(yl, torch_cuda):
+    g = ref.Geometry(37, 4, 2, 64, page=16, lens=[30], rows=[2])
+    k, v = (x.cuda() for x in g.pool(torch.float16))
+    pages, batch = yl.KvPages.of(k, v), g.device(yl)
+    q, out = (torch.zeros(2, 4, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+    ws = torch.empty(yl.paged_attention_workspace(pages, batch, 4), dtype=torch.uint8, device="cuda")
+    qkv = torch.zeros(2, 8 * 64, device="cuda")
+    lp = torch.zeros(2, device="cuda")
+    attend_ = lambda **kw: yl.paged_attention(**{**dict(output=out, q=q, pages=pages, batch=batch, n_heads=4,  # noqa: E731
+                                                       attn_scale=0.1, workspace=ws), **kw})
+    append_ = lambda **kw: yl.paged_append(**{**dict(qkv=qkv, pages=pages, batch=batch, n_heads=4), **kw})  # noqa: E731
+    for kind, call in (
+            (TypeError, lambda: attend_(q=q.float())), (TypeError, lambda: attend_(output=out.double())),
+            (yl.YlError, lambda: attend_(output=out.bfloat16())), (ValueError, lambda: attend_(q=q[:1])),
+            (ValueError, lambda: attend_(q=q.cpu())), (ValueError, lambda: attend_(q=q.transpose(1, 2))),
+            (yl.YlError, lambda: attend_(workspace=ws[: ws.numel() // 2])), (TypeError, lambda: attend_(workspace=ws.float())),
+            (ValueError, lambda: attend_(lse=lp)), (ValueError, lambda: attend_(n_heads=8)),
+            (TypeError, lambda: append_(qkv=qkv.half())), (ValueError, lambda: append_(qkv=qkv[:, 1:])),
+            (TypeError, lambda: append_(q_out=q.float())), (ValueError, lambda: append_(rope_cs=lp)),
+            (ValueError, lambda: yl.KvPages.of(k, v[:, :8])), (ValueError, lambda: yl.KvPages.of(k.cpu(), v.cpu())),
+            (ValueError, lambda: yl.SeqBatch(batch._keep[0], batch._keep[1], batch._keep[2][0], 2)),
+            (TypeError, lambda: yl.SeqBatch(batch._keep[0].long(), batch._keep[1], batch._keep[2], 2)),
+            (TypeError, lambda: yl.token_logprobs(qkv.double(), entropy=lp)),
+            (TypeError, lambda: yl.token_logprobs(qkv, lp, lp)), (ValueError, lambda: yl.token_logprobs(qkv.t(), entropy=lp)),
+            (yl.YlError, lambda: yl.token_logprobs(qkv, logprobs=lp))):
+        with pytest.raises(kind):
+            call()
+    attend_(), append_()
+
+
+def test_pages_from_the_library(yl, torch_cuda):
+    """A cache that the library allocates: append, then attend, as with torch's."""
+    g = ref.Geometry(38, 4, 2, 64, page=16, lens=[5], rows=[5])
+    qkv = torch.from_numpy(g.rng.standard_normal((5, 8 * 64))).float().cuda()
+    k, v = torch.zeros(g.n_pages, 16, 2, 64, device="cuda"), torch.zeros(g.n_pages, 16, 2, 64, device="cuda")
+    mine = yl.KvPages.alloc(yl.DType.F32, g.n_pages, 16, 2, 64)
+    batch, outs = g.device(yl), []
+    for pages in (yl.KvPages.of(k, v), mine):
+        q, out = torch.empty(5, 4, 64, device="cuda"), torch.empty(5, 4, 64, device="cuda")
+        yl.paged_append(qkv, pages, batch, 4, q_out=q)
+        ws = torch.empty(yl.paged_attention_workspace(pages, batch, 4), dtype=torch.uint8, device="cuda")
+        yl.paged_attention(out, q, pages, batch, 4, 0.125, ws)
+        outs.append(out)
+    assert torch.equal(*outs)
+    torch.cuda.synchronize()
+    mine.free()
+
+
+@pytest.mark.parametrize("preset,over", [("tiny", {}), ("tiny", {"llama3_scaling": True}), ("tiny128", {})])
+def test_a_model_layer_served_from_pages(yl, torch_cuda, model_factory, preset, over):
+    """The step of a server, next to the library's own: the projections of a model's first layer on the rows of three
+    sequences that share a prefix, the rows appended with the model's rotation table, attention over the pages. Keys and
+    values in an f32 cache have the bits of the decode kernel's cache, the outputs agree within the f32 bound, and a
+    bf16 cache within its own."""
+    m = yl.load_transformer(model_factory(preset, **over), max_ctx_len=256)
+    sh = m.shape()
+    heads, kv, hd, dim = sh.n_heads, sh.n_kv_heads, sh.head_size, sh.dim
+    cs, cs_len = m.rope_table()
+    mode = yl.ROPE_LLAMA3 if sh.rope_mode else yl.ROPE_GGUF
+    scale = 1.0 / math.sqrt(hd)
+    lens, shared, page = [70, 41, 33], 32, 16
+
+    def project(x):
+        act = yl.new_workspace_buffer(yl.WeightFormat.Q8_0, x.numel(), 32)
+        yl.quantize(yl.WeightFormat.Q8_0, act, x, x.numel(), 32)
+        parts = []
+        for which, rows in ((0, heads * hd), (1, kv * hd), (2, kv * hd)):
+            out = torch.zeros(x.shape[0], rows, device="cuda")
+            yl.matmul(out, act, m.weight(0, which), dim, rows, 32, accumulate=False)
+            parts.append(out)
+        return torch.cat(parts, 1)
+
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    prefix = torch.randn(shared, dim, generator=gen, device="cuda") * 4
+    own = [torch.randn(n - shared, dim, generator=gen, device="cuda") * 4 for n in lens]
+    qkv_prefix, qkv_own = project(prefix), [project(x) for x in own]
+    for dtype in (torch.float32, torch.bfloat16):
+        g = ref.Geometry(39, heads, kv, hd, page=page, lens=lens, rows=[1, 1, 1], shared=shared)
+        k, v = (torch.zeros(g.n_pages, page, kv, hd, dtype=dtype, device="cuda") for _ in range(2))
+        pages = yl.KvPages.of(k, v)
+
+        def append(rows, counts, upto, q_out=None):
+            part = ref.Geometry(39, heads, kv, hd, page=page, lens=upto, rows=counts, shared=shared)
+            part.table = g.table[: len(upto)]
+            yl.paged_append(rows, pages, part.device(yl), heads, rope_cs=cs, rope_len=cs_len, rope_mode=mode, q_out=q_out)
+
+        append(qkv_prefix, [shared], [shared])  # the prefix once, through the first sequence's table
+        append(torch.cat([x[:-1] for x in qkv_own]), [n - shared - 1 for n in lens], [n - 1 for n in lens])
+        last = torch.cat([x[-1:] for x in qkv_own])
+        q, out = (torch.empty(3, heads, hd, dtype=dtype, device="cuda") for _ in range(2))
+        append(last, [1, 1, 1], lens, q)
+        batch = g.device(yl)
+        ws = torch.empty(yl.paged_attention_workspace(pages, batch, heads), dtype=torch.uint8, device="cuda")
+        yl.paged_attention(out, q, pages, batch, heads, scale, ws)
+        want, _, ob, _ = ref.attention(g, q.cpu(), k.cpu(), v.cpu(), scale)
+        within(out, want, ob + (want.abs() + ob) * ref.half_step(dtype), "out")
+        if dtype != torch.float32:
+            continue
+        for i, n in enumerate(lens):  # the decode kernel on a cache of its own
+            kc, vc, o = (torch.zeros(n, kv * hd, device="cuda") for _ in range(3))
+            o = torch.zeros(heads * hd, device="cuda")
+            for pos, row in enumerate(torch.cat([qkv_prefix, qkv_own[i]])):
+                m.attention_decode(row.contiguous(), kc, vc, pos, out=o)
+            assert torch.equal(g.gather(i, k.cpu()), kc.cpu().double().view(n, kv, hd))
+            assert torch.equal(g.gather(i, v.cpu()), vc.cpu().double().view(n, kv, hd))
+            bound = 2 * ob[i].flatten() + 2 * want[i].abs().flatten() * ref.U32
+            within(out[i].flatten(), o.double().cpu(), bound, "decode kernel")
+    m.close()
+
+
+def test_logprobs_of_sessions_and_batches(yl, torch_cuda, model_factory):
+    """Log probabilities straight from the device logits of a session and of a batch, against the host's logits."""
+    m = yl.load_transformer(model_factory("tiny"), max_ctx_len=64)
+    vocab = m.vocab_size()
+    sessions = [m.create_session() for _ in range(3)]
+    for i, s in enumerate(sessions):
+        logits, best = m.forward_x_full([1 + i, 7, 9], 0, s)
+        lp, ids, top = torch.empty(1, device="cuda"), torch.empty(1, 3, dtype=torch.int32, device="cuda"), torch.empty(1, 3, device="cuda")
+        yl.token_logprobs(yl.session_logits(s), torch.tensor([best], dtype=torch.int32, device="cuda"), lp, top_ids=ids,
+                          top_logprobs=top, shape=(1, vocab))
+        want = ref.logprobs(torch.from_numpy(logits)[None], torch.tensor([best]), 3)
+        within(lp, want[0], want[4], "lp")
+        assert ids.tolist() == want[2].tolist() and ids[0, 0].item() == best
+    b = m.create_batch(3)
+    _, logits = b.forward(sessions, [5, 6, 7], [3, 3, 3], want_logits=True)
+    tokens = torch.tensor([1, 2, 3], dtype=torch.int32)
+    lp, en = torch.empty(3, device="cuda"), torch.empty(3, device="cuda")
+    yl.token_logprobs(b.logits(), tokens.cuda(), lp, entropy=en, shape=(3, vocab))
+    want = ref.logprobs(torch.from_numpy(logits), tokens, 0)
+    within(lp, want[0], want[4], "lp")
+    within(en, want[1], want[5], "entropy")
+    b.close()
+    for s in sessions:
+        s.close()
+    m.close()
+
+
 # -------------------------------------------------------------- logprobs ---
 
 def run_logprobs(yl, x, tokens, k):

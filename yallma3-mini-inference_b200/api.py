@@ -529,16 +529,23 @@ def paged_attention(output, q, pages: KvPages, batch: SeqBatch, n_heads: int, at
 
 
 def token_logprobs(logits, tokens=None, logprobs=None, entropy=None, top_ids=None, top_logprobs=None,
-                   stream=None) -> None:
+                   shape=None, stream=None) -> None:
     """Log probabilities of the given tokens, entropies and most likely tokens of rows of logits [rows, vocab]
     (yl_token_logprobs). Device tensors: tokens int32 [rows], logprobs and entropy f32 [rows], top_ids int32 and
-    top_logprobs f32 [rows, k]; each of the three groups may be left out."""
+    top_logprobs f32 [rows, k]; each of the three groups may be left out. logits may be an address of f32 rows
+    (session_logits, SessionBatch.logits) with their shape (rows, vocab)."""
     if _torch is None:
         _load_torch()
-    n, vocab = logits.shape
-    k, dev = 0 if top_ids is None else top_ids.shape[-1], _device()
+    dev = _device()
+    if isinstance(logits, int):
+        (n, vocab), ptr, dtype = shape, logits, 0
+        stride = vocab
+    else:
+        n, vocab = logits.shape
+        ptr, dtype, stride = logits.data_ptr(), _dtype(logits, "logits"), _row_stride(logits, "logits", vocab, n, dev)
+    k = 0 if top_ids is None else top_ids.shape[-1]
     rc = _lib.yl_token_logprobs(
-        logits.data_ptr(), _dtype(logits, "logits"), _row_stride(logits, "logits", vocab, n, dev), n, vocab,
+        ptr, dtype, stride, n, vocab,
         _flat(tokens, "tokens", _i32, n, dev), _flat(logprobs, "logprobs", _f32, n, dev),
         _flat(entropy, "entropy", _f32, n, dev), k, _flat(top_ids, "top_ids", _i32, n * k, dev),
         _flat(top_logprobs, "top_logprobs", _f32, n * k, dev), _raw_stream(stream, dev))

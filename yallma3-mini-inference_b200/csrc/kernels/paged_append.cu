@@ -6,7 +6,9 @@
 // cache's type; a thread moves 16 elements of a head (64 bytes in), which are
 // eight whole pairs in either pairing, so no value is exchanged between
 // threads. One block per row: the row's sequence, position and page are looked
-// up once per warp, after the row's loads are in flight.
+// up once per warp, after the row's loads are in flight. Measured on one B200:
+// 7000 rows of 32+2x8 heads of 128 into f16 48.7 us (271 MB, 85 % of a copy's
+// rate); 64 rows 3.2 us, one row 2.2 us (launch and three dependent lookups).
 #include "serve.cuh"
 
 namespace yl {
@@ -14,6 +16,14 @@ namespace k {
 using namespace yl::dev;
 
 namespace {
+
+// Every product and sum rounded by itself, as in the other kernels: an f32 cache
+// gets the bits that a session's own cache has.
+__device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
+  const float a0 = a;
+  a = __fsub_rn(__fmul_rn(a0, c), __fmul_rn(b, s));
+  b = __fadd_rn(__fmul_rn(a0, s), __fmul_rn(b, c));
+}
 
 template <typename T>
 __device__ __forceinline__ void store8(T* dst, const float (&v)[8]) {
@@ -71,14 +81,12 @@ __global__ void append_kernel(AppendArgs a) {
       for (int i = 0; i < 4; ++i) {
         const float4 t = cs[i];  // two (cos, sin)
         if (HALF) {
-          const float p0 = x[2 * i], q0 = y[2 * i], p1 = x[2 * i + 1], q1 = y[2 * i + 1];
-          x[2 * i] = p0 * t.x - q0 * t.y, y[2 * i] = p0 * t.y + q0 * t.x;
-          x[2 * i + 1] = p1 * t.z - q1 * t.w, y[2 * i + 1] = p1 * t.w + q1 * t.z;
+          rotate(x[2 * i], y[2 * i], t.x, t.y);
+          rotate(x[2 * i + 1], y[2 * i + 1], t.z, t.w);
         } else {
           float* v = i < 2 ? x + 4 * i : y + 4 * (i - 2);
-          const float p0 = v[0], q0 = v[1], p1 = v[2], q1 = v[3];
-          v[0] = p0 * t.x - q0 * t.y, v[1] = p0 * t.y + q0 * t.x;
-          v[2] = p1 * t.z - q1 * t.w, v[3] = p1 * t.w + q1 * t.z;
+          rotate(v[0], v[1], t.x, t.y);
+          rotate(v[2], v[3], t.z, t.w);
         }
       }
     }
