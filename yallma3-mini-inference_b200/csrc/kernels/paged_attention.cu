@@ -66,19 +66,19 @@ template <typename T>
 __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>
 __device__ __forceinline__ void mma16<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 template <>
 __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -278,44 +278,52 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
 #pragma unroll
           for (int j = 0; j < NB; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
           if constexpr (S::F32) {
-// The tensor cores drop what falls below an accumulator's last bit, so
+            // The tensor cores drop what falls below an accumulator's last bit, so
             // long chains lose digits: two accumulators for the large products
-            // and one for the small ones, added at the end.
-            float s1[NB][4], sl[NB][4];
+            // and one for the small ones, added at the end; 32 keys at a time,
+            // for the registers.
+            constexpr int JG = NB < 4 ? NB : 4;
 #pragma unroll
-            for (int j = 0; j < NB; ++j)
+            for (int j0 = 0; j0 < NB; j0 += JG) {
+              float s1[JG][4], sl[JG][4];
 #pragma unroll
-              for (int c = 0; c < 4; ++c) s1[j][c] = sl[j][c] = 0.0f;
+              for (int j = 0; j < JG; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s1[j][c] = sl[j][c] = 0.0f;
 #pragma unroll 2
-            for (int ks = 0; ks < HD / 16; ++ks) {  // 16 elements: two k-steps of 8
-              uint32_t ah[2][4], al[2][4];
-              const float* q0 = qs + (wm * 16 + g) * S::QP + 16 * ks + t4;
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                split(q0[8 * h], ah[h][0], al[h][0]);
-                split(q0[8 * h + 8 * S::QP], ah[h][1], al[h][1]);
-                split(q0[8 * h + 4], ah[h][2], al[h][2]);
-                split(q0[8 * h + 4 + 8 * S::QP], ah[h][3], al[h][3]);
-              }
-#pragma unroll
-              for (int j = 0; j < NB; ++j) {
-                uint32_t r[4];
-                ldsm4(r, base + at<S>(wk * S::WKEYS + 8 * j + (lane & 7), 4 * ks + (lane >> 3)));
+              for (int ks = 0; ks < HD / 16; ++ks) {  // 16 elements: two k-steps of 8
+                uint32_t ah[2][4], al[2][4];
+                const float* q0 = qs + (wm * 16 + g) * S::QP + 16 * ks + t4;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                  uint32_t bh[2], bl[2];
-                  split(__uint_as_float(r[2 * h]), bh[0], bl[0]);
-                  split(__uint_as_float(r[2 * h + 1]), bh[1], bl[1]);
-                  mma_tf32(sl[j], al[h], bh[0], bh[1]);
-                  mma_tf32(sl[j], ah[h], bl[0], bl[1]);
-                  mma_tf32(h ? s1[j] : s[j], ah[h], bh[0], bh[1]);
+                  split(q0[8 * h], ah[h][0], al[h][0]);
+                  split(q0[8 * h + 8 * S::QP], ah[h][1], al[h][1]);
+                  split(q0[8 * h + 4], ah[h][2], al[h][2]);
+                  split(q0[8 * h + 4 + 8 * S::QP], ah[h][3], al[h][3]);
+                }
+#pragma unroll
+                for (int j = 0; j < JG; ++j) {
+                  uint32_t r[4];
+                  ldsm4(r, base + at<S>(wk * S::WKEYS + 8 * (j0 + j) + (lane & 7), 4 * ks + (lane >> 3)));
+                  uint32_t bh[2][2], bl[2][2];
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    split(__uint_as_float(r[2 * h]), bh[h][0], bl[h][0]);
+                    split(__uint_as_float(r[2 * h + 1]), bh[h][1], bl[h][1]);
+                  }
+                  mma_tf32(s[j0 + j], ah[0], bh[0][0], bh[0][1]);
+                  mma_tf32(sl[j], al[0], bh[0][0], bh[0][1]);
+                  mma_tf32(s1[j], ah[1], bh[1][0], bh[1][1]);
+                  mma_tf32(sl[j], ah[0], bl[0][0], bl[0][1]);
+                  mma_tf32(sl[j], al[1], bh[1][0], bh[1][1]);
+                  mma_tf32(sl[j], ah[1], bl[1][0], bl[1][1]);
                 }
               }
+#pragma unroll
+              for (int j = 0; j < JG; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s[j0 + j][c] = (s[j0 + j][c] + s1[j][c]) + sl[j][c];
             }
-#pragma unroll
-            for (int j = 0; j < NB; ++j)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) s[j][c] = (s[j][c] + s1[j][c]) + sl[j][c];
           } else {
 #pragma unroll
             for (int ks = 0; ks < HD / 16; ++ks)
@@ -399,17 +407,26 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
               split(s[j][3], ph[3], pl[3]);
               const uint32_t key = wk * S::WKEYS + 8 * j + 2 * t4;
 #pragma unroll
-              for (int d = 0; d < OB; ++d) {
-                const uint32_t c = 2 * d + (g >> 2), e = (g & 3) * 4;
-                uint32_t vh[2], vl[2];
-                split(lds(base + at<S>(key, c) + e), vh[0], vl[0]);
-                split(lds(base + at<S>(key + 1, c) + e), vh[1], vl[1]);
-                float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // (added with rounding, see above)
-                mma_tf32(t, pl, vh[0], vh[1]);
-                mma_tf32(t, ph, vl[0], vl[1]);
-                mma_tf32(t, ph, vh[0], vh[1]);
+              for (int d = 0; d < OB; d += 2) {  // two columns at a time: the chains of three MMAs are long
+                uint32_t vh[2][2], vl[2][2];
+                float t[2][4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) o[d][c] += t[c];
+                for (int e = 0; e < 2; ++e) {
+                  const uint32_t c = 2 * (d + e) + (g >> 2), w = (g & 3) * 4;
+                  split(lds(base + at<S>(key, c) + w), vh[e][0], vl[e][0]);
+                  split(lds(base + at<S>(key + 1, c) + w), vh[e][1], vl[e][1]);
+                  t[e][0] = t[e][1] = t[e][2] = t[e][3] = 0.0f;  // (added with rounding, see above)
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) mma_tf32(t[e], pl, vh[e][0], vh[e][1]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) mma_tf32(t[e], ph, vl[e][0], vl[e][1]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) mma_tf32(t[e], ph, vh[e][0], vh[e][1]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                  for (int c = 0; c < 4; ++c) o[d + e][c] += t[e][c];
               }
             }
           } else {
@@ -769,10 +786,11 @@ cudaError_t launch(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
     j.pass[i].rowpart = p.rowpart;
     j.pass[i].grid = p.grid;
     j.pass[i].bm = pl.bm[i];
-    const cudaError_t e = pl.bm[i] == 16   ? launch_pass<T, O, HD, 1, 4>(mk, mv, p, lc)
-                          : pl.bm[i] == 32 ? launch_pass<T, O, HD, 2, 2>(mk, mv, p, lc)
-                          : pl.bm[i] == TC_TILE ? attend_tc(p, sizeof(O) == 4, lc)
-                                           : launch_pass<T, O, HD, 4, 1>(mk, mv, p, lc);
+    cudaError_t e;
+    if (pl.bm[i] == 16) e = launch_pass<T, O, HD, 1, 4>(mk, mv, p, lc);
+    else if (pl.bm[i] == 32) e = launch_pass<T, O, HD, 2, 2>(mk, mv, p, lc);
+    else if constexpr (sizeof(T) == 4) e = launch_pass<T, O, HD, 4, 1>(mk, mv, p, lc);
+    else e = attend_tc(p, sizeof(O) == 4, lc);
     if (e != cudaSuccess) return e;
     lc.pdl = true;
   }
