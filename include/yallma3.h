@@ -215,6 +215,9 @@ int yl_batch_forward(yl_batch* b, yl_session* const* sessions, uint32_t n, const
  *  "gemm_tc_min" token count from which gemm_tc applies (default 96)
  *  "gemm_f16_min" F16 passes of this many tokens on the f16 tensor-core GEMM
  *                (default 16, env YL_GEMM_F16_MIN; 0 = the matvec at every N)
+ *  "paged_share" yl_paged_attention reads a prefix that a batch shares in a
+ *                pass of its own: -1 where that pays (default), 0 never, 1
+ *                wherever it can (also counts for the workspace's size)
  * YL_ERR_ARG for an unknown key. */
 int yl_config_set(const char* key, int64_t value);
 
@@ -515,8 +518,10 @@ int yl_kv_pages_free(yl_kv_pages* p);
  * shared_len (a multiple of page_size): every sequence holds the same pages as
  * the first sequence's table row for its first shared_len positions, as far as
  * it is that long (the first row's entries for them are valid even if its slot
- * is idle). Attention then reads those pages once for all sequences. With 0
- * every sequence's pages are read for itself; the results agree to rounding.
+ * is idle). Attention then reads those pages once for all sequences where that
+ * saves enough (long prefixes, sequences of few rows; yl_config_set
+ * "paged_share"). With 0 every sequence's pages are read for itself; the
+ * results agree to rounding.
  * The arrays are on the device (one call's geometry may be computed there, and
  * a captured graph replays with new contents), so they are checked there, and
  * YL_ERR_RANGE is stored to *status (nullable; never cleared here) for

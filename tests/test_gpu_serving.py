@@ -108,6 +108,13 @@ def test_append_reports_bad_positions(yl, torch_cuda):
 
 # ------------------------------------------------------------- attention ---
 
+@pytest.fixture
+def own_pass(yl):
+    """A shared prefix gets a pass of its own however short it is."""
+    yl.config_set("paged_share", 1)
+    yield
+    yl.config_set("paged_share", -1)
+
 def attend(yl, g, q, k, v, scale, out_dtype=None, shared=None, status=None, fill=7.0, stream=None):
     pages = yl.KvPages.of(k, v)
     batch = g.device(yl, status, shared)
@@ -157,7 +164,7 @@ def test_prompts(yl, torch_cuda, dtype, shape):
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("shape", [(9, 3, 64), (32, 8, 128)])
 @pytest.mark.parametrize("shared", [16, 272, 1024])
-def test_shared_prefix_decode(yl, torch_cuda, dtype, shape, shared):
+def test_shared_prefix_decode(yl, torch_cuda, own_pass, dtype, shape, shared):
     lens = [shared + n for n in (0, 1, 5, 16, 17, 64, 90, 200, 333)]
     g = ref.Geometry(6, *shape, page=16, lens=lens, rows=[1] * 8 + [0], shared=shared, pad_rows=1)
     check_attention(yl, g, DTYPES[dtype])
@@ -165,20 +172,39 @@ def test_shared_prefix_decode(yl, torch_cuda, dtype, shape, shared):
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("shape", [(9, 3, 64), (8, 2, 128)])
-def test_shared_prefix_prompts(yl, torch_cuda, dtype, shape):
+def test_shared_prefix_prompts(yl, torch_cuda, own_pass, dtype, shape):
     """Rows behind the prefix, and rows inside it (a sequence whose chunk begins before the prefix ends)."""
     g = ref.Geometry(7, *shape, page=32, lens=[96 + 70, 96 + 1, 100, 96], rows=[70, 1, 60, 96], shared=96)
     check_attention(yl, g, DTYPES[dtype])
 
 
+@pytest.mark.parametrize("dtype,kv,n", [("f32", 2, 3), ("f16", 2, 8), ("bf16", 1, 50), ("f16", 4, 40)])
+def test_shared_prefix_where_it_pays(yl, torch_cuda, dtype, kv, n):
+    """The rule's own choice: prefixes long enough for a pass of their own (passes side by side, and on tcgen05), and
+    the same without one, which is held to the same bounds."""
+    shared = 12288
+    g = ref.Geometry(40, 4 * kv, kv, 64, page=64, lens=shared + np.arange(n) * 7, rows=[1] * n, shared=shared)
+    batch = g.device(yl)
+    k, v = (torch.empty(g.n_pages, 64, kv, 64, dtype=DTYPES[dtype], device="cuda") for _ in range(2))
+    with_pass = yl.paged_attention_workspace(yl.KvPages.of(k, v), batch, g.heads)
+    yl.config_set("paged_share", 0)
+    try:
+        without = yl.paged_attention_workspace(yl.KvPages.of(k, v), batch, g.heads)
+        check_some_rows(yl, g, DTYPES[dtype], [0, n // 2, n - 1])
+    finally:
+        yl.config_set("paged_share", -1)
+    assert with_pass > without
+    check_some_rows(yl, g, DTYPES[dtype], [0, n // 2, n - 1])
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("shared", [0, 64])
-def test_f32_output_of_16_bit_cache(yl, torch_cuda, dtype, shared):
+def test_f32_output_of_16_bit_cache(yl, torch_cuda, own_pass, dtype, shared):
     g = ref.Geometry(8, 8, 2, 128, page=32, lens=[64 + 30, 64 + 129, 65], rows=[1, 40, 1], shared=64)
     check_attention(yl, g, DTYPES[dtype], shared=shared, out_dtype=torch.float32)
 
 
-def test_long_rows(yl, torch_cuda):
+def test_long_rows(yl, torch_cuda, own_pass):
     """Long sequences, split over many blocks: one token against 40000, next to short ones."""
     for dtype in ("f32", "bf16"):
         g = ref.Geometry(9, 2, 1, 64, page=64, lens=[40000, 3, 12345], rows=[1, 1, 2])
@@ -188,7 +214,7 @@ def test_long_rows(yl, torch_cuda):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
-def test_layouts(yl, torch_cuda, dtype):
+def test_layouts(yl, torch_cuda, own_pass, dtype):
     """Heads before tokens, keys and values interleaved by page, one layer of several, q and output rows inside wider
     ones: the same bits as the plain layout."""
     t = DTYPES[dtype]
@@ -213,7 +239,7 @@ def test_layouts(yl, torch_cuda, dtype):
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-def test_garbage_behind_the_sequences(yl, torch_cuda, dtype, bad):
+def test_garbage_behind_the_sequences(yl, torch_cuda, own_pass, dtype, bad):
     """Slots behind a sequence's last position and pages of nobody hold NaN or infinities: nothing changes."""
     t = DTYPES[dtype]
     g = ref.Geometry(11, 8, 2, 64, page=32, lens=[64 + 9, 64 + 70, 64, 67], rows=[1, 20, 1, 3], shared=64)
@@ -304,7 +330,7 @@ def test_cache_beyond_32_bits(yl, torch_cuda):
     within(lse, wlse, lb, "lse")
 
 
-def test_same_bits_again_and_on_another_stream(yl, torch_cuda):
+def test_same_bits_again_and_on_another_stream(yl, torch_cuda, own_pass):
     g = ref.Geometry(16, 8, 2, 128, page=16, lens=[512 + 900, 512 + 3, 512 + 77], rows=[1, 1, 1], shared=512)
     q, (k, v) = queries(g, torch.bfloat16).cuda(), (x.cuda() for x in g.pool(torch.bfloat16))
     first = attend(yl, g, q, k, v, 0.1)
@@ -339,7 +365,7 @@ def test_one_long_prompt(yl, torch_cuda, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
-def test_many_sequences(yl, torch_cuda, dtype):
+def test_many_sequences(yl, torch_cuda, own_pass, dtype):
     """More sequences than a block has threads, idle slots among them."""
     rng = np.random.default_rng(31)
     lens = rng.integers(1, 90, 700)
@@ -352,7 +378,7 @@ def test_many_sequences(yl, torch_cuda, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
-def test_mixed_prompts_and_tokens(yl, torch_cuda, dtype):
+def test_mixed_prompts_and_tokens(yl, torch_cuda, own_pass, dtype):
     """One prompt chunk next to single tokens, with and without a shared prefix."""
     for shared in (0, 128):
         g = ref.Geometry(33, 6, 2, 128, page=64, lens=[shared + n for n in (400, 1, 17, 90, 300)], rows=[300, 1, 1, 1, 2],
@@ -361,7 +387,7 @@ def test_mixed_prompts_and_tokens(yl, torch_cuda, dtype):
 
 
 @pytest.mark.parametrize("seed", range(24))
-def test_random_geometries(yl, torch_cuda, seed):
+def test_random_geometries(yl, torch_cuda, own_pass, seed):
     rng = np.random.default_rng(1000 + seed)
     pick = lambda *a: a[rng.integers(len(a))]  # noqa: E731
     kv, group, hd = pick(1, 2, 3), pick(1, 2, 3, 4, 5, 7, 8, 12, 16), pick(64, 128)
@@ -394,7 +420,7 @@ def test_row_starts_behind_zero_and_out_of_order(yl, torch_cuda):
     torch.cuda.synchronize()
 
 
-def test_captured_step_follows_its_arrays(yl, torch_cuda):
+def test_captured_step_follows_its_arrays(yl, torch_cuda, own_pass):
     """Append, attention and log probabilities captured once and replayed while the sequences grow: the arrays' new
     contents count, and each replay equals the eager calls."""
     t, hd, heads, kv, vocab = torch.bfloat16, 64, 8, 2, 5000
@@ -511,7 +537,7 @@ def test_pages_from_the_library(yl, torch_cuda):
 
 
 @pytest.mark.parametrize("preset,over", [("tiny", {}), ("tiny", {"llama3_scaling": True}), ("tiny128", {})])
-def test_a_model_layer_served_from_pages(yl, torch_cuda, model_factory, preset, over):
+def test_a_model_layer_served_from_pages(yl, torch_cuda, own_pass, model_factory, preset, over):
     """The step of a server, next to the library's own: the projections of a model's first layer on the rows of three
     sequences that share a prefix, the rows appended with the model's rotation table, attention over the pages. Keys and
     values in an f32 cache have the bits of the decode kernel's cache, the outputs agree within the f32 bound, and a

@@ -108,6 +108,25 @@ def test_empty_calls(yl):
     assert lib.yl_token_logprobs(P, 0, 100, 0, 100, P, P, P, 5, P, P, None) == 0
 
 
+def test_paged_share_counts_for_the_workspace(yl):
+    """The option decides whether a prefix gets a pass (and its parts room); by rule a short one gets none."""
+    lib, p, n = yl.raw_lib(), pages(yl, n_pages=40), C.c_uint64()
+    b = batch(yl, n_seqs=4, n_rows=4, shared_len=32)
+    size = {}
+    for share in (0, 1, -1):
+        yl.config_set("paged_share", share)
+        assert lib.yl_paged_attention_workspace(p, b, 4, n) == 0
+        size[share] = n.value
+    assert size[0] == size[-1] < size[1]
+    b = batch(yl, n_seqs=64, n_rows=64, shared_len=1 << 16, table_stride=1 << 13)
+    assert lib.yl_paged_attention_workspace(p, b, 4, n) == 0
+    by_rule = n.value
+    yl.config_set("paged_share", 0)
+    assert lib.yl_paged_attention_workspace(p, b, 4, n) == 0
+    yl.config_set("paged_share", -1)
+    assert n.value < by_rule
+
+
 HARNESS = r"""
 #include <cassert>
 #include <cstdio>

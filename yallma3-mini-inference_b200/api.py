@@ -199,7 +199,7 @@ def last_error() -> str:
 
 
 def config_set(key: str, value: int) -> None:
-    """Process-wide device-path option (yl_config_set): gemm, gemm_tc, gemm_tc_min, gemm_f16_min."""
+    """Process-wide device-path option (yl_config_set): gemm, gemm_tc, gemm_tc_min, gemm_f16_min, paged_share."""
     _check(_lib.yl_config_set(key.encode(), int(value)))
 
 

@@ -154,6 +154,7 @@ int set_tunable(const std::string& key, int64_t value) {
   else if (key == "gemm_tc_min") t.gemm_tc_min = (uint32_t)std::max<int64_t>(1, value);
   else if (key == "gemm") t.gemm = value != 0;
   else if (key == "gemm_f16_min") t.gemm_f16_min = (uint32_t)std::max<int64_t>(0, value);
+  else if (key == "paged_share") t.paged_share = value < 0 ? -1 : value != 0;
   else return fail(YL_ERR_ARG, "unknown option " + key);
   return YL_OK;
 }

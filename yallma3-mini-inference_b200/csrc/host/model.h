@@ -173,6 +173,7 @@ struct Tunables {
   // decode: L2 prefetch of the next matrix's first bytes per launch (YL_PF_MB).
   // Off: measured slower at every size tried (16, 32, 48 MB).
   uint64_t pf_bytes = 0;
+  int paged_share = -1;      // yl_paged_attention: a pass of its own for a shared prefix (-1: where it pays)
 };
 // Batched decode of independent sessions (one token each per step): the
 // projections run once over the stacked rows, the attention is one launch
@@ -194,7 +195,7 @@ int batch_create(const Model* m, uint32_t cap, Batch** out);
 int forward_batch(Batch* b, Session* const* ss, uint32_t n, const uint32_t* tokens, const uint32_t* pos);
 
 const Tunables& tunables();
-// Runtime override of a tunable (yl_config_set): gemm, gemm_tc, gemm_tc_min, gemm_f16_min.
+// Runtime override of a tunable (yl_config_set): gemm, gemm_tc, gemm_tc_min, gemm_f16_min, paged_share.
 int set_tunable(const std::string& key, int64_t value);
 // Launches the matvec for `ntok` tokens (groups of 8) with activations x*.
 int run_matvec(const DevWeight& w, bool f32act, const int8_t* xq, const float* xs, const float* xf,

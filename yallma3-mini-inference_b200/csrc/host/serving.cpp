@@ -143,7 +143,8 @@ int attention_workspace(const yl_kv_pages* pages, const yl_seq_batch* batch, uin
   if (int rc = make_pages(pages, &a->pages)) return rc;
   if (int rc = make_seqs(batch, pages, &a->seqs)) return rc;
   if (int rc = check_heads(n_heads, pages->n_kv_heads)) return rc;
-  *bytes = k::paged_attention_workspace(a->pages, a->seqs, pages->dtype, n_heads);
+  a->share = tunables().paged_share;
+  *bytes = k::paged_attention_workspace(a->pages, a->seqs, pages->dtype, n_heads, a->share);
   return YL_OK;
 }
 

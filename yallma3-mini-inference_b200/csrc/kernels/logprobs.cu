@@ -19,11 +19,11 @@
 // the order of atomics.
 //
 // Bound by reading the row (4 bytes and one exponential per value): 1999 rows of
-// 128256 f32 in 18x us on one B200 (5.5 TB/s); 64 rows with 20 alternatives 15 us
-// (from L2; the join and the choice of the largest take about 8), one row 6 us. A row is
-// read by a thread-block cluster of 1..8 blocks, more for few rows, so that
-// one row of a large vocabulary does not wait for one SM; its parts are joined
-// over distributed shared memory.
+// 128256 f32 in 186 us on one B200 (5.5 TB/s); 64 rows with 20 alternatives 15 us
+// (from L2; the join and the choice of the largest take about 8), one row 6 us.
+// A row is read by a thread-block cluster of 1..8 blocks, more for few rows, so
+// that one row of a large vocabulary does not wait for one SM; its parts are
+// joined over distributed shared memory.
 #include <cooperative_groups.h>
 
 #include "serve.cuh"

@@ -26,12 +26,17 @@
 // tensor, which reads as zeros) into a ring of 16 KB buffers; the others
 // multiply with mma.sync, WM warps of 16 rows each times WK warps that split
 // the tile's keys and join at the item's end. Decoding has 1..16 rows per
-// item and is bound by reading the cache, so WK = 4; from 33 rows on WK = 1.
+// item and is bound by reading the cache, so WK = 4; f32 from 33 rows on WK = 1.
 // f32 operands are split into two tf32 numbers and multiplied as hi*hi + hi*lo
 // + lo*hi (2^-21 relative); 16-bit ones are exact, and the softmax weights are
 // rounded to their type for the second product (the sum l takes them
 // unrounded), f16 weights at 2^10 times their value so that small ones do not
 // fall below f16's range.
+//
+// Measured on one B200, 32 query and 8 key heads of 128, bf16: 16 sequences of 17
+// to 8000 tokens 52 us (268 MB, 5.2 TB/s; bound by HBM and the items' ends), one
+// of 100000 tokens 72 us (5.7 TB/s); one token of 9 / 3 heads of 64, f32, 301 keys
+// 9 us (two launches, four dependent trips to memory each).
 #include <cmath>
 
 #include "paged_attention.cuh"
@@ -694,15 +699,19 @@ __global__ void __launch_bounds__(128) join_rows_kernel(JoinArgs j) {
 }
 
 // ---- host --------------------------------------------------------------------
-// Row tile for items of `rows` rows.
+// Row tile for items of `rows` rows. Decoding pads to 16 rows. 12, 16 and 32
+// sequences of 4 query heads per key head over 8192 shared tokens (48, 64 and 128
+// rows) took 32.9, 36.9 and 39.7 us on tcgen05 and 37.0, 39.6 and 39.7 us in
+// 64-row tiles on mma.sync; 8 of them (32 rows) 27.7 us on mma.sync and 30.5 on
+// tcgen05. f32 has no tcgen05 form.
 uint32_t tile_rows(uint64_t rows, int dtype) {
   if (dtype != DT_F32 && rows > 32) return TC_TILE;
   return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 // Two blocks per SM; two passes that both leave room for the other get one each
-// and run side by side.
+// and run side by side (12 sequences over 4096 f32 tokens 42 us, one after the
+// other 48).
 uint32_t blocks_of(uint32_t bm, bool beside) { return bm == TC_TILE || beside ? 148 : 2 * 148; }
-
 
 // What a call launches, by its counts alone.
 struct Plan {
@@ -711,16 +720,25 @@ struct Plan {
   uint32_t bm[2];     // row tiles of the sequences' pass, and of the prefix pass
   uint64_t cut[2], desc[2], slots[2], rowpart[2], bytes;  // workspace offsets
 };
-Plan plan_of(const Pages& p, const Seqs& s, int dtype, uint32_t n_heads) {
+Plan plan_of(const Pages& p, const Seqs& s, int dtype, uint32_t n_heads, int share) {
   const uint64_t group = n_heads / p.n_kv_heads, hd = p.head_size;
   const uint64_t each = ((uint64_t)s.n_rows + s.n_seqs - 1) / s.n_seqs * group;
   Plan pl{};
-  // Reading the prefix once pays where an item has few rows; items of many
-  // rows (prompts) read it a few times from L2, without parts to be joined.
-  pl.shared = s.shared_len && s.n_seqs > 1 && each <= 32;
   pl.bm[0] = tile_rows(each, dtype);
   pl.bm[1] = tile_rows((uint64_t)s.n_rows * group, dtype);
-  pl.beside = pl.shared && pl.bm[0] != TC_TILE && pl.bm[1] != TC_TILE;
+  pl.beside = pl.bm[0] != TC_TILE && pl.bm[1] != TC_TILE;
+  // A pass over the prefix for all sequences saves reading it n_seqs - 1 times
+  // (from L2, as a rule) and costs its launch and the joining of every row.
+  // Measured, us with and without it (8 key heads of 128, bf16, own keys 100..300):
+  //   side by side:  4 x 1024 tokens 12.7 / 12.6,  8 x 1024 16.1 / 15.2,  8 x 2048 17.3 / 18.4,  4 x 16384 29 / 43
+  //   on tcgen05:    16 x 1024 23.6 / 19.1,  16 x 2048 25.5 / 26.9,  64 x 512 39 / 36,  64 x 1024 41 / 50
+  //   f32, head 64:  4 x 1024 13.1 / 14.7,  12 x 4096 39 / 59
+  // Rows of a prompt share what they read by themselves: 16 sequences of 16 tokens
+  // (64 rows each) behind 4096 62 / 76, of 32 tokens 91 / 80.
+  const double saved = (s.n_seqs - 1.0) * s.shared_len * p.n_kv_heads * hd * (dtype == DT_F32 ? 8 : 4);
+  const double worth = dtype == DT_F32 ? 8 << 20 : pl.beside ? 40 << 20 : 128 << 20;
+  pl.shared = s.shared_len && s.n_seqs > 1 && each <= 64 && (share < 0 ? saved >= worth : share > 0);
+  pl.beside = pl.beside && pl.shared;
   uint64_t at = 0;
   auto take = [&](uint64_t n) {
     const uint64_t o = at;
@@ -749,7 +767,7 @@ cudaError_t launch_pass(const CUtensorMap& mk, const CUtensorMap& mv, const Pass
 template <typename T, typename O, int HD>
 cudaError_t launch(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
   constexpr uint32_t KT = BUF / (HD * sizeof(T));
-  const Plan pl = plan_of(a.pages, a.seqs, dtype, a.n_heads);
+  const Plan pl = plan_of(a.pages, a.seqs, dtype, a.n_heads, a.share);
   const uint32_t ps = 1u << a.pages.page_shift, tokens = ps < KT ? ps : KT;
   CUtensorMap mk, mv;
   if (!encode_pages(&mk, a.pages, a.pages.k, dtype, tokens) || !encode_pages(&mv, a.pages, a.pages.v, dtype, tokens))
@@ -773,7 +791,11 @@ cudaError_t launch(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
     p.prefix = i;
     p.from = pl.shared && !i ? a.seqs.shared_len : 0;
     p.group = j.group;
-    p.min_chunk = dtype == DT_F32 ? 1 : 2;  // (an f32 tile takes as long as joining its part)
+    // A piece is at least so long: an f32 tile takes as long as joining its part
+    // (one token against 301: pieces of 1 9.0 us, of 2 11.1); 16-bit ones less (8
+    // sequences behind 2048 tokens: 24.5 us with pieces of 1, 17.2 with 2).
+    p.min_chunk = dtype == DT_F32 ? 1 : 2;
+    // (an 8191-token prompt on tcgen05: 722 us without it, 579 with 2, later 544 with 2, 551 with 3, 556 with 4)
     p.item_cost = pl.bm[i] == TC_TILE ? 2 : 1;
     p.joined = pl.shared;
     p.cut = reinterpret_cast<uint4*>(ws + pl.cut[i]);
@@ -815,8 +837,8 @@ cudaError_t paged_attention(const PagedAttnArgs& a, int dtype, bool out_f32, cud
                  : launch_hd<__nv_bfloat16, __nv_bfloat16>(a, dtype, stream);
 }
 
-uint64_t paged_attention_workspace(const Pages& p, const Seqs& s, int dtype, uint32_t n_heads) {
-  const Plan pl = plan_of(p, s, dtype, n_heads);
+uint64_t paged_attention_workspace(const Pages& p, const Seqs& s, int dtype, uint32_t n_heads, int share) {
+  const Plan pl = plan_of(p, s, dtype, n_heads, share);
   return pl.bytes > 256 ? pl.bytes : 256;
 }
 

@@ -91,10 +91,11 @@ struct PagedAttnArgs {
   uint64_t q_stride;
   uint32_t n_heads;
   float scale;
+  int share;  // a pass of its own for the shared prefix: -1 where it pays, 0 never, 1 wherever it can be
   void* workspace;
 };
 cudaError_t paged_attention(const PagedAttnArgs& a, int dtype, bool out_f32, cudaStream_t stream);
-uint64_t paged_attention_workspace(const Pages& p, const Seqs& s, int dtype, uint32_t n_heads);
+uint64_t paged_attention_workspace(const Pages& p, const Seqs& s, int dtype, uint32_t n_heads, int share);
 
 struct LogprobArgs {
   const void* logits;
