@@ -483,7 +483,9 @@ int yl_session_logits(const yl_session* s, float** logits);
  * No counterpart in the reference, which keeps one contiguous f32 cache per
  * session: these are additions of this library for callers that serve many
  * sequences from one cache. All three enqueue on `stream`, allocate nothing,
- * keep no state between calls and may be captured into a graph. */
+ * keep no state between calls and may be captured into a graph. Memory and
+ * stream belong to the current device; outputs overlap no input. A call of no
+ * rows does nothing and may leave the rows' arrays null. */
 
 /* Element type of a paged cache, of its queries, and of logits. */
 enum yl_dtype { YL_DT_F32 = 0, YL_DT_F16 = 1, YL_DT_BF16 = 2 };
@@ -515,9 +517,9 @@ int yl_kv_pages_free(yl_kv_pages* p);
  * padding: they are neither read nor written. Position p of sequence i lies
  * at offset p % page_size of page page_table[i*table_stride + p/page_size];
  * table entries behind the sequence's last position are not used.
- * shared_len (a multiple of page_size): every sequence holds the same pages as
- * the first sequence's table row for its first shared_len positions, as far as
- * it is that long (the first row's entries for them are valid even if its slot
+ * shared_len (a multiple of page_size): every sequence's table row holds the
+ * same pages as the first sequence's for its first shared_len positions, as far
+ * as it is that long (the first row's entries for them are valid even if its slot
  * is idle). Attention then reads those pages once for all sequences where that
  * saves enough (long prefixes, sequences of few rows; yl_config_set
  * "paged_share"). With 0 every sequence's pages are read for itself; the
@@ -569,7 +571,8 @@ int yl_paged_append(void* q_out, uint64_t q_stride, const float* qkv, uint64_t q
  * infinities and NaN included. A value that is not finite reaches all rows
  * that see it, and may reach rows of the same chunk before it (their weight
  * for it is 0, and 0 times infinity is NaN); in an f32 cache an infinite key
- * or value gives NaN. The summation order depends on the batch's geometry
+ * or value gives NaN. A score that is beyond f32 in powers of two (score x
+ * attn_scale x log2 e) gives its row NaN. The summation order depends on the batch's geometry
  * alone: the same call gives the same bits.
  * workspace: device memory of at least the bytes yl_paged_attention_workspace
  * gives for a batch of these counts (n_seqs, n_rows, shared_len) and heads,

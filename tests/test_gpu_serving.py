@@ -736,3 +736,56 @@ def test_logprobs_rows_inside_wider_ones(yl, torch_cuda):
             x = wide[:, start : start + vocab].contiguous()
             check_logprobs(yl, x, torch.tensor([0, 1, vocab - 1, 3, 4], dtype=torch.int32), 7,
                            device_x=dev[:, start : start + vocab])
+
+
+# ------------------------------------------------------------ the mirror ---
+
+def test_calls_without_rows(yl, torch_cuda):
+    """Tensors of no rows have no address; the calls return and touch nothing."""
+    g = ref.Geometry(50, 8, 2, 64, page=16, lens=[20, 5], rows=[0, 0])
+    k, v = (x.cuda() for x in g.pool(torch.bfloat16))
+    before, pages, batch = k.clone(), yl.KvPages.of(k, v), g.device(yl)
+    assert batch.n_rows == 0
+    q = torch.empty(0, 8, 64, dtype=torch.bfloat16, device="cuda")
+    ws = torch.empty(yl.paged_attention_workspace(pages, batch, 8), dtype=torch.uint8, device="cuda")
+    yl.paged_append(torch.empty(0, 12 * 64, device="cuda"), pages, batch, 8, q_out=q)
+    yl.paged_attention(torch.empty_like(q), q, pages, batch, 8, 0.1, ws)
+    i32, f32 = (torch.empty(0, 4, dtype=t, device="cuda") for t in (torch.int32, torch.float32))
+    yl.token_logprobs(torch.empty(0, 100, device="cuda"), i32[:, 0], f32[:, 0], f32[:, 0], i32, f32)
+    torch.cuda.synchronize()
+    assert torch.equal(k, before)
+
+
+def test_mirror_refusals(yl, torch_cuda):
+    """Cache or batch of another device than the current one, halves of the alternatives' outputs, alternatives of
+    different shapes."""
+    g = ref.Geometry(51, 8, 2, 64, page=16, lens=[20, 5], rows=[1, 1])
+    k, v = (x.cuda() for x in g.pool(torch.float32))
+    q, qkv = torch.zeros(2, 8, 64, device="cuda"), torch.zeros(2, 12 * 64, device="cuda")
+    ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    for which in ("pages", "batch"):
+        pages, batch = yl.KvPages.of(k, v), g.device(yl)
+        (pages if which == "pages" else batch).device += 1
+        with pytest.raises(ValueError):
+            yl.paged_append(qkv, pages, batch, 8)
+        with pytest.raises(ValueError):
+            yl.paged_attention(q.clone(), q, pages, batch, 8, 0.1, ws)
+    x = torch.zeros(3, 50, device="cuda")
+    ids, lp = torch.zeros(3, 4, dtype=torch.int32, device="cuda"), torch.zeros(3, 4, device="cuda")
+    for a, b in ((ids, None), (None, lp), (ids, torch.zeros(3, 5, device="cuda"))):
+        with pytest.raises(ValueError):
+            yl.token_logprobs(x, top_ids=a, top_logprobs=b)
+
+
+@pytest.mark.parametrize("dtype,rows", [("f32", 1), ("f32", 30), ("bf16", 1), ("bf16", 6), ("bf16", 90)])
+def test_scores_beyond_f32(yl, torch_cuda, dtype, rows):
+    """A finite score that overflows once it is scaled: NaN, not a row of zeros. Rows of other sequences are as ever."""
+    t = DTYPES[dtype]
+    g = ref.Geometry(52, 4, 1, 64, page=16, lens=[rows, 40], rows=[rows, rows if rows <= 40 else 40])
+    q, (k, v) = queries(g, t), g.pool(t)
+    q[:rows] = 1.5e18
+    for p in g.positions(0):
+        k[int(g.table[0, p // g.page]), int(p % g.page)] = 1.5e18
+    out, lse = attend(yl, g, q.cuda(), k.cuda(), v.cuda(), 4.0)  # 64 * 2.25e36 * 4 log2(e) = 8.3e38
+    assert out[:rows].isnan().all() and lse[:rows].isnan().all()
+    assert out[rows:].isfinite().all() and lse[rows:].isfinite().all()

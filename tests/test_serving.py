@@ -31,7 +31,8 @@ BAD_PAGES = [(dict(dtype=3), -1), (dict(dtype=-1), -1), (dict(head_size=96), -8)
              (dict(page_stride=16 * 128 + 4), -1), (dict(token_stride=1), -1), (dict(head_stride=32), -1),
              (dict(page_stride=1 << 40), -1)]
 BAD_BATCH = [(dict(n_seqs=0), -1), (dict(n_seqs=1 << 21), -1), (dict(n_rows=(1 << 24) + 1), -1),
-             (dict(table_stride=0), -1), (dict(shared_len=8), -1), (dict(shared_len=64), -6), (dict(row_start=None), -1),
+             (dict(table_stride=0), -1), (dict(shared_len=8), -1), (dict(shared_len=64), -6),
+             (dict(shared_len=0x7FFFFF10, table_stride=1 << 30), -6), (dict(row_start=None), -1),
              (dict(seq_len=None), -1), (dict(page_table=None), -1)]
 
 
@@ -106,6 +107,10 @@ def test_empty_calls(yl):
     assert lib.yl_paged_attention_workspace(p, b, 4, n) == 0
     assert lib.yl_paged_attention(P, 256, 1, None, P, 256, p, b, 4, 0.1, P, n.value, None) == 0
     assert lib.yl_token_logprobs(P, 0, 100, 0, 100, P, P, P, 5, P, P, None) == 0
+    # arrays of no rows have no address
+    assert lib.yl_paged_append(None, 256, None, 512, p, b, 4, P, 64, 0, None) == 0
+    assert lib.yl_paged_attention(None, 256, 1, None, None, 256, p, b, 4, 0.1, P, n.value, None) == 0
+    assert lib.yl_token_logprobs(None, 0, 100, 0, 100, None, None, None, 5, None, None, None) == 0
 
 
 def test_paged_share_counts_for_the_workspace(yl):
@@ -154,6 +159,10 @@ int main() {
         }
       }
     assert(page_of(s, p, 0, 0xFFFFFFFFu) == NO_PAGE);
+    // past the last position nothing is looked up, however long the table says it is
+    Seqs endless = s;
+    endless.table_stride = 0xFFFFFFFFu;
+    assert(page_of(endless, p, 0, MAX_POS) == NO_PAGE && page_of(endless, p, 0, 0xFFFFFFFFu) == NO_PAGE);
     // offsets beyond 32 bits
     Pages big{nullptr, nullptr, 10, shift, 3, 64, 1ull << 35, 3 * 64, 64};
     assert(slot_offset(big, 9, 1, 2) == (9ull << 35) + 192 + 128);

@@ -413,6 +413,14 @@ def _row_stride(t, what: str, width: int, n_rows: int, dev: int) -> int:
     return stride[0] if rows > 1 else width
 
 
+def _on_device(pages, batch) -> int:
+    """The current device, on which the cache and the batch's arrays must be."""
+    dev = _device()
+    if pages.device != dev or batch.device != dev:
+        raise ValueError("cache and batch must be on the current CUDA device")
+    return dev
+
+
 def _raw_stream(stream, dev: int) -> int:
     """cudaStream_t of `stream` (torch's current stream where it is None)."""
     if stream is None:
@@ -424,7 +432,10 @@ class KvPages:
     """One layer's paged key/value cache (yl_kv_pages): allocated by the library, or a view of torch tensors."""
 
     def __init__(self, c: KvPagesC, keep=None):
+        if _torch is None:
+            _load_torch()
         self.c = c
+        self.device = _device()
         self.ref = C.byref(c)
         self.dtype, self.n_kv_heads, self.head_size = c.dtype, c.n_kv_heads, c.head_size
         self._keep = keep
@@ -468,6 +479,7 @@ class SeqBatch:
         if _torch is None:
             _load_torch()
         n, dev = seq_len.numel(), _device()
+        self.device = dev
         if page_table.dim() != 2 or page_table.shape[0] != n:
             raise ValueError("page_table must be [n_seqs, slots]")
         self._keep = (row_start, seq_len, page_table, status)
@@ -484,7 +496,7 @@ def paged_append(qkv, pages: KvPages, batch: SeqBatch, n_heads: int, rope_cs=Non
     """Rotates the new rows' queries and keys and writes keys and values to their pages (yl_paged_append). qkv: f32
     rows [q | k | v]; q_out: rows of rotated queries in the cache's type, or None; rope_cs: [len, head_size/2, 2]
     (or an address from Transformer.rope_table, with rope_len), or None for no rotation."""
-    n, hd, dev = batch.n_rows, pages.head_size, _device()
+    n, hd, dev = batch.n_rows, pages.head_size, _on_device(pages, batch)
     if qkv.dtype is not _f32:
         raise TypeError(f"qkv must be float32, got {qkv.dtype}")
     q_ptr = q_stride = 0
@@ -515,7 +527,7 @@ def paged_attention(output, q, pages: KvPages, batch: SeqBatch, n_heads: int, at
     """Causal attention of the batch's rows over the paged cache (yl_paged_attention). q: rows of the cache's type,
     output: rows of that type or f32 ([rows, n_heads, head_size] or flat); lse: f32 [rows, n_heads] or None;
     workspace: a uint8 tensor of at least paged_attention_workspace bytes."""
-    n, dev = batch.n_rows, _device()
+    n, dev = batch.n_rows, _on_device(pages, batch)
     width = n_heads * pages.head_size
     if _dtypes.get(q.dtype) != pages.dtype:
         raise TypeError(f"q must have the cache's type, got {q.dtype}")
@@ -543,6 +555,8 @@ def token_logprobs(logits, tokens=None, logprobs=None, entropy=None, top_ids=Non
     else:
         n, vocab = logits.shape
         ptr, dtype, stride = logits.data_ptr(), _dtype(logits, "logits"), _row_stride(logits, "logits", vocab, n, dev)
+    if (top_ids is None) != (top_logprobs is None) or (top_ids is not None and top_ids.shape != top_logprobs.shape):
+        raise ValueError("top_ids and top_logprobs go together, [rows, k] each")
     k = 0 if top_ids is None else top_ids.shape[-1]
     rc = _lib.yl_token_logprobs(
         ptr, dtype, stride, n, vocab,

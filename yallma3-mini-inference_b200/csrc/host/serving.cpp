@@ -59,6 +59,7 @@ int make_seqs(const yl_seq_batch* b, const yl_kv_pages* p, k::Seqs* out) {
   if (b->table_stride == 0) return fail(YL_ERR_ARG, "empty page table");
   if (b->shared_len % p->page_size) return fail(YL_ERR_ARG, "shared_len must be a multiple of page_size");
   if (b->shared_len / p->page_size > b->table_stride) return fail(YL_ERR_RANGE, "shared_len longer than the page table");
+  if (b->shared_len > k::MAX_POS) return fail(YL_ERR_RANGE, "shared_len beyond the last position");
   if (!b->row_start || !b->seq_len || !b->page_table) return fail(YL_ERR_ARG, "null batch array");
   *out = k::Seqs{b->n_seqs, b->n_rows, b->table_stride, b->shared_len, b->row_start, b->seq_len, b->page_table,
                  b->status};
@@ -71,8 +72,9 @@ int check_heads(uint32_t n_heads, uint32_t n_kv_heads) {
   return YL_OK;
 }
 
-int check_rows(const void* p, uint64_t stride, uint64_t width, uint64_t size, const char* what) {
-  if (!p) return fail(YL_ERR_ARG, std::string("null ") + what);
+// Rows of a call's arrays; a call of no rows may have none.
+int check_rows(const void* p, uint64_t stride, uint64_t width, uint64_t size, uint64_t n_rows, const char* what) {
+  if (!p && n_rows) return fail(YL_ERR_ARG, std::string("null ") + what);
   if (stride < width || stride >= (1ull << 36)) return fail(YL_ERR_ARG, std::string(what) + ": row stride smaller than a row, or too large");
   if (!aligned16(p) || stride * size % 16) return fail(YL_ERR_ARG, std::string(what) + ": rows must be 16-byte aligned");
   return YL_OK;
@@ -123,9 +125,9 @@ int append(void* q_out, uint64_t q_stride, const float* qkv, uint64_t qkv_stride
   if (rope_mode != YL_ROPE_GGUF && rope_mode != YL_ROPE_LLAMA3) return fail(YL_ERR_ARG, "unknown rope mode");
   if (rope_cs && (!aligned16(rope_cs) || rope_len == 0)) return fail(YL_ERR_ARG, "rope table must be 16-byte aligned and not empty");
   const uint64_t hd = pages->head_size;
-  if (int rc = check_rows(qkv, qkv_stride, ((uint64_t)n_heads + 2 * pages->n_kv_heads) * hd, 4, "qkv")) return rc;
+  if (int rc = check_rows(qkv, qkv_stride, ((uint64_t)n_heads + 2 * pages->n_kv_heads) * hd, 4, batch->n_rows, "qkv")) return rc;
   if (q_out)
-    if (int rc = check_rows(q_out, q_stride, n_heads * hd, dtype_size(pages->dtype), "q_out")) return rc;
+    if (int rc = check_rows(q_out, q_stride, n_heads * hd, dtype_size(pages->dtype), batch->n_rows, "q_out")) return rc;
   if (batch->n_rows == 0) return YL_OK;
   a.qkv = qkv;
   a.qkv_stride = qkv_stride;
@@ -157,8 +159,8 @@ int attention(void* output, uint64_t out_stride, int out_dtype, float* lse, cons
   if (out_dtype != YL_DT_F32 && out_dtype != pages->dtype)
     return fail(YL_ERR_UNSUPPORTED, "output must be f32 or of the cache's type");
   const uint64_t width = (uint64_t)n_heads * pages->head_size;
-  if (int rc = check_rows(q, q_stride, width, dtype_size(pages->dtype), "q")) return rc;
-  if (int rc = check_rows(output, out_stride, width, dtype_size(out_dtype), "output")) return rc;
+  if (int rc = check_rows(q, q_stride, width, dtype_size(pages->dtype), batch->n_rows, "q")) return rc;
+  if (int rc = check_rows(output, out_stride, width, dtype_size(out_dtype), batch->n_rows, "output")) return rc;
   if ((uintptr_t)lse % 4) return fail(YL_ERR_ARG, "lse must be 4-byte aligned");
   if (!workspace || (uintptr_t)workspace % 256) return fail(YL_ERR_ARG, "workspace must be 256-byte aligned");
   if (workspace_bytes < need) return fail(YL_ERR_ARG, "workspace smaller than yl_paged_attention_workspace says");
@@ -186,9 +188,9 @@ int logprobs(const void* logits, int dtype, uint64_t row_stride, uint32_t n_rows
   if (row_stride < vocab || row_stride >= (1ull << 36)) return fail(YL_ERR_ARG, "row stride smaller than a row, or too large");
   if (top_k > k::LP_MAX_TOP) return fail(YL_ERR_UNSUPPORTED, "top_k must be at most 32");
   if (top_k > vocab) return fail(YL_ERR_ARG, "top_k larger than the vocabulary");
-  if (!logits || (uintptr_t)logits % size) return fail(YL_ERR_ARG, "logits null or not aligned to their type");
-  if (!tokens != !logprobs) return fail(YL_ERR_ARG, "tokens and logprobs go together");
-  if (top_k && (!top_ids || !top_logprobs)) return fail(YL_ERR_ARG, "top_k needs top_ids and top_logprobs");
+  if ((!logits && n_rows) || (uintptr_t)logits % size) return fail(YL_ERR_ARG, "logits null or not aligned to their type");
+  if (n_rows && !tokens != !logprobs) return fail(YL_ERR_ARG, "tokens and logprobs go together");
+  if (n_rows && top_k && (!top_ids || !top_logprobs)) return fail(YL_ERR_ARG, "top_k needs top_ids and top_logprobs");
   if (((uintptr_t)tokens | (uintptr_t)logprobs | (uintptr_t)entropy | (uintptr_t)top_ids | (uintptr_t)top_logprobs) % 4)
     return fail(YL_ERR_ARG, "outputs and tokens must be 4-byte aligned");
   if (n_rows == 0) return YL_OK;

@@ -460,6 +460,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
       for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(FULL, l[i], 1);
         l[i] += __shfl_xor_sync(FULL, l[i], 2);
+        if (m[i] == INFINITY) l[i] = NAN;  // finite scores whose maximum overflowed have lost their weights
       }
       const bool whole = w.whole();
       if (w.kt0 == 0 && warp == 0) {

@@ -524,6 +524,7 @@ __global__ void __launch_bounds__(384, 1)
       if (!ok) break;
       o_phase ^= 1;
       tc_fence_after();
+      if (mx == INFINITY) l = NAN;  // finite scores whose maximum overflowed have lost their weights
       if (busy) {
         const bool whole = w.whole(), direct = whole && !p.joined;
         const float inv = mx == -INFINITY && l == l ? 0.0f : 1.0f / l;

@@ -48,16 +48,19 @@ YL_SHD uint32_t row_end(const Seqs& s, uint32_t i) {
   const uint32_t b = row_begin(s, i), e = row_begin(s, i + 1);
   return e > b ? e : b;
 }
-// Positions that the page table has slots for (kernels count them in 31 bits).
+// Positions from here on are no positions: kernels count keys, and those of the
+// tile they are in, in 31 bits.
+constexpr uint32_t MAX_POS = 0x7FFFFF00u;
+// Positions that the page table has slots for.
 YL_SHD uint32_t table_limit(const Seqs& s, const Pages& p) {
   const uint64_t n = (uint64_t)s.table_stride << p.page_shift;
-  return n < 0x7FFFFF00ull ? (uint32_t)n : 0x7FFFFF00u;
+  return n < MAX_POS ? (uint32_t)n : MAX_POS;
 }
 // Page that holds position pos of sequence seq, or NO_PAGE where the table
 // has no slot for it or its entry is no page.
 YL_SHD uint32_t page_of(const Seqs& s, const Pages& p, uint32_t seq, uint32_t pos) {
   const uint32_t slot = pos >> p.page_shift;
-  if (slot >= s.table_stride) return NO_PAGE;
+  if (slot >= s.table_stride || pos >= MAX_POS) return NO_PAGE;
   const uint32_t id = s.page_table[(uint64_t)seq * s.table_stride + slot];
   return id < p.n_pages ? id : NO_PAGE;
 }
