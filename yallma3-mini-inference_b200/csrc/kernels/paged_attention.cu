@@ -57,7 +57,7 @@ struct Shape {
   static constexpr int KT = BUF / ROW;             // keys per tile
   static constexpr int WKEYS = KT / WK;
   static constexpr bool F32 = sizeof(T) == 4;
-  static constexpr int NBUF = F32 && HD == 128 ? (WM == 2 ? 3 : 4) : WK > 1 ? 4 : 5;  // what two blocks per SM leave room for
+  static constexpr int NBUF = F32 && HD == 128 && WM == 2 ? 3 : 4;  // what two blocks per SM leave room for
   static constexpr int QP = HD + 4;  // f32 queries and the warps' joining: row stride in shared memory, no bank conflicts
   static constexpr uint32_t Q_BYTES = F32 ? BM * QP * 4 : 0;
   static constexpr uint32_t M_BYTES = WK > 1 ? NW * 16 * QP * 4 : 0;
@@ -94,6 +94,12 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
   hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
   lo = __float_as_uint(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ void split2(uint32_t x, uint32_t y, uint32_t (&hi)[2], uint32_t (&lo)[2]) {
+  hi[0] = (x + 0x1000u) & 0xFFFFE000u, hi[1] = (y + 0x1000u) & 0xFFFFE000u;
+  const float2 l = fma2(make_float2(__uint_as_float(hi[0]), __uint_as_float(hi[1])), make_float2(-1.0f, -1.0f),
+                        make_float2(__uint_as_float(x), __uint_as_float(y)));
+  lo[0] = __float_as_uint(l.x), lo[1] = __float_as_uint(l.y);
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -207,7 +213,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
     // ---- consumers ----
     Walk<S> w(p, tpt, start);
     const uint32_t wm = warp / WK, wk = warp % WK, g = lane >> 2, t4 = lane & 3;
-    const uint32_t flip = p.flip ? (S::F32 ? 0x80000000u : 0x80008000u) : 0;  // sign bits of q
+    const uint32_t flip = p.flip ? 0x80008000u : 0;  // sign bits of 16-bit q
     constexpr int NB = S::WKEYS / 8, OB = HD / 8;
     uint32_t n = 0;
     bool ok = true;
@@ -249,7 +255,10 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
             v = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) +
                                                  (uint64_t)(w.r.row0 + w.t + m / p.group) * a.q_stride +
                                                  (uint64_t)(w.head * p.group + m % p.group) * HD + 4 * c);
-          if (flip) v = make_float4(-v.x, -v.y, -v.z, -v.w);
+          // f32 queries take the factor, in two f32, with one rounding: scores come in powers of two
+          const float sc = p.flip ? -p.sc : p.sc, lo = p.flip ? -p.sc_lo : p.sc_lo;
+          v = make_float4(fmaf(v.x, sc, v.x * lo), fmaf(v.y, sc, v.y * lo), fmaf(v.z, sc, v.z * lo),
+                          fmaf(v.w, sc, v.w * lo));
           *reinterpret_cast<float4*>(qs + m * S::QP + 4 * c) = v;
         }
         named_bar_sync(1, 32 * S::NW);
@@ -298,30 +307,30 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
 #pragma unroll 2
               for (int ks = 0; ks < HD / 16; ++ks) {  // 16 elements: two k-steps of 8
                 uint32_t ah[2][4], al[2][4];
+                // (split again for every tile: kept split, in shared memory, the loads
+                // cost more than the arithmetic, 455 us and not 428 as below)
                 const float* q0 = qs + (wm * 16 + g) * S::QP + 16 * ks + t4;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  split(q0[8 * h], ah[h][0], al[h][0]);
-                  split(q0[8 * h + 8 * S::QP], ah[h][1], al[h][1]);
-                  split(q0[8 * h + 4], ah[h][2], al[h][2]);
-                  split(q0[8 * h + 4 + 8 * S::QP], ah[h][3], al[h][3]);
-                }
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) split(q0[8 * h + 8 * (i & 1) * S::QP + 4 * (i >> 1)], ah[h][i], al[h][i]);
+                // (all splits, then the products across the keys: the chains are as long as they look)
+                uint32_t bh[JG][2][2], bl[JG][2][2];
 #pragma unroll
                 for (int j = 0; j < JG; ++j) {
                   uint32_t r[4];
                   ldsm4(r, base + at<S>(wk * S::WKEYS + 8 * (j0 + j) + (lane & 7), 4 * ks + (lane >> 3)));
-                  uint32_t bh[2][2], bl[2][2];
+                  split2(r[0], r[1], bh[j][0], bl[j][0]);
+                  split2(r[2], r[3], bh[j][1], bl[j][1]);
+                }
 #pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    split(__uint_as_float(r[2 * h]), bh[h][0], bl[h][0]);
-                    split(__uint_as_float(r[2 * h + 1]), bh[h][1], bl[h][1]);
-                  }
-                  mma_tf32(s[j0 + j], ah[0], bh[0][0], bh[0][1]);
-                  mma_tf32(sl[j], al[0], bh[0][0], bh[0][1]);
-                  mma_tf32(s1[j], ah[1], bh[1][0], bh[1][1]);
-                  mma_tf32(sl[j], ah[0], bl[0][0], bl[0][1]);
-                  mma_tf32(sl[j], al[1], bh[1][0], bh[1][1]);
-                  mma_tf32(sl[j], ah[1], bl[1][0], bl[1][1]);
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                  for (int j = 0; j < JG; ++j) mma_tf32(sl[j], al[h], bh[j][h][0], bh[j][h][1]);
+#pragma unroll
+                  for (int j = 0; j < JG; ++j) mma_tf32(h ? s1[j] : s[j0 + j], ah[h], bh[j][h][0], bh[j][h][1]);
+#pragma unroll
+                  for (int j = 0; j < JG; ++j) mma_tf32(sl[j], ah[h], bl[j][h][0], bl[j][h][1]);
                 }
               }
 #pragma unroll
@@ -346,20 +355,23 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
         ++n;
         float corr[2];
         if (busy) {
-          const bool mask = k0 + S::KT > all_see;
+          if (k0 + S::KT > all_see) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                if ((int32_t)(k0 + wk * S::WKEYS + 8 * j + 2 * t4 + (c & 1)) >= lim[c >> 1]) s[j][c] = -INFINITY;
+          }
           float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
           for (int j = 0; j < NB; ++j)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              if (mask && (int32_t)(k0 + wk * S::WKEYS + 8 * j + 2 * t4 + (c & 1)) >= lim[c >> 1]) s[j][c] = -INFINITY;
-              top[c >> 1] = fmaxf(top[c >> 1], s[j][c]);
-            }
+            for (int c = 0; c < 4; ++c) top[c >> 1] = fmaxf(top[c >> 1], s[j][c]);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             top[i] = fmaxf(top[i], __shfl_xor_sync(FULL, top[i], 1));
             top[i] = fmaxf(top[i], __shfl_xor_sync(FULL, top[i], 2));
-            const float mn = fmaxf(m[i], top[i] * p.sc);
+            const float mn = fmaxf(m[i], S::F32 ? top[i] : top[i] * p.sc);
             const float ref = mn == -INFINITY ? 0.0f : mn - SHIFT;
             corr[i] = ex2(m[i] - (mn == -INFINITY ? 0.0f : mn));  // 0 from -inf
             m[i] = mn;
@@ -368,10 +380,8 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
             for (int j = 0; j < NB; ++j)
 #pragma unroll
               for (int c = 2 * i; c < 2 * i + 2; ++c) {
-                // the product with the factor is exact before the maximum is taken off
-                float d = fmaf(s[j][c], p.sc, -ref);
-                if (S::F32) d = fmaf(fmaxf(s[j][c], -1e30f), p.sc_lo, d);  // (-inf stays in d alone)
-                s[j][c] = ex2(d);
+                // (the product with the factor is exact before the maximum is taken off)
+                s[j][c] = ex2(S::F32 ? s[j][c] - ref : fmaf(s[j][c], p.sc, -ref));
                 sum += s[j][c];
               }
             l[i] = l[i] * corr[i] + sum;
@@ -402,32 +412,44 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
             __syncwarp();
           }
           if constexpr (S::F32) {
+            constexpr int JP = NB < 2 ? 1 : 2;  // 16 keys in a chain (2000 tokens of 32 / 8 heads of 64: 428 us; of 8 keys 470, of 32 no less)
 #pragma unroll
-            for (int j = 0; j < NB; ++j) {
+            for (int j = 0; j < NB; j += JP) {
               // keys 2i of the eight are the MMA's k = i, keys 2i+1 its k = 4+i: the weights are where QK left them
-              uint32_t ph[4], pl[4];
-              split(s[j][0], ph[0], pl[0]);
-              split(s[j][2], ph[1], pl[1]);
-              split(s[j][1], ph[2], pl[2]);
-              split(s[j][3], ph[3], pl[3]);
+              uint32_t ph[JP][4], pl[JP][4];
+#pragma unroll
+              for (int x = 0; x < JP; ++x) {
+                split(s[j + x][0], ph[x][0], pl[x][0]);
+                split(s[j + x][2], ph[x][1], pl[x][1]);
+                split(s[j + x][1], ph[x][2], pl[x][2]);
+                split(s[j + x][3], ph[x][3], pl[x][3]);
+              }
               const uint32_t key = wk * S::WKEYS + 8 * j + 2 * t4;
 #pragma unroll
-              for (int d = 0; d < OB; d += 2) {  // two columns at a time: the chains of three MMAs are long
-                uint32_t vh[2][2], vl[2][2];
+              for (int d = 0; d < OB; d += 2) {  // two columns at a time: the chains are long
+                uint32_t vh[JP][2][2], vl[JP][2][2];
                 float t[2][4];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                   const uint32_t c = 2 * (d + e) + (g >> 2), w = (g & 3) * 4;
-                  split(lds(base + at<S>(key, c) + w), vh[e][0], vl[e][0]);
-                  split(lds(base + at<S>(key + 1, c) + w), vh[e][1], vl[e][1]);
+#pragma unroll
+                  for (int x = 0; x < JP; ++x) {
+                    split(lds(base + at<S>(key + 8 * x, c) + w), vh[x][e][0], vl[x][e][0]);
+                    split(lds(base + at<S>(key + 8 * x + 1, c) + w), vh[x][e][1], vl[x][e][1]);
+                  }
                   t[e][0] = t[e][1] = t[e][2] = t[e][3] = 0.0f;  // (added with rounding, see above)
                 }
 #pragma unroll
-                for (int e = 0; e < 2; ++e) mma_tf32(t[e], pl, vh[e][0], vh[e][1]);
+                for (int x = 0; x < JP; ++x) {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) mma_tf32(t[e], ph, vl[e][0], vl[e][1]);
+                  for (int e = 0; e < 2; ++e) mma_tf32(t[e], pl[x], vh[x][e][0], vh[x][e][1]);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) mma_tf32(t[e], ph, vh[e][0], vh[e][1]);
+                  for (int e = 0; e < 2; ++e) mma_tf32(t[e], ph[x], vl[x][e][0], vl[x][e][1]);
+                }
+#pragma unroll
+                for (int x = 0; x < JP; ++x)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) mma_tf32(t[e], ph[x], vh[x][e][0], vh[x][e][1]);
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
