@@ -36,7 +36,11 @@
 // Measured on one B200, 32 query and 8 key heads of 128, bf16: 16 sequences of 17
 // to 8000 tokens 52 us (268 MB, 5.2 TB/s; bound by HBM and the items' ends), one
 // of 100000 tokens 72 us (5.7 TB/s); one token of 9 / 3 heads of 64, f32, 301 keys
-// 9 us (two launches, four dependent trips to memory each).
+// 9 us (two launches, four dependent trips to memory each); a prompt of 2000
+// tokens of 32 / 8 heads of 64, f32, 428 us, of which its 3 x 8 million tf32 MMAs
+// (8.2 cycles each per scheduler) would take 190: two warps per scheduler at 168
+// registers wait for one another's chains. More warps with fewer registers spill:
+// 440 us with three blocks per SM, 515 with eight warps per block.
 #include <cmath>
 
 #include "paged_attention.cuh"
@@ -732,8 +736,8 @@ uint32_t tile_rows(uint64_t rows, int dtype) {
   return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 // Two blocks per SM; two passes that both leave room for the other get one each
-// and run side by side (12 sequences over 4096 f32 tokens 42 us, one after the
-// other 48).
+// and run side by side (12 sequences over 4096 f32 tokens 38.6 us, one after the
+// other 45.0).
 uint32_t blocks_of(uint32_t bm, bool beside) { return bm == TC_TILE || beside ? 148 : 2 * 148; }
 
 // What a call launches, by its counts alone.
@@ -755,7 +759,7 @@ Plan plan_of(const Pages& p, const Seqs& s, int dtype, uint32_t n_heads, int sha
   // Measured, us with and without it (8 key heads of 128, bf16, own keys 100..300):
   //   side by side:  4 x 1024 tokens 12.7 / 12.6,  8 x 1024 16.1 / 15.2,  8 x 2048 17.3 / 18.4,  4 x 16384 29 / 43
   //   on tcgen05:    16 x 1024 23.6 / 19.1,  16 x 2048 25.5 / 26.9,  64 x 512 39 / 36,  64 x 1024 41 / 50
-  //   f32, head 64:  4 x 1024 13.1 / 14.7,  12 x 4096 39 / 59
+  //   f32, head 64:  4 x 1024 12.7 / 14.1,  12 x 1024 20 / 22,  12 x 4096 35 / 55
   // Rows of a prompt share what they read by themselves: 16 sequences of 16 tokens
   // (64 rows each) behind 4096 62 / 76, of 32 tokens 91 / 80.
   const double saved = (s.n_seqs - 1.0) * s.shared_len * p.n_kv_heads * hd * (dtype == DT_F32 ? 8 : 4);
@@ -815,7 +819,7 @@ cudaError_t launch(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
     p.from = pl.shared && !i ? a.seqs.shared_len : 0;
     p.group = j.group;
     // A piece is at least so long: an f32 tile takes as long as joining its part
-    // (one token against 301: pieces of 1 9.0 us, of 2 11.1); 16-bit ones less (8
+    // (one token against 301: pieces of 1 8.9 us, of 2 10.1); 16-bit ones less (8
     // sequences behind 2048 tokens: 24.5 us with pieces of 1, 17.2 with 2).
     p.min_chunk = dtype == DT_F32 ? 1 : 2;
     // (an 8191-token prompt on tcgen05: 722 us without it, 579 with 2, later 544 with 2, 551 with 3, 556 with 4)
