@@ -822,8 +822,11 @@ cudaError_t launch(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
     // (one token against 301: pieces of 1 8.9 us, of 2 10.1); 16-bit ones less (8
     // sequences behind 2048 tokens: 24.5 us with pieces of 1, 17.2 with 2).
     p.min_chunk = dtype == DT_F32 ? 1 : 2;
-    // (an 8191-token prompt on tcgen05: 722 us without it, 579 with 2, later 544 with 2, 551 with 3, 556 with 4)
-    p.item_cost = pl.bm[i] == TC_TILE ? 2 : 1;
+    // 16-bit items cost as much as two tiles more (with 1 / 2 / 3: 64 sequences of up
+    // to 1000 tokens 41.0 / 33.3 / 33.5 us, of 6 rows each 66 / 52 / 48, an 8191-token
+    // prompt on tcgen05 579 / 544 / 551, without any 722); an f32 tile takes as long as
+    // an item's ends (a 900-token prompt of 9 / 3 heads 77 / 78 / 91).
+    p.item_cost = dtype == DT_F32 ? 1 : 2;
     p.joined = pl.shared;
     p.cut = reinterpret_cast<uint4*>(ws + pl.cut[i]);
     p.desc = reinterpret_cast<uint2*>(ws + pl.desc[i]);
