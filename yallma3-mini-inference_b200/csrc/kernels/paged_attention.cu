@@ -612,7 +612,8 @@ __device__ __forceinline__ void join_row(const PagedAttnArgs& a, uint32_t row, u
   for (int e = 0; e < PER; ++e) o[e] = 0.0f;
   constexpr uint32_t U = 4;  // parts in flight
   for (uint32_t i0 = first; i0 < n; i0 += U * each) {
-    float pm[U], pl[U], po[U][PER];
+    float pm[U], pl[U];
+    __align__(16) float po[U][PER];
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
       pm[u] = -INFINITY, pl[u] = 0.0f;
@@ -622,9 +623,8 @@ __device__ __forceinline__ void join_row(const PagedAttnArgs& a, uint32_t row, u
         const float* q = part(i0 + u * each);
         const float2 ml = *reinterpret_cast<const float2*>(q + HD);
         pm[u] = ml.x, pl[u] = ml.y;
-#pragma unroll
-        for (int e = 0; e < PER; e += 2)
-          *reinterpret_cast<float2*>(&po[u][e]) = *reinterpret_cast<const float2*>(q + PER * lane + e);
+        if constexpr (PER == 4) *reinterpret_cast<float4*>(po[u]) = *reinterpret_cast<const float4*>(q + PER * lane);
+        else *reinterpret_cast<float2*>(po[u]) = *reinterpret_cast<const float2*>(q + PER * lane);
       }
     }
     const float top = fmaxf(m, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]))), ref = top == -INFINITY ? 0.0f : top;
@@ -683,11 +683,10 @@ __global__ void __launch_bounds__(256) join_cut_kernel(JoinArgs j) {
   const auto& ps = j.pass[0];
   const uint4 c = ps.cut[blockIdx.x];  // {first row, tokens, head, blocks}
   const uint32_t rows = c.y * j.group, n = c.w, warp = threadIdx.x >> 5;
+  const uint32_t slot = ps.bm * PART<HD>;
   auto each_part = [&](uint32_t mr) {
-    return [&, mr](uint32_t i) -> const float* {
-      const uint64_t slot = i == 0 ? 2ull * blockIdx.x + 1 : 2ull * (blockIdx.x + i);
-      return ps.slots + (slot * ps.bm + mr) * PART<HD>;
-    };
+    const float* at = ps.slots + (2ull * blockIdx.x * ps.bm + mr) * PART<HD>;
+    return [at, slot](uint32_t i) { return at + (i ? 2 * i : 1) * slot; };
   };
   if (n > 8) {
     for (uint32_t mr = blockIdx.y; mr < rows; mr += gridDim.y)
@@ -715,12 +714,18 @@ __global__ void __launch_bounds__(128) join_rows_kernel(JoinArgs j) {
     // (row ranges that overlap or leave gaps: nothing outside the workspace is read)
     if (d[p].y >> 16 && ((uint64_t)d[p].x + n[p] > j.pass[p].grid || (d[p].y & 0xFFFFu) >= j.pass[p].bm / j.group)) return;
   }
-  auto part = [&](uint32_t i) -> const float* {
+  const float* at[2];
+  uint32_t slot[2];  // 0: the whole item, in rowpart
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    slot[p] = d[p].y >> 16 ? j.pass[p].bm * PART<HD> : 0;
+    at[p] = slot[p] ? j.pass[p].slots + (2ull * d[p].x * j.pass[p].bm + (d[p].y & 0xFFFFu) * j.group + head % j.group) * PART<HD>
+                    : j.pass[p].rowpart + ((uint64_t)row * a.n_heads + head) * PART<HD>;
+  }
+  auto part = [&](uint32_t i) {
     const int p = i < n[0] ? 0 : 1;
     const uint32_t k = p ? i - n[0] : i;
-    if (!(d[p].y >> 16)) return j.pass[p].rowpart + ((uint64_t)row * a.n_heads + head) * PART<HD>;
-    const uint64_t slot = k == 0 ? 2ull * d[p].x + 1 : 2ull * (d[p].x + k);
-    return j.pass[p].slots + (slot * j.pass[p].bm + (d[p].y & 0xFFFFu) * j.group + head % j.group) * PART<HD>;
+    return (p ? at[1] : at[0]) + (k ? 2 * k : 1) * (p ? slot[1] : slot[0]);
   };
   join_row<O, HD>(a, row, head, n[0] + n[1], part, threadIdx.x >> 5, 4, meet);
 }
