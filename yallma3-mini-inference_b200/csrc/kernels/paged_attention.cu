@@ -34,7 +34,7 @@
 // fall below f16's range.
 //
 // Measured on one B200, 32 query and 8 key heads of 128, bf16: 16 sequences of 17
-// to 8000 tokens 52 us (268 MB, 5.2 TB/s; bound by HBM and the items' ends), one
+// to 8000 tokens 51 us (268 MB, 5.2 TB/s; bound by HBM and the items' ends), one
 // of 100000 tokens 72 us (5.7 TB/s); one token of 9 / 3 heads of 64, f32, 301 keys
 // 9 us (two launches, four dependent trips to memory each); a prompt of 2000
 // tokens of 32 / 8 heads of 64, f32, 428 us, of which its 3 x 8 million tf32 MMAs
