@@ -789,3 +789,40 @@ def test_scores_beyond_f32(yl, torch_cuda, dtype, rows):
     out, lse = attend(yl, g, q.cuda(), k.cuda(), v.cuda(), 4.0)  # 64 * 2.25e36 * 4 log2(e) = 8.3e38
     assert out[:rows].isnan().all() and lse[:rows].isnan().all()
     assert out[rows:].isfinite().all() and lse[rows:].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("vocab", [49152, 128256, 50001])
+@pytest.mark.parametrize("rows", [1, 3, 64, 200])
+def test_logprobs_near_certain_rows_of_several_blocks(yl, torch_cuda, dtype, vocab, rows):
+    """Rows of one to eight blocks, nearly certain of a token anywhere in them (first and last values, odd rows of an odd
+    vocabulary that begin and end inside 16 bytes): S' = S - 1 from 1e-9 over values a few last bits of 1 around the
+    border 2^-7, where the sum is taken again, to 2^-5.
+    Below the border everything is relative to S' (sums in chains of V/512 + 64 of two half steps each, exp of an f32
+    difference d: |d| * 4 half steps, exp itself 8), above it S has lost what the general bound allows."""
+    t = DTYPES[dtype]
+    rng = np.random.default_rng(vocab + rows)
+    gen = torch.Generator(device="cuda").manual_seed(vocab + rows)
+    x = torch.randn(rows, vocab, generator=gen, device="cuda").to(t)
+    places = [0, vocab - 1, vocab // 2, 1, vocab // 8, vocab // 8 - 1, vocab - 2, 7 * vocab // 8, 3, vocab // 4 + 1]
+    at = torch.tensor([places[i % 10] if i < 20 else int(rng.integers(vocab)) for i in range(rows)], device="cuda")
+    near = [2.0**-7 * (1 + (i % 17 - 8) * 2.0**-17) for i in range(rows)]
+    target = torch.tensor([near[i] if i % 2 else (1e-9, 1e-6, 2.0**-12, 2.0**-8, 2.0**-6, 2.0**-5)[i // 2 % 6]
+                           for i in range(rows)], dtype=torch.float64, device="cuda")
+    r = torch.arange(rows, device="cuda")
+    x[r, at] = -math.inf
+    rest = x.double().exp().sum(1)
+    x[r, at] = (rest / target).log().to(t)
+    d = x.double() - x.double()[r, at][:, None]
+    assert (d <= 0).all()
+    e = d.exp()
+    e[r, at] = 0.0
+    s, w = e.sum(1), (e * d).sum(1)  # S', W
+    far = float(-d.min())
+    lp, en, ids, _ = run_logprobs(yl, x, at.int(), 2)
+    rel = (vocab / 512 + 64) * 2 * ref.U32 + 8 * ref.U32 + 4 * ref.U32 * far
+    below = s < 2.0**-7 * (1 - 2.0**-10)
+    scale = torch.where(below, s, 1.0)
+    within(lp, -s.log1p(), rel * scale + 4 * ref.U32 * s, "logprobs")
+    within(en, s.log1p() - w / (1 + s), 2 * rel * scale * (1 + far) + 4 * ref.U32 * s * (1 + far), "entropy")
+    assert torch.equal(ids[:, 0], at.cpu().int())

@@ -332,6 +332,10 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(LogprobArgs a) 
   Part q = {-INFINITY, 0.0f, 0.0f};
   if (lane < C) q = C > 1 ? cluster.map_shared_rank(&sh, lane)->whole : sh.whole;
   q = warp_join(q);
+  // Lanes join in different orders and may end a last bit apart (a product and a
+  // sum are fused in one order and not in the other). Barriers depend on the
+  // value below: every thread of the row's blocks takes what lane 0 has.
+  q = {__shfl_sync(FULL, q.m, 0), __shfl_sync(FULL, q.s, 0), __shfl_sync(FULL, q.w, 0)};
   // NaN, +inf, or nothing above -inf: no distribution
   const bool none = isnan(q.s) || fabsf(q.m) == INFINITY;
   float rest = q.s - 1.0f;  // S'
