@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes as C
 import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -185,3 +186,37 @@ def test_index_arithmetic(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=address,undefined", f"-I{inc}", "-I/usr/local/cuda/include",
                     str(src), "-o", str(exe)], check=True)
     assert subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout == "ok\n"
+
+
+@pytest.fixture
+def mirror(yl, monkeypatch):
+    """The Python mirror on CPU tensors (whose device is -1): its checks and the library's, up to a launch."""
+    import torch
+    api = sys.modules[yl.__name__ + ".api"]
+    for name, value in dict(_torch=torch, _dtypes={torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}, _f32=torch.float32,
+                            _i32=torch.int32, _u8=torch.uint8, _device=lambda: -1, _stream_of=lambda dev: 0).items():
+        monkeypatch.setattr(api, name, value)
+    return yl
+
+
+def mirror_batch(yl, **kw):
+    import torch
+    ints = lambda *shape: torch.zeros(*shape, dtype=torch.int32)  # noqa: E731
+    return yl.SeqBatch(ints(3), ints(2), ints(2, 3), **{**dict(n_rows=2), **kw})
+
+
+def test_pages_of_expanded_tensors(mirror):
+    """Heads, tokens or pages that lie on one another are refused, not taken for others behind them; an axis of one
+    entry may have any stride."""
+    import torch
+    yl, b = mirror, mirror_batch(mirror)
+    for shape, to in (((4, 16, 1, 64), (4, 16, 2, 64)), ((4, 1, 2, 64), (4, 16, 2, 64)), ((1, 16, 2, 64), (4, 16, 2, 64))):
+        k = torch.zeros(*shape).expand(*to)
+        with pytest.raises(yl.YlError, match="strides"):
+            yl.paged_attention_workspace(yl.KvPages.of(k, k), b, 2)
+    k = torch.zeros(4, 16, 2, 64).as_strided((4, 16, 2, 64), (2048, 128, 32, 1))
+    with pytest.raises(yl.YlError, match="strides"):
+        yl.paged_attention_workspace(yl.KvPages.of(k, k), b, 2)
+    for k in (torch.zeros(4, 16, 1, 64).as_strided((4, 16, 1, 64), (1024, 64, 1, 1)), torch.zeros(1, 16, 2, 64).expand(1, 16, 2, 64),
+              torch.zeros(16, 2, 64).as_strided((1, 16, 2, 64), (0, 128, 64, 1))):
+        assert yl.paged_attention_workspace(yl.KvPages.of(k, k), b, 2) > 0

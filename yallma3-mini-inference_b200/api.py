@@ -457,7 +457,8 @@ class KvPages:
         if k.get_device() != _device() or v.get_device() != _device():
             raise ValueError("k and v must be on the current CUDA device")
         n, ps, h, hd = k.shape
-        sp, st, sh, _ = (max(x, hd) for x in k.stride())
+        # (an axis of one entry has any stride; the others' are refused by the calls where heads would overlap)
+        sp, st, sh = (x if size > 1 else hd for x, size in zip(k.stride(), k.shape[:3]))
         return cls(KvPagesC(_dtype(k, "pages"), 0, n, ps, h, hd, sp, st, sh, k.data_ptr(), v.data_ptr()), (k, v))
 
     def free(self) -> None:
