@@ -534,7 +534,8 @@ int yl_kv_pages_free(yl_kv_pages* p);
  *  - a row to append at a position before 0 or beyond the rope table: the row
  *    is left out.
  * row_start values are limited to n_rows and to ascending order. A device wait
- * that runs out stores YL_ERR_TIMEOUT. */
+ * that runs out stores YL_ERR_TIMEOUT. Without a status word nothing tells of
+ * any of these. All arrays are 4-byte aligned. */
 typedef struct yl_seq_batch {
   uint32_t n_seqs, n_rows, table_stride, shared_len;
   const uint32_t* row_start;  /* [n_seqs + 1] */

@@ -220,3 +220,11 @@ def test_pages_of_expanded_tensors(mirror):
     for k in (torch.zeros(4, 16, 1, 64).as_strided((4, 16, 1, 64), (1024, 64, 1, 1)), torch.zeros(1, 16, 2, 64).expand(1, 16, 2, 64),
               torch.zeros(16, 2, 64).as_strided((1, 16, 2, 64), (0, 128, 64, 1))):
         assert yl.paged_attention_workspace(yl.KvPages.of(k, k), b, 2) > 0
+
+
+@pytest.mark.parametrize("name", ["row_start", "seq_len", "page_table", "status"])
+def test_batch_arrays_off_their_alignment(yl, name):
+    lib, p, b, n = yl.raw_lib(), pages(yl), batch(yl, **{name: P + 2}), C.c_uint64()
+    refused(yl, lib.yl_paged_append(P, 256, P, 512, p, b, 4, P, 64, 0, None), -1)
+    refused(yl, lib.yl_paged_attention_workspace(p, b, 4, n), -1)
+    refused(yl, lib.yl_paged_attention(P, 256, 1, None, P, 256, p, b, 4, 0.1, P, 1 << 30, None), -1)

@@ -61,6 +61,8 @@ int make_seqs(const yl_seq_batch* b, const yl_kv_pages* p, k::Seqs* out) {
   if (b->shared_len / p->page_size > b->table_stride) return fail(YL_ERR_RANGE, "shared_len longer than the page table");
   if (b->shared_len > k::MAX_POS) return fail(YL_ERR_RANGE, "shared_len beyond the last position");
   if (!b->row_start || !b->seq_len || !b->page_table) return fail(YL_ERR_ARG, "null batch array");
+  if (((uintptr_t)b->row_start | (uintptr_t)b->seq_len | (uintptr_t)b->page_table | (uintptr_t)b->status) % 4)
+    return fail(YL_ERR_ARG, "batch arrays must be 4-byte aligned");
   *out = k::Seqs{b->n_seqs, b->n_rows, b->table_stride, b->shared_len, b->row_start, b->seq_len, b->page_table,
                  b->status};
   return YL_OK;
