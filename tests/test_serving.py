@@ -228,3 +228,19 @@ def test_batch_arrays_off_their_alignment(yl, name):
     refused(yl, lib.yl_paged_append(P, 256, P, 512, p, b, 4, P, 64, 0, None), -1)
     refused(yl, lib.yl_paged_attention_workspace(p, b, 4, n), -1)
     refused(yl, lib.yl_paged_attention(P, 256, 1, None, P, 256, p, b, 4, 0.1, P, 1 << 30, None), -1)
+
+
+def test_counts_that_wrap_in_32_bits(mirror):
+    """Counts that C would take modulo 2^32: refused before they could name rows or positions that are not there."""
+    import torch
+    yl, k = mirror, torch.zeros(4, 16, 2, 64)
+    for kw in (dict(n_rows=-1), dict(n_rows=2 - (1 << 32)), dict(shared_len=-16), dict(shared_len=1 << 32)):
+        with pytest.raises(ValueError):
+            mirror_batch(yl, **kw)
+    qkv, cs = torch.zeros(2, 6 * 64), torch.zeros(32, 32, 2)
+    for cs_or_address, n in ((cs, -1), (cs, 16 - (1 << 32)), (P, -1), (P, 1 << 32)):
+        with pytest.raises(ValueError):
+            yl.paged_append(qkv, yl.KvPages.of(k, k.clone()), mirror_batch(yl), 2, rope_cs=cs_or_address, rope_len=n)
+    for shape in (None, (2,), (-1, 100), (1 - (1 << 32), 100), (2, -1)):
+        with pytest.raises(ValueError):
+            yl.token_logprobs(P, entropy=torch.zeros(2), shape=shape)

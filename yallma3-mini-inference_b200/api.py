@@ -483,6 +483,8 @@ class SeqBatch:
         self.device = dev
         if page_table.dim() != 2 or page_table.shape[0] != n:
             raise ValueError("page_table must be [n_seqs, slots]")
+        if not (0 <= n_rows < 1 << 32 and 0 <= shared_len < 1 << 32):
+            raise ValueError(f"n_rows and shared_len must be 32-bit counts, got {n_rows} and {shared_len}")
         self._keep = (row_start, seq_len, page_table, status)
         self.n_rows = n_rows
         self.c = SeqBatchC(n, n_rows, page_table.shape[1], shared_len,
@@ -509,6 +511,8 @@ def paged_append(qkv, pages: KvPages, batch: SeqBatch, n_heads: int, rope_cs=Non
         rows = rope_cs.shape[0]
         rope_len = rows if rope_len is None else min(rope_len, rows)
         rope_cs = _flat(rope_cs, "rope_cs", _f32, rows * hd, dev)
+    if rope_len is not None and not 0 <= rope_len < 1 << 32:
+        raise ValueError(f"rope_len must be a number of positions, got {rope_len}")
     rc = _lib.yl_paged_append(q_ptr, q_stride, qkv.data_ptr(),
                               _row_stride(qkv, "qkv", (n_heads + 2 * pages.n_kv_heads) * hd, n, dev), pages.ref,
                               batch.ref, n_heads, rope_cs, rope_len or 0, rope_mode, _raw_stream(stream, dev))
@@ -551,6 +555,8 @@ def token_logprobs(logits, tokens=None, logprobs=None, entropy=None, top_ids=Non
         _load_torch()
     dev = _device()
     if isinstance(logits, int):
+        if shape is None or len(shape) != 2 or min(shape) < 0:
+            raise ValueError(f"logits given by address need their shape (rows, vocab), got {shape}")
         (n, vocab), ptr, dtype = shape, logits, 0
         stride = vocab
     else:
