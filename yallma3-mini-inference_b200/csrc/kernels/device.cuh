@@ -256,6 +256,17 @@ __device__ __forceinline__ void l2_prefetch_next(const k::L2Prefetch& pf, uint32
 __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
+// The same, and whether `yes` holds in all of them.
+__device__ __forceinline__ bool named_bar_all(int id, int nthreads, bool yes) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\t"
+      "bar.red.and.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(id), "r"(nthreads), "r"((uint32_t)yes)
+      : "memory");
+  return all != 0;
+}
 
 // ---- integer dot ----------------------------------------------------------
 __device__ __forceinline__ int dp4a(int a, int b, int c) { return __dp4a(a, b, c); }

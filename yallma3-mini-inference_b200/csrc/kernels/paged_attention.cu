@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
 
       uint32_t qf[S::F32 ? 1 : HD / 16][4];
       if constexpr (S::F32) {
-        named_bar_sync(1, 32 * S::NW);  // every warp is done with the item before
+        // (every warp is done with the item before: they met at its end)
         for (uint32_t u = threadIdx.x; u < S::BM * (HD / 4); u += 32 * S::NW) {
           const uint32_t m = u / (HD / 4), c = u % (HD / 4);
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -479,9 +479,14 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
         if (lane == 0) mbar_arrive(&empty[b]);
         ++n;
       }
-      if (!ok) break;
-
       // ---- the item's end ----
+      // All consumers meet, those too whose wait ran out, and leave together or go
+      // on together: nobody is left at this barrier or at the item's next ones.
+      // (A warp that gave up hands no buffer on, so the others' waits for later
+      // ones run out as well.) Behind it nobody reads this item's queries or the
+      // join's buffers of the item before.
+      ok = named_bar_all(1, 32 * S::NW, ok);
+      if (!ok) break;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(FULL, l[i], 1);
@@ -505,7 +510,6 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
       const bool direct = whole && !p.joined;
       if constexpr (WK > 1) {
         // the warps of a row group join over shared memory
-        named_bar_sync(1, 32 * S::NW);  // the item before has been read
         float* mine = join + warp * 16 * S::QP;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
