@@ -826,3 +826,26 @@ def test_logprobs_near_certain_rows_of_several_blocks(yl, torch_cuda, dtype, voc
     within(lp, -s.log1p(), rel * scale + 4 * ref.U32 * s, "logprobs")
     within(en, s.log1p() - w / (1 + s), 2 * rel * scale * (1 + far) + 4 * ref.U32 * s * (1 + far), "entropy")
     assert torch.equal(ids[:, 0], at.cpu().int())
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("hd", [64, 128])
+def test_hidden_values_weigh_nothing(yl, torch_cuda, own_pass, dtype, hd):
+    """The last tokens' values are as large as the type allows, nearly: rows before them keep their bits, in chunks on
+    tcgen05 and on mma.sync, and rows that end inside a shared prefix."""
+    t = DTYPES[dtype]
+    large = 6e4 if dtype == "f16" else 1e37
+    for lens, rows, shared in (([100, 300], [100, 90], 0), ([40, 90, 33], [3, 4, 2], 0), ([128 + 40, 90], [30, 20], 128)):
+        g = ref.Geometry(60, 4, 2, hd, page=32, lens=lens, rows=rows, shared=shared)
+        q, (k, v) = queries(g, t), g.pool(t)
+        clean = attend(yl, g, q.cuda(), k.cuda(), v.cuda(), 0.125)
+        before = []
+        for i, n in enumerate(lens):
+            last = n - 20 if rows[i] > 20 else n - 1
+            if shared and n < shared:
+                continue  # (its last tokens are everyone's)
+            for p in range(last, n):
+                v[int(g.table[i, p // g.page]), p % g.page] = large
+            before += [int(g.row_start[i]) + j for j, p in enumerate(g.positions(i)) if p < last]
+        got = attend(yl, g, q.cuda(), k.cuda(), v.cuda(), 0.125)
+        assert before and torch.equal(got[0][before], clean[0][before]) and torch.equal(got[1], clean[1])

@@ -120,13 +120,14 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // 2^x for x up to 127 without the special-function unit, which gives 16 results
 // per clock and SM and would bound the softmax: x = n + f, |f| <= 1/2, 2^f by a
 // polynomial fitted to it by least squares of the relative error on Chebyshev
-// nodes (2^-22, as ex2.approx), times 2^n. Below -126 it stays at 2^-126, next
-// to which every weight is 0; NaN stays NaN.
+// nodes (off by 2^-22.2 at most, roundings included, as ex2.approx), times 2^n.
+// Below -126.5 n is -127, whose exponent field is 0: the result is 0, as it
+// is for hidden keys (-inf), whose values may be anything finite. NaN stays NaN.
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
   constexpr float C0 = 1.00000012f, C1 = 0.693146944f, C2 = 0.240221217f, C3 = 0.0555074252f, C4 = 0.00967545994f,
                   C5 = 0.0013266971f;
   constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are n
-  x = make_float2(max_nan(x.x, -126.0f), max_nan(x.y, -126.0f));
+  x = make_float2(max_nan(x.x, -127.0f), max_nan(x.y, -127.0f));
   const float2 t = add2(x, make_float2(MAGIC, MAGIC));
   const float2 n = add2(t, make_float2(-MAGIC, -MAGIC));
   const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
