@@ -849,3 +849,31 @@ def test_hidden_values_weigh_nothing(yl, torch_cuda, own_pass, dtype, hd):
             before += [int(g.row_start[i]) + j for j, p in enumerate(g.positions(i)) if p < last]
         got = attend(yl, g, q.cuda(), k.cuda(), v.cuda(), 0.125)
         assert before and torch.equal(got[0][before], clean[0][before]) and torch.equal(got[1], clean[1])
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_garbage_in_a_prefix_behind_sequences_inside_it(yl, torch_cuda, own_pass, dtype, bad, hd):
+    """Sequences that end inside the shared prefix do not see what lies behind them there: not a value that others read,
+    nor what nobody has written yet. Decoding, small and large chunks, passes of every shape."""
+    t = DTYPES[dtype]
+    for lens, rows in (([100, 296, 257, 30, 326], [1, 1, 1, 1, 1]), ([100, 296, 257, 30, 326], [1, 3, 1, 3, 20]),
+                       ([100, 30, 150], [1, 1, 1]), ([150, 30, 199], [30, 12, 20]),
+                       ([100 + 3 * i for i in range(20)] + [270] * 20, [1] * 40)):
+        g = ref.Geometry(61, 4, 2, hd, page=32, lens=lens, rows=rows, shared=256)
+        q, (k, v) = queries(g, t), g.pool(t)
+        check = attend(yl, g, q.cuda(), k.cuda(), v.cuda(), 0.125)
+        want, wlse, ob, lb = ref.attention(g, q, k, v, 0.125)
+        within(check[0], want, ob + (want.abs() + ob) * ref.half_step(t) + 2.0**-25 * (t == torch.float16), "out")
+        within(check[1], wlse, lb, "lse")
+        for p in range(200, 256):
+            k[int(g.table[0, p // g.page]), p % g.page] = bad
+            v[int(g.table[0, p // g.page]), p % g.page] = bad
+        out, lse = attend(yl, g, q.cuda(), k.cuda(), v.cuda(), 0.125)
+        for i, n in enumerate(lens):
+            mine = slice(int(g.row_start[i]), int(g.row_start[i + 1]))
+            if n <= 200:
+                assert torch.equal(out[mine], check[0][mine]) and torch.equal(lse[mine], check[1][mine]), (lens, i)
+            else:
+                assert not out[mine].isfinite().any(), (lens, i)

@@ -17,7 +17,8 @@
 //
 // Shared prefix: a first launch lets the rows of all sequences attend to the
 // prefix together, as rows of one sequence (its keys are read once per row
-// tile, not once per sequence), a second one to the rest; the parts are joined
+// tile, not once per sequence), a second one to the rest, or, for sequences
+// that begin or end inside the prefix, to all they see; the parts are joined
 // likewise. Blocks of the second start as those of the first end (programmatic
 // dependent launch; it waits for the first only before it ends).
 //
@@ -174,8 +175,8 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
       const uint32_t kend = w.kend(), tseq = p.prefix ? 0 : w.seq;
       if (lane == 0 && !p.prefix && a.seqs.status && w.r.pos0 + (int64_t)w.r.n > (int64_t)w.r.limit)
         *a.seqs.status = STATUS_RANGE;
-      for (uint32_t kt = w.kt0; kt < w.kt1 && ok; ++kt) {
-        const uint32_t k0 = p.from + kt * S::KT;
+      uint32_t k0 = w.kbegin();
+      for (uint32_t left = w.kt1 - w.kt0; left && ok; --left, k0 += S::KT) {
         const uint32_t live = kend > k0 ? min(pieces, (kend - k0 + tb - 1) / tb) : 0;  // loads with a visible key
         for (uint32_t kv = 0; kv < 2 && ok; ++kv, ++n) {
           const uint32_t b = n % S::NBUF, round = n / S::NBUF;
@@ -236,10 +237,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
         int64_t e = w.r.pos0 + w.t + tok + 1;
         if (p.prefix) {
           e = kend;
-          if (start.masked && live[i]) {
-            const uint32_t s = find_seq(a.seqs, row[i]);
-            e = (int64_t)a.seqs.seq_len[s] - row_end(a.seqs, s) + row[i] + 1;
-          }
+          if (start.masked && live[i] && left_out(a.seqs, row[i])) e = 0;
         }
         lim[i] = live[i] ? (int32_t)(e < 0 ? 0 : e < (int64_t)kend ? e : kend) : 0x7FFFFFFF;
       }
@@ -284,8 +282,8 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
       const bool busy = wm * 16 < nrow;  // a warp without a row only hands the buffers on
 
-      for (uint32_t kt = w.kt0; kt < w.kt1 && ok; ++kt) {
-        const uint32_t k0 = p.from + kt * S::KT;
+      uint32_t k0 = w.kbegin();
+      for (uint32_t left = w.kt1 - w.kt0; left && ok; --left, k0 += S::KT) {
         uint32_t b = n % S::NBUF;
         uint32_t base = smem_u32(smem) + b * BUF;
         ok = mbar_wait(&full[b], (n / S::NBUF) & 1, nullptr);
@@ -547,6 +545,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
             if (c == 0 && a.lse)
               a.lse[(uint64_t)r * a.n_heads + h] = sum == 0.0f ? -INFINITY : (top - SHIFT + log2f(sum)) * LN2;
           } else {
+            if (sum == 0.0f) acc = make_float4(0.f, 0.f, 0.f, 0.f);  // no key seen: 0 times what was there, which may be NaN
             float* d = part(mr, r, h);
             reinterpret_cast<float2*>(d + 4 * c)[0] = make_float2(acc.x, acc.y);
             reinterpret_cast<float2*>(d + 4 * c)[1] = make_float2(acc.z, acc.w);
@@ -573,7 +572,8 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
             float* d0 = part(wm * 16 + g + 8 * i, row[i], head[i]);
 #pragma unroll
             for (int d = 0; d < OB; ++d)
-              *reinterpret_cast<float2*>(d0 + 8 * d + 2 * t4) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+              *reinterpret_cast<float2*>(d0 + 8 * d + 2 * t4) =
+                  l[i] == 0.0f ? make_float2(0.f, 0.f) : make_float2(o[d][2 * i], o[d][2 * i + 1]);  // (as above)
             if (t4 == 0) d0[HD] = m[i] - SHIFT, d0[HD + 1] = l[i];
           }
         }

@@ -14,7 +14,8 @@ constexpr float LN2 = 0.6931471805599453f;
 constexpr int STATUS_TIMEOUT = -7;  // YL_ERR_TIMEOUT
 
 // One launch: over the sequences' own keys (from `from` on), or over the
-// shared prefix with all rows as one sequence.
+// shared prefix with all rows as one sequence. A sequence whose rows do not all
+// see the whole prefix (starts_inside) has all of its keys in the first.
 struct Pass {
   PagedAttnArgs a;
   int dtype;
@@ -99,6 +100,10 @@ __device__ __forceinline__ Rows rows_of(const Pass& p, uint32_t i) {
   }
   return r;
 }
+// First key of the pass for these rows.
+__device__ __forceinline__ uint32_t keys_begin(const Pass& p, const Rows& r) {
+  return p.from && r.pos0 + 1 < (int64_t)p.from ? 0 : p.from;
+}
 // First key behind those that tokens [.., t) of the sequence see.
 __device__ __forceinline__ uint32_t keys_end(const Pass& p, const Rows& r, uint32_t t) {
   if (p.prefix) return r.limit;
@@ -109,8 +114,8 @@ __device__ __forceinline__ uint32_t keys_end(const Pass& p, const Rows& r, uint3
 // the line it takes item_cost units more, before its first tile.
 template <typename S>
 __device__ __forceinline__ uint32_t tiles_of(const Pass& p, const Rows& r, uint32_t t) {
-  const uint32_t e = keys_end(p, r, t);
-  return e > p.from + S::KT ? (e - p.from + S::KT - 1) / S::KT : 1;
+  const uint32_t b = keys_begin(p, r), e = keys_end(p, r, t);
+  return e > b + S::KT ? (e - b + S::KT - 1) / S::KT : 1;
 }
 __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
 #pragma unroll 1
@@ -148,7 +153,7 @@ struct Start {
   uint64_t begin, end, chunk;  // on the line
   uint32_t seq, head, t;       // sequence, head, first token of the row tile
   uint64_t g0;                 // where the item begins on the line
-  int masked;                  // prefix pass: some row does not see all of the prefix
+  int masked;                  // prefix pass: some sequence is left to the other pass
 };
 
 // a / b; 64-bit division is a long piece of code that hardly ever runs.
@@ -167,12 +172,9 @@ __device__ void find_start(const Pass& p, uint32_t tpt, Start* out, uint64_t* sc
   const uint32_t n = p.prefix ? 1 : p.a.seqs.n_seqs;
   constexpr uint32_t NWARPS = S::THREADS / 32;
   bool masked = false;
-  if (p.prefix)  // rows inside the prefix
+  if (p.prefix)
 #pragma unroll 1
-    for (uint32_t i = tid; i < p.a.seqs.n_seqs; i += S::THREADS) {
-      const uint32_t rn = row_end(p.a.seqs, i) - row_begin(p.a.seqs, i);
-      masked |= rn && (int64_t)p.a.seqs.seq_len[i] - rn + 1 < (int64_t)p.a.seqs.shared_len;
-    }
+    for (uint32_t i = tid; i < p.a.seqs.n_seqs; i += S::THREADS) masked |= starts_inside(p.a.seqs, i);
   if (tid == 0) out->seq = 0xFFFFFFFFu;
   Rows r{};
   uint64_t per_head = 0, mine = 0, first = 0;  // this thread's sequence of the width: units, and where they begin
@@ -304,6 +306,7 @@ struct Walk {
     return cut();
   }
   __device__ uint32_t tokens() const { return r.n - t < tpt ? r.n - t : tpt; }
+  __device__ uint32_t kbegin() const { return keys_begin(p, r) + kt0 * S::KT; }  // of the piece
   __device__ uint32_t kend() const { return keys_end(p, r, t + tpt); }
   // All of the item lies in this block; else how many blocks it lies in, this
   // one, where it begins, the first.
@@ -313,15 +316,15 @@ struct Walk {
   }
 };
 
-// Sequence of a row by bisection (rows inside the prefix only).
-__device__ uint32_t find_seq(const Seqs& s, uint32_t row) {
+// Whether the prefix pass leaves this row to the other one (the row's sequence by bisection).
+__device__ __forceinline__ bool left_out(const Seqs& s, uint32_t row) {
   uint32_t lo = 0, hi = s.n_seqs;
   while (hi - lo > 1) {
     const uint32_t mid = (lo + hi) / 2;
     if (row_begin(s, mid) <= row) lo = mid;
     else hi = mid;
   }
-  return lo;
+  return starts_inside(s, lo);
 }
 
 // (element, head, token, page), boxes of 128 bytes x 1 x `tokens` x 1, swizzled.

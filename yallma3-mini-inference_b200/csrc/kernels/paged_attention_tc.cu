@@ -251,8 +251,8 @@ __global__ void __launch_bounds__(384, 1)
                  &q_full);
       }
       ++items;
-      for (uint32_t kt = w.kt0; kt < w.kt1 && ok; ++kt) {
-        const uint32_t k0 = p.from + kt * S::KT;
+      uint32_t k0 = w.kbegin();
+      for (uint32_t left = w.kt1 - w.kt0; left && ok; --left, k0 += S::KT) {
         const uint32_t live = kend > k0 ? min(pieces, (kend - k0 + tb - 1) / tb) : 0;  // loads with a visible key
         // the tile's pages, one per lane: the same for keys and values (pieces <= 16, NH <= 2)
         const uint32_t piece = lane / S::NH, col = lane % S::NH, pos = k0 + piece * tb;
@@ -341,8 +341,9 @@ __global__ void __launch_bounds__(384, 1)
       if (mine) qk(n % S::NBUF);
       release(&empty[n % S::NBUF], mine);
       if (nt == 1) release(&q_empty, mine);
-      for (uint32_t i = 0; i < nt; ++i) {
-        const uint32_t v = n + 1, kn = n + 2, k0 = p.from + (w.kt0 + i) * S::KT;
+      uint32_t k0 = w.kbegin();
+      for (uint32_t i = 0; i < nt; ++i, k0 += S::KT) {
+        const uint32_t v = n + 1, kn = n + 2;
         const bool more = i + 1 < nt;
         if (!wait_full(v)) break;
         if (mine && k0 + S::KT > kend) {
@@ -420,18 +421,15 @@ __global__ void __launch_bounds__(384, 1)
         e = e0 = kend;
         if (start.masked) {
           e0 = 0;
-          if (live) {
-            const uint32_t s = find_seq(a.seqs, row);
-            e = (int64_t)a.seqs.seq_len[s] - row_end(a.seqs, s) + row + 1;
-          }
+          if (live && left_out(a.seqs, row)) e = 0;
         }
       }
       const uint32_t lim = e < 0 ? 0 : e < (int64_t)kend ? (uint32_t)e : kend;
       const uint32_t all_see = e0 < 0 ? 0 : e0 < (int64_t)kend ? (uint32_t)e0 : kend;
       float mx = -INFINITY, l = 0.0f;  // the maximum that O and l are taken relative to, in powers of two
 
-      for (uint32_t kt = w.kt0; kt < w.kt1; ++kt) {
-        const uint32_t k0 = p.from + kt * S::KT;
+      uint32_t k0 = w.kbegin();
+      for (uint32_t kt = w.kt0; kt < w.kt1; ++kt, k0 += S::KT) {
         ok = mbar_wait(&s_full[x], s_phase, nullptr);
         ok = __all_sync(FULL, ok);
         if (!ok) break;
@@ -555,6 +553,10 @@ __global__ void __launch_bounds__(384, 1)
                 for (int i = 0; i < 32; i += 8) store32(out + 32 * c + i, o + i, wide);
               }
             } else {
+              if (l == 0.0f) {  // no key seen: 0 times what was there, which may be NaN
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = 0;
+              }
 #pragma unroll
               for (int i = 0; i < 32; i += 8) store32(part + 32 * c + i, o + i, true);
             }

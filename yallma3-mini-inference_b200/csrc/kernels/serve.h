@@ -48,6 +48,14 @@ YL_SHD uint32_t row_end(const Seqs& s, uint32_t i) {
   const uint32_t b = row_begin(s, i), e = row_begin(s, i + 1);
   return e > b ? e : b;
 }
+// Whether some row of the sequence does not see the whole shared prefix. Such a
+// sequence is attended to by itself: the keys of the prefix behind its end are
+// other sequences', or nobody's yet, and a weight of 0 does not hide a value
+// that is not finite.
+YL_SHD bool starts_inside(const Seqs& s, uint32_t i) {
+  const uint32_t n = row_end(s, i) - row_begin(s, i);
+  return n && (int64_t)s.seq_len[i] - n + 1 < (int64_t)s.shared_len;
+}
 // Positions from here on are no positions: kernels count keys, and those of the
 // tile they are in, in 31 bits.
 constexpr uint32_t MAX_POS = 0x7FFFFF00u;
