@@ -572,9 +572,10 @@ int yl_paged_append(void* q_out, uint64_t q_stride, const float* qkv, uint64_t q
  * infinities and NaN included. A value that is not finite reaches all rows
  * that see it, and may reach rows of the same chunk before it (their weight
  * for it is 0, and 0 times infinity is NaN); in an f32 cache an infinite key
- * or value gives NaN. A score that is beyond f32 in powers of two (score x
- * attn_scale x log2 e) gives its row NaN. The summation order depends on the batch's geometry
- * alone: the same call gives the same bits.
+ * or value gives NaN. Scores are held in powers of two (score x attn_scale
+ * x log2 e): one above f32's range gives its row NaN, one below it weighs 0,
+ * and a row that sees none but such gets NaN too. The summation order depends
+ * on the batch's geometry alone: the same call gives the same bits.
  * workspace: device memory of at least the bytes yl_paged_attention_workspace
  * gives for a batch of these counts (n_seqs, n_rows, shared_len) and heads,
  * 256-byte aligned, with any contents; not to be shared by calls that may

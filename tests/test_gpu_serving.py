@@ -877,3 +877,30 @@ def test_garbage_in_a_prefix_behind_sequences_inside_it(yl, torch_cuda, own_pass
                 assert torch.equal(out[mine], check[0][mine]) and torch.equal(lse[mine], check[1][mine]), (lens, i)
             else:
                 assert not out[mine].isfinite().any(), (lens, i)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 3, 6, 30, 90])
+def test_scores_below_f32(yl, torch_cuda, own_pass, dtype, rows):
+    """Finite scores that overflow downwards once they are scaled: next to a score in range such a key weighs nothing,
+    and a row of nothing else is NaN, not a row of zeros that looks like one without keys. In one piece, in many, and
+    in passes that join."""
+    t = DTYPES[dtype]
+    for lens, shared in (([90, 100, 95], 0), ([5000, 90, 300], 0), ([64 + 90, 64 + 95, 64 + 100], 64)):
+        n = min(rows, 30) if shared else rows
+        g = ref.Geometry(62, 4, 1, 64, page=16, lens=lens, rows=[n, n, n], shared=shared)
+        q, (k, v) = queries(g, t), g.pool(t)
+        q[: 2 * n] = 1.5e18
+        for i in (0, 1):
+            for p in range(lens[i]):
+                k[int(g.table[i, p // g.page]), p % g.page] = -1.5e18  # 64 * 2.25e36 * 4 log2(e) = 8.3e38
+        k[int(g.table[1, (lens[1] - n) // g.page]), (lens[1] - n) % g.page] = 0.0  # every row's one key in range
+        out, lse = attend(yl, g, q.cuda(), k.cuda(), v.cuda(), 4.0)
+        assert out[:n].isnan().all() and lse[:n].isnan().all(), (lens, shared)
+        one = v[int(g.table[1, (lens[1] - n) // g.page]), (lens[1] - n) % g.page].double()
+        within(out[n : 2 * n], one.expand(n, 4, 64), (one.abs() * (2.0**-20 + ref.half_step(t))).expand(n, 4, 64), "one key")
+        within(lse[n : 2 * n], torch.zeros(n, 4), torch.full((n, 4), 2.0**-20), "lse")
+        if not shared:  # (the prefix's keys of the third are the others')
+            want, wlse, ob, lb = ref.attention(g, q, k, v, 4.0, only=set(range(2 * n, 3 * n)))
+            within(out[2 * n :], want[2 * n :], (ob + (want.abs() + ob) * ref.half_step(t))[2 * n :], "out")
+            within(lse[2 * n :], wlse[2 * n :], lb[2 * n :], "lse")

@@ -490,6 +490,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
         l[i] += __shfl_xor_sync(FULL, l[i], 1);
         l[i] += __shfl_xor_sync(FULL, l[i], 2);
         if (m[i] == INFINITY) l[i] = NAN;  // finite scores whose maximum overflowed have lost their weights
+        if (l[i] == 0.0f && lim[i] > (int32_t)(w.kbegin() + wk * S::WKEYS)) m[i] = BELOW;
       }
       const bool whole = w.whole();
       if (w.kt0 == 0 && warp == 0) {
@@ -536,6 +537,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
           }
           const uint32_t r = w.r.row0 + w.t + mr / p.group, h = w.head * p.group + mr % p.group;
           if (direct) {
+            sum = settled(top, sum);
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             O* out = static_cast<O*>(a.out) + (uint64_t)r * a.out_stride + (uint64_t)h * HD + 4 * c;
             if constexpr (sizeof(O) == 4)
@@ -545,7 +547,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
             if (c == 0 && a.lse)
               a.lse[(uint64_t)r * a.n_heads + h] = sum == 0.0f ? -INFINITY : (top - SHIFT + log2f(sum)) * LN2;
           } else {
-            if (sum == 0.0f) acc = make_float4(0.f, 0.f, 0.f, 0.f);  // no key seen: 0 times what was there, which may be NaN
+            if (top == -INFINITY) acc = make_float4(0.f, 0.f, 0.f, 0.f);  // no key seen: 0 times what was there, which may be NaN
             float* d = part(mr, r, h);
             reinterpret_cast<float2*>(d + 4 * c)[0] = make_float2(acc.x, acc.y);
             reinterpret_cast<float2*>(d + 4 * c)[1] = make_float2(acc.z, acc.w);
@@ -557,6 +559,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
         for (int i = 0; i < 2; ++i) {
           if (!live[i]) continue;
           if (direct) {
+            l[i] = settled(m[i], l[i]);
             const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
             O* out = static_cast<O*>(a.out) + (uint64_t)row[i] * a.out_stride + (uint64_t)head[i] * HD + 2 * t4;
 #pragma unroll
@@ -573,7 +576,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
 #pragma unroll
             for (int d = 0; d < OB; ++d)
               *reinterpret_cast<float2*>(d0 + 8 * d + 2 * t4) =
-                  l[i] == 0.0f ? make_float2(0.f, 0.f) : make_float2(o[d][2 * i], o[d][2 * i + 1]);  // (as above)
+                  m[i] == -INFINITY ? make_float2(0.f, 0.f) : make_float2(o[d][2 * i], o[d][2 * i + 1]);  // (as above)
             if (t4 == 0) d0[HD] = m[i] - SHIFT, d0[HD + 1] = l[i];
           }
         }
@@ -666,6 +669,7 @@ __device__ __forceinline__ void join_row(const PagedAttnArgs& a, uint32_t row, u
       for (int e = 0; e < PER; ++e) o[e] += f * meet[w][PER * lane + e];
     }
   }
+  l = settled(m, l);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   O* out = static_cast<O*>(a.out) + (uint64_t)row * a.out_stride + (uint64_t)head * HD + PER * lane;
 #pragma unroll

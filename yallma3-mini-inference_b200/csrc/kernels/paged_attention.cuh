@@ -2,6 +2,7 @@
 // line and cut into pieces (paged_attention.cu tells why), and the page loads.
 #pragma once
 #include <atomic>
+#include <cfloat>
 #include <type_traits>
 
 #include "serve.cuh"
@@ -63,6 +64,11 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// A part (m, l, O) of a row that sees none of its keys has m = -inf and l = 0. One
+// whose scores are all below f32's range has l = 0 too; its m is this, below any
+// score, so that it weighs nothing next to other parts, and alone gives NaN.
+constexpr float BELOW = -FLT_MAX;
+__device__ __forceinline__ float settled(float m, float l) { return l == 0.0f && m != -INFINITY ? NAN : l; }
 // 4-D tiled load of a page's part: (element, head, token in the page, page).
 __device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t head, uint32_t tok,
                                          uint32_t page, uint64_t* bar) {

@@ -526,9 +526,11 @@ __global__ void __launch_bounds__(384, 1)
       o_phase ^= 1;
       tc_fence_after();
       if (mx == INFINITY) l = NAN;  // finite scores whose maximum overflowed have lost their weights
+      if (l == 0.0f && lim > w.kbegin()) mx = BELOW;
       if (busy) {
         const bool whole = w.whole(), direct = whole && !p.joined;
-        const float inv = mx == -INFINITY && l == l ? 0.0f : 1.0f / l;
+        if (direct) l = settled(mx, l);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         float* part = whole ? p.rowpart + ((uint64_t)row * a.n_heads + head) * PART<HD>
                             : p.slots + ((uint64_t)(2 * blockIdx.x + (w.kt0 == 0 ? 1 : 0)) * TC_TILE + tok * p.group + gh) * PART<HD>;
         O* out = static_cast<O*>(a.out) + (uint64_t)row * a.out_stride + (uint64_t)head * HD;
@@ -553,7 +555,7 @@ __global__ void __launch_bounds__(384, 1)
                 for (int i = 0; i < 32; i += 8) store32(out + 32 * c + i, o + i, wide);
               }
             } else {
-              if (l == 0.0f) {  // no key seen: 0 times what was there, which may be NaN
+              if (mx == -INFINITY) {  // no key seen: 0 times what was there, which may be NaN
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = 0;
               }
@@ -564,7 +566,7 @@ __global__ void __launch_bounds__(384, 1)
         }
         if (live) {
           if (!direct) part[HD] = mx - SHIFT, part[HD + 1] = l;
-          else if (a.lse) a.lse[(uint64_t)row * a.n_heads + head] = mx == -INFINITY && l == l ? -INFINITY : (mx - SHIFT + log2f(l)) * LN2;
+          else if (a.lse) a.lse[(uint64_t)row * a.n_heads + head] = l == 0.0f ? -INFINITY : (mx - SHIFT + log2f(l)) * LN2;
         }
       }
       tc_fence_before();  // O has been read before the next item's first product, which waits for its weights
