@@ -496,7 +496,8 @@ enum yl_dtype { YL_DT_F32 = 0, YL_DT_F16 = 1, YL_DT_BF16 = 2 };
  * three axes, so several layers may share one allocation). k and v and every
  * stride are multiples of 16 bytes. page_size: a power of two, 8..256;
  * head_size: 64 or 128. Filled in by the caller, or by yl_kv_pages_alloc
- * (zeroed, [n_pages][page_size][n_kv_heads][head_size]). */
+ * (zeroed, [n_pages][page_size][n_kv_heads][head_size]; it returns when the
+ * zeros are there, so any stream may write next). */
 typedef struct yl_kv_pages {
   int32_t dtype; /* yl_dtype */
   int32_t owned; /* 1 if freed by yl_kv_pages_free */

@@ -904,3 +904,23 @@ def test_scores_below_f32(yl, torch_cuda, own_pass, dtype, rows):
             want, wlse, ob, lb = ref.attention(g, q, k, v, 4.0, only=set(range(2 * n, 3 * n)))
             within(out[2 * n :], want[2 * n :], (ob + (want.abs() + ob) * ref.half_step(t))[2 * n :], "out")
             within(lse[2 * n :], wlse[2 * n :], lb[2 * n :], "lse")
+
+
+def test_pages_from_the_library_are_ready(yl, torch_cuda):
+    """The allocation's zeros are there when it returns: none are on their way that another stream's tokens could meet."""
+    side = torch.cuda.Stream()
+    g = ref.Geometry(63, 4, 2, 64, page=64, lens=[5], rows=[5])
+    n = 1 << 17
+    g.table[0, 0] = n - 1
+    batch, qkv = g.device(yl), torch.full((5, 8 * 64), 3.0, device="cuda")
+    ones, out = torch.ones(5, 4, 64, device="cuda"), torch.empty(5, 4, 64, device="cuda")
+    torch.cuda.synchronize()
+    pages = yl.KvPages.alloc(yl.DType.F32, n, 64, 2, 64)  # 4 GiB each of keys and values
+    assert torch.cuda.default_stream().query()
+    with torch.cuda.stream(side):
+        yl.paged_append(qkv, pages, batch, 4)
+        ws = torch.empty(yl.paged_attention_workspace(pages, batch, 4), dtype=torch.uint8, device="cuda")
+        yl.paged_attention(out, ones, pages, batch, 4, 0.125, ws)
+    torch.cuda.synchronize()
+    assert (out == 3.0).all()
+    pages.free()

@@ -106,6 +106,9 @@ int kv_pages_alloc(int dtype, uint32_t n_pages, uint32_t page_size, uint32_t n_k
   if (e == cudaSuccess) e = cudaMalloc(&p.v, bytes);
   if (e == cudaSuccess) e = cudaMemset(p.k, 0, bytes);
   if (e == cudaSuccess) e = cudaMemset(p.v, 0, bytes);
+  // the zeros are there before a caller's stream, which does not wait for the
+  // legacy one, writes tokens
+  if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
   if (e != cudaSuccess) {
     cudaFree(p.k);
     cudaFree(p.v);
