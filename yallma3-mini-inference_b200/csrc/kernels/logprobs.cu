@@ -391,7 +391,7 @@ cudaError_t launch_w(const LogprobArgs& a, cudaStream_t stream) {
   // blocks per row: enough to have one on every SM, while each still reads
   // 4096 values or more
   uint32_t c = 1;
-  while (c < 8 && (uint64_t)a.n_rows * c < 148 && a.vocab / (2 * c) >= 4096) c *= 2;
+  while (c < 8 && (uint64_t)a.n_rows * c < SMS && a.vocab / (2 * c) >= 4096) c *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.n_rows * c);
   cfg.blockDim = dim3(LP_THREADS);

@@ -555,6 +555,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
           }
         }
       } else if (busy) {
+        static_assert(WK > 1 || std::is_same<O, float>::value, "f32 alone has rows that one warp finishes");
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (!live[i]) continue;
@@ -563,11 +564,8 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
             const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
             O* out = static_cast<O*>(a.out) + (uint64_t)row[i] * a.out_stride + (uint64_t)head[i] * HD + 2 * t4;
 #pragma unroll
-            for (int d = 0; d < OB; ++d) {
-              const float x = o[d][2 * i] * inv, y = o[d][2 * i + 1] * inv;
-              if constexpr (sizeof(O) == 4) *reinterpret_cast<float2*>(out + 8 * d) = make_float2(x, y);
-              else *reinterpret_cast<uint32_t*>(out + 8 * d) = pack2<O>(x, y);
-            }
+            for (int d = 0; d < OB; ++d)
+              *reinterpret_cast<float2*>(out + 8 * d) = make_float2(o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
             if (t4 == 0 && a.lse)
               a.lse[(uint64_t)row[i] * a.n_heads + head[i]] =
                   l[i] == 0.0f ? -INFINITY : (m[i] - SHIFT + log2f(l[i])) * LN2;
@@ -595,7 +593,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
 // ---- joining the parts -------------------------------------------------------
 struct JoinArgs {
   PagedAttnArgs a;
-  uint32_t group, n_passes;
+  uint32_t group;
   struct {
     const uint4* cut;
     const uint2* desc;
@@ -751,7 +749,7 @@ uint32_t tile_rows(uint64_t rows, int dtype) {
 // Two blocks per SM; two passes that both leave room for the other get one each
 // and run side by side (12 sequences over 4096 f32 tokens 38.6 us, one after the
 // other 45.0).
-uint32_t blocks_of(uint32_t bm, bool beside) { return bm == TC_TILE || beside ? 148 : 2 * 148; }
+uint32_t blocks_of(uint32_t bm, bool beside) { return bm == TC_TILE || beside ? SMS : 2 * SMS; }
 
 // What a call launches, by its counts alone.
 struct Plan {
@@ -816,7 +814,6 @@ cudaError_t launch(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
   JoinArgs j{};
   j.a = a;
   j.group = a.n_heads / a.pages.n_kv_heads;
-  j.n_passes = pl.shared ? 2 : 1;
   LaunchCfg lc;
   lc.stream = stream;
   for (int i = pl.shared ? 1 : 0; i >= 0; --i) {  // the prefix first

@@ -35,6 +35,7 @@ struct Seqs {
   int* status;
 };
 
+constexpr uint32_t SMS = 148;  // of a B200; grids are cut for it
 constexpr uint32_t NO_PAGE = 0xFFFFFFFFu;
 constexpr int STATUS_RANGE = -6;  // YL_ERR_RANGE
 
