@@ -924,3 +924,34 @@ def test_pages_from_the_library_are_ready(yl, torch_cuda):
     torch.cuda.synchronize()
     assert (out == 3.0).all()
     pages.free()
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("vocab", [40, 1889, 16000, 128256])
+def test_logprobs_with_few_terms_left(yl, torch_cuda, dtype, vocab):
+    """Rows whose probability besides the likeliest token's lies in one to four others, 0.5 to 40 below it: the log
+    probability of that token and the entropy to f32's last bits. A term is off by the exponential (4 half steps of f32,
+    2^-22), the factor's product and its argument's rounding (2), a sum of four (3), log1p (2) and the sums of a thread's
+    own terms next to larger ones (at most |d| e^-d 4, below 2): 13 half steps, and the last subtraction of the entropy,
+    of which W / S is as large as S' at least and has 4 more, two more."""
+    t = DTYPES[dtype]
+    rng = np.random.default_rng(vocab)
+    n = 300
+    x = np.full((n, vocab), -np.inf)
+    at = np.zeros(n, np.int64)
+    for i in range(n):
+        place = rng.permutation(vocab)[:5]
+        at[i] = place[0]
+        x[i, place[0]] = rng.normal() * 3 + 8
+        for p in place[1 : 2 + i % 4]:
+            x[i, p] = x[i, place[0]] - rng.uniform(0.5, 40)
+    x = torch.from_numpy(x).to(t)
+    d = x.double() - x.double().gather(1, torch.from_numpy(at)[:, None])
+    e = d.exp()
+    e[torch.arange(n), torch.from_numpy(at)] = 0.0
+    s, w = e.sum(1), torch.where(e > 0, e * d, 0.0).sum(1)
+    lp, en, ids, _ = run_logprobs(yl, x.cuda(), torch.from_numpy(at.astype(np.int32)).cuda(), 1)
+    likely = s < 0.4  # (from 1/2 on S' is what S = 1 + S' has kept)
+    assert int(likely.sum()) > n // 2 and np.array_equal(ids[:, 0].numpy(), at)
+    within(lp[likely], -s.log1p()[likely], (13 * ref.U32 * s)[likely], "logprobs")
+    within(en[likely], (s.log1p() - w / (1 + s))[likely], (19 * ref.U32 * (s - w))[likely], "entropy")

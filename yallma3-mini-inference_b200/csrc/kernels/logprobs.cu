@@ -3,12 +3,16 @@
 //
 // With m = max x: S = sum of exp(x_i - m) and W = sum of exp(x_i - m) (x_i - m) give
 //   logprob(t) = (x_t - m) - log S,  entropy = log S - W / S.
-// Partial (m, S, W) join as
-//   m1 >= m2, d = m2 - m1:  S = S1 + e^d S2,  W = W1 + e^d (W2 + d S2).
-// S is 1 + S', S' the sum without the largest term, and log S = log1p(S'). Where
-// S' is small (a nearly certain token), S - 1 has lost its digits: the one
-// thread whose sum holds the largest term then has its values summed again
-// without it, so that log probabilities near 0 keep theirs.
+// Parts (m_i, S_i, W_i) of the threads, then of the blocks, join under the
+// largest m: with d = m_i - m, S = sum of e^d S_i, W = sum of e^d (W_i + d S_i).
+// S is 1 + S', S' the sum without the largest term, and log S = log1p(S'). So that
+// log probabilities near 0 keep their digits, the sum of the one thread that has
+// the 1 joins the others' without it, and, where S' is below 1/2, is taken again
+// from that thread's values. What is left beside a likely token are often a few
+// terms far below it. Each of them is the largest its thread has, as a
+// rule, so the factors e^d of the parts are taken with differences and products
+// in two f32 (the rounding of d log2(e) = -40 alone is 2^-19.5), a thread's own
+// terms with one.
 //
 // Most likely tokens: every thread knows the largest of the values it reads.
 // The k-th largest of the threads' maxima bounds the k-th largest value from
@@ -19,8 +23,8 @@
 // the order of atomics.
 //
 // Bound by reading the row (4 bytes and one exponential per value): 1999 rows of
-// 128256 f32 in 186 us on one B200 (5.5 TB/s); 64 rows with 20 alternatives 15 us
-// (from L2; the join and the choice of the largest take about 8), one row 6 us.
+// 128256 f32 in 186 us on one B200 (5.5 TB/s); 64 rows with 20 alternatives 16 us
+// (from L2; the join and the choice of the largest take about 8), one row 6.4 us.
 // A row is read by a thread-block cluster of 1..8 blocks, more for few rows, so
 // that one row of a large vocabulary does not wait for one SM; its parts are
 // joined over distributed shared memory.
@@ -68,22 +72,19 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// m; S = sum of 2^d and W = sum of 2^d d, d = (x - m) log2(e). The difference is
-// taken first: x log2(e) may be beyond f32 where x is a mask of the lowest value.
-struct Part {
-  float m, s, w;
-};
-__device__ __forceinline__ Part join(Part a, Part b) {
-  const float m = fmaxf(a.m, b.m), r = m == -INFINITY ? 0.0f : m;
-  const float da = fmaxf((a.m - r) * LOG2E, FLOOR), db = fmaxf((b.m - r) * LOG2E, FLOOR);
-  const float fa = ex2(da), fb = ex2(db);
-  return {m, fa * a.s + fb * b.s, fa * (a.w + da * a.s) + fb * (b.w + db * b.s)};
-}
-__device__ __forceinline__ Part warp_join(Part p) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    p = join(p, Part{__shfl_xor_sync(FULL, p.m, o), __shfl_xor_sync(FULL, p.s, o), __shfl_xor_sync(FULL, p.w, o)});
-  return p;
+// 2^t, t = (x - m) log2(e), for x <= m; off by 2^-21.5 however large t is. 0, and t
+// = 0, where that is below f32's normal numbers or x is -inf.
+__device__ __forceinline__ float exp_below(float x, float m, float& t) {
+  constexpr float LOG2E_LO = 1.92596299e-8f;  // log2(e) - LOG2E
+  const float d = x - m, z = d - x, d_lo = (x - (d - z)) - (m + z);  // x - m = d + d_lo
+  t = __fmul_rn(d, LOG2E);  // (rounded, whatever it is fused with below)
+  if (!(t >= -126.0f)) {
+    t = 0.0f;
+    return 0.0f;
+  }
+  const float t_lo = fmaf(d_lo, LOG2E, fmaf(d, LOG2E_LO, fmaf(d, LOG2E, -t)));
+  const float n = rintf(t);
+  return ex2((t - n) + t_lo) * __int_as_float(((int)n + 127) << 23);
 }
 // Sorts a warp's 32 keys, largest in lane 0 (bitonic network).
 __device__ __forceinline__ uint64_t warp_sort_desc(uint64_t v, uint32_t lane) {
@@ -154,15 +155,22 @@ struct Row {
   }
 };
 
+// A block's largest value m; S' and W: sums of 2^t and of 2^t t, t = (x - m) log2(e),
+// S' without the largest term. The difference is taken first: x log2(e) may be
+// beyond f32 where x is a mask of the lowest value.
+struct Part {
+  float m, s, w;
+};
+
 struct LpShared {
   uint64_t list[LP_WARPS][32];
   uint64_t cand[LP_CAND];
-  Part part[LP_WARPS];
+  float top_of[LP_WARPS];  // the warps' largest values
+  float s[LP_WARPS], w[LP_WARPS];  // theirs, the largest term of all left out
   uint32_t group[LP_MAX_TOP];
   uint64_t red[LP_WARPS];
   uint32_t n_group, n_cand;
-  Part whole;
-  float rest[LP_WARPS], whole_rest;
+  Part whole, own;  // own: of the thread that has m, the largest term in it
   uint32_t owner;
   uint64_t top[32];  // this block's largest keys, in order
 };
@@ -251,8 +259,25 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(LogprobArgs a) 
   // a NaN left its mark in the sum alone
   const bool nan = isnan(r.s);
   if (nan) r.m = INFINITY;
-  const Part p = warp_join(Part{r.m, r.s, r.w});
-  if (lane == 0) sh.part[warp] = p;
+  const float wm = warp_max(r.m);
+  if (lane == 0) sh.top_of[warp] = wm;
+  __syncthreads();
+  float bm = sh.top_of[0];  // the block's, and the first warp that has it
+  uint32_t first = 0;
+#pragma unroll
+  for (uint32_t i = 1; i < LP_WARPS; ++i)
+    if (sh.top_of[i] > bm) bm = sh.top_of[i], first = i;
+  {
+    float t, s = exp_below(r.m, bm, t), w = s * (r.w + t * r.s);
+    s *= r.s;
+    if (warp == first) {  // the first thread that has it keeps its sum apart
+      const uint32_t owner = __ffs(__ballot_sync(FULL, r.m == bm)) - 1;
+      if (lane == owner) sh.owner = tid, sh.own = {bm, s, w}, s = w = 0.0f;
+    }
+    s = warp_sum(s);
+    if (W) w = warp_sum(w);
+    if (lane == 0) sh.s[warp] = s, sh.w[warp] = w;
+  }
 
   if (a.top_k) {
     // where the thread's largest value lies: the first of its batch that equals it
@@ -323,63 +348,51 @@ __global__ void __launch_bounds__(LP_THREADS, 4) logprobs_kernel(LogprobArgs a) 
   }
   __syncthreads();
   if (warp == 0) {
-    const Part q = warp_join(lane < LP_WARPS ? sh.part[lane] : Part{-INFINITY, 0.0f, 0.0f});
-    if (lane == 0) sh.whole = q;
+    float s = lane < LP_WARPS ? sh.s[lane] : 0.0f, w = W && lane < LP_WARPS ? sh.w[lane] : 0.0f;
+    const float rest = sh.own.s - 1.0f;
+    if (bm > -INFINITY && warp_sum(s) + rest < 0.5f) {
+      part.each(sh.owner, lane, [&](float v, uint32_t) {  // (equals of m are not here: S' were 1 or more)
+        float t;
+        const float e = exp_below(v, bm, t);
+        if (v != bm) s += e, w = fmaf(e, t, w);
+      });
+    } else if (lane == 0) {
+      s += rest, w += sh.own.w;
+    }
+    s = warp_sum(s);
+    if (W) w = warp_sum(w);
+    if (lane == 0) sh.whole = {bm, s, w};
   }
-  // ---- join the cluster's blocks: every block has the row's (m, S, W) ----
+  // ---- join the cluster's blocks: every block's first warp has the row's (m, S', W) ----
   if (C > 1) cluster.sync();
   else __syncthreads();
-  Part q = {-INFINITY, 0.0f, 0.0f};
-  if (lane < C) q = C > 1 ? cluster.map_shared_rank(&sh, lane)->whole : sh.whole;
-  q = warp_join(q);
-  // Lanes join in different orders and may end a last bit apart (a product and a
-  // sum are fused in one order and not in the other). Barriers depend on the
-  // value below: every thread of the row's blocks takes what lane 0 has.
-  q = {__shfl_sync(FULL, q.m, 0), __shfl_sync(FULL, q.s, 0), __shfl_sync(FULL, q.w, 0)};
-  // NaN, +inf, or nothing above -inf: no distribution
-  const bool none = isnan(q.s) || fabsf(q.m) == INFINITY;
-  float rest = q.s - 1.0f;  // S'
-  if (!none && rest < 0.0078125f) {
-    // Nearly certain: 2^-24 of 1 is more than 2^-17 of S'. One thread of the
-    // row has the 1 in its sum; a warp sums its values again without it, the
-    // other threads' sums are as good as they were.
-    if (tid == 0) sh.owner = 0xFFFFFFFFu;
-    __syncthreads();
-    if (r.m == q.m) sh.owner = tid;
-    float s = r.m == q.m ? 0.0f : r.s * ex2(fmaxf((r.m - q.m) * LOG2E, FLOOR));
-    __syncthreads();
-    if (warp == 0 && sh.owner != 0xFFFFFFFFu)
-      part.each(sh.owner, lane, [&](float v, uint32_t) { s += v == q.m ? 0.0f : ex2((v - q.m) * LOG2E); });
-    s = warp_sum(s);
-    if (lane == 0) sh.rest[warp] = s;
-    __syncthreads();
-    if (tid == 0) {
-      float t = 0.0f;
-      for (uint32_t w = 0; w < LP_WARPS; ++w) t += sh.rest[w];
-      sh.whole_rest = t;
-    }
-    if (C > 1) cluster.sync();
-    else __syncthreads();
-    rest = 0.0f;
-    if (lane < C) rest = C > 1 ? cluster.map_shared_rank(&sh, lane)->whole_rest : sh.whole_rest;
-    rest = warp_sum(rest);
-  }
   if (rank == 0) {
     if (a.top_k) {
       if (warp < C) sh.list[warp][lane] = C > 1 ? cluster.map_shared_rank(&sh, warp)->top[lane] : sh.top[lane];
       join_lists(sh.list, C, warp, lane);
     }
     if (warp == 0) {
+      Part q = {-INFINITY, 0.0f, 0.0f};
+      if (lane < C) q = C > 1 ? cluster.map_shared_rank(&sh, lane)->whole : sh.whole;
+      const float m = warp_max(q.m);
+      // the blocks' largest terms but one count; the first of equals stays apart
+      const bool owner = (int)lane == __ffs(__ballot_sync(FULL, q.m == m)) - 1;
+      float t, f = exp_below(q.m, m, t);
+      if (owner) f = 1.0f, t = 0.0f;
+      const float one = owner ? 0.0f : 1.0f;
+      const float rest = warp_sum(f * (one + q.s)), w = W ? warp_sum(f * (q.w + t * (one + q.s))) : 0.0f;
+      // NaN, +inf, or nothing above -inf: no distribution
+      const bool none = isnan(rest) || fabsf(m) == INFINITY;
       const float nanf_ = __int_as_float(0x7FC00000);
       const float log_sum = log1pf(rest);
       if (lane == 0) {
-        if (a.tokens) a.logprobs[row] = none || token < 0 ? nanf_ : (xt - q.m) - log_sum;
-        if (W) a.entropy[row] = none ? nanf_ : log_sum - q.w * LN2 / (1.0f + rest);
+        if (a.tokens) a.logprobs[row] = none || token < 0 ? nanf_ : (xt - m) - log_sum;
+        if (W) a.entropy[row] = none ? nanf_ : log_sum - w * LN2 / (1.0f + rest);
       }
       if (lane < a.top_k) {
         const uint64_t key = sh.list[0][lane];
         a.top_ids[(uint64_t)row * a.top_k + lane] = none ? -1 : (int32_t)key_index(key);
-        a.top_logprobs[(uint64_t)row * a.top_k + lane] = none ? nanf_ : (key_value(key) - q.m) - log_sum;
+        a.top_logprobs[(uint64_t)row * a.top_k + lane] = none ? nanf_ : (key_value(key) - m) - log_sum;
       }
     }
   }
