@@ -572,11 +572,14 @@ int yl_paged_append(void* q_out, uint64_t q_stride, const float* qkv, uint64_t q
  * Contents of the cache behind a sequence's last position do not matter,
  * infinities and NaN included. A value that is not finite reaches all rows
  * that see it, and may reach rows of the same chunk before it (their weight
- * for it is 0, and 0 times infinity is NaN); in an f32 cache an infinite key
- * or value gives NaN. Scores are held in powers of two (score x attn_scale
- * x log2 e): one above f32's range gives its row NaN, one below it weighs 0,
- * and a row that sees none but such gets NaN too. The summation order depends
- * on the batch's geometry alone: the same call gives the same bits.
+ * for it is 0, and 0 times infinity is NaN); in an f32 cache an infinite query,
+ * key or value gives NaN, and one within 2^-12 of the largest f32 counts as
+ * infinite. Values are summed in f32, times weights of up to 2^8, before they
+ * are divided by the weights' sum: those that add up to 2^120 or more may
+ * overflow. Scores are held in powers of two (score x attn_scale x log2 e): one
+ * above f32's range gives its row NaN, one below it weighs 0, and a row that
+ * sees none but such gets NaN too. The summation order depends on the batch's
+ * geometry alone: the same call gives the same bits.
  * workspace: device memory of at least the bytes yl_paged_attention_workspace
  * gives for a batch of these counts (n_seqs, n_rows, shared_len) and heads,
  * 256-byte aligned, with any contents; not to be shared by calls that may

@@ -35,13 +35,13 @@
 // fall below f16's range.
 //
 // Measured on one B200, 32 query and 8 key heads of 128, bf16: 16 sequences of 17
-// to 8000 tokens 51 us (268 MB, 5.2 TB/s; bound by HBM and the items' ends), one
+// to 8000 tokens 52 us (268 MB, 5.2 TB/s; bound by HBM and the items' ends), one
 // of 100000 tokens 72 us (5.7 TB/s); one token of 9 / 3 heads of 64, f32, 301 keys
 // 9 us (two launches, four dependent trips to memory each); a prompt of 2000
-// tokens of 32 / 8 heads of 64, f32, 428 us, of which its 3 x 8 million tf32 MMAs
+// tokens of 32 / 8 heads of 64, f32, 433 us, of which its 3 x 8 million tf32 MMAs
 // (8.2 cycles each per scheduler) would take 190: two warps per scheduler at 168
 // registers wait for one another's chains. More warps with fewer registers spill:
-// 440 us with three blocks per SM, 515 with eight warps per block.
+// 3 % longer with three blocks per SM, 20 % with eight warps per block.
 #include <cmath>
 
 #include "paged_attention.cuh"
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
               for (int ks = 0; ks < HD / 16; ++ks) {  // 16 elements: two k-steps of 8
                 uint32_t ah[2][4], al[2][4];
                 // (split again for every tile: kept split, in shared memory, the loads
-                // cost more than the arithmetic, 455 us and not 428 as below)
+                // cost more than the arithmetic, 6 % of the time below)
                 const float* q0 = qs + (wm * 16 + g) * S::QP + 16 * ks + t4;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(Shape<T, HD, WM, WK>::THREADS, 2)
             __syncwarp();
           }
           if constexpr (S::F32) {
-            constexpr int JP = NB < 2 ? 1 : 2;  // 16 keys in a chain (2000 tokens of 32 / 8 heads of 64: 428 us; of 8 keys 470, of 32 no less)
+            constexpr int JP = NB < 2 ? 1 : 2;  // 16 keys in a chain (2000 tokens of 32 / 8 heads of 64: 433 us; of 8 keys 10 % longer, of 32 no less)
 #pragma unroll
             for (int j = 0; j < NB; j += JP) {
               // keys 2i of the eight are the MMA's k = i, keys 2i+1 its k = 4+i: the weights are where QK left them
@@ -740,15 +740,16 @@ __global__ void __launch_bounds__(128) join_rows_kernel(JoinArgs j) {
 // Row tile for items of `rows` rows. Decoding pads to 16 rows. 12, 16 and 32
 // sequences of 4 query heads per key head over 8192 shared tokens (48, 64 and 128
 // rows) took 32.9, 36.9 and 39.7 us on tcgen05 and 37.0, 39.6 and 39.7 us in
-// 64-row tiles on mma.sync; 8 of them (32 rows) 27.7 us on mma.sync and 30.5 on
-// tcgen05. f32 has no tcgen05 form.
+// 64-row tiles on mma.sync, which are no longer built for 16 bits; 8 of them (32
+// rows) 26.7 us on mma.sync and 31.0 on tcgen05, 64 sequences of 6 rows each (24)
+// 54 and 64. f32 has no tcgen05 form.
 uint32_t tile_rows(uint64_t rows, int dtype) {
   if (dtype != DT_F32 && rows > 32) return TC_TILE;
   return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 // Two blocks per SM; two passes that both leave room for the other get one each
-// and run side by side (12 sequences over 4096 f32 tokens 38.6 us, one after the
-// other 45.0).
+// and run side by side (12 sequences over 4096 f32 tokens 15 % faster than one
+// after the other).
 uint32_t blocks_of(uint32_t bm, bool beside) { return bm == TC_TILE || beside ? SMS : 2 * SMS; }
 
 // What a call launches, by its counts alone.
@@ -768,11 +769,11 @@ Plan plan_of(const Pages& p, const Seqs& s, int dtype, uint32_t n_heads, int sha
   // A pass over the prefix for all sequences saves reading it n_seqs - 1 times
   // (from L2, as a rule) and costs its launch and the joining of every row.
   // Measured, us with and without it (8 key heads of 128, bf16, own keys 100..300):
-  //   side by side:  4 x 1024 tokens 12.7 / 12.6,  8 x 1024 16.1 / 15.2,  8 x 2048 17.3 / 18.4,  4 x 16384 29 / 43
-  //   on tcgen05:    16 x 1024 23.6 / 19.1,  16 x 2048 25.5 / 26.9,  64 x 512 39 / 36,  64 x 1024 41 / 50
-  //   f32, head 64:  4 x 1024 12.7 / 14.1,  12 x 1024 20 / 22,  12 x 4096 35 / 55
+  //   side by side:  4 x 1024 tokens 12.9 / 11.7,  8 x 1024 16.6 / 14.3,  8 x 2048 16.9 / 18.5,  4 x 16384 28 / 42
+  //   on tcgen05:    16 x 1024 24.0 / 19.3,  16 x 2048 25.9 / 27.0,  64 x 512 41 / 36,  64 x 1024 42 / 51
+  //   f32, head 64:  4 x 1024 12.1 / 14.3,  12 x 1024 20 / 22,  12 x 4096 35 / 56
   // Rows of a prompt share what they read by themselves: 16 sequences of 16 tokens
-  // (64 rows each) behind 4096 62 / 76, of 32 tokens 91 / 80.
+  // (64 rows each) behind 4096 63 / 77, of 32 tokens 93 / 81.
   const double saved = (s.n_seqs - 1.0) * s.shared_len * p.n_kv_heads * hd * (dtype == DT_F32 ? 8 : 4);
   const double worth = dtype == DT_F32 ? 8 << 20 : pl.beside ? 40 << 20 : 128 << 20;
   pl.shared = s.shared_len && s.n_seqs > 1 && each <= 64 && (share < 0 ? saved >= worth : share > 0);
@@ -829,13 +830,14 @@ cudaError_t launch(const PagedAttnArgs& a, int dtype, cudaStream_t stream) {
     p.from = pl.shared && !i ? a.seqs.shared_len : 0;
     p.group = j.group;
     // A piece is at least so long: an f32 tile takes as long as joining its part
-    // (one token against 301: pieces of 1 8.9 us, of 2 10.1); 16-bit ones less (8
-    // sequences behind 2048 tokens: 24.5 us with pieces of 1, 17.2 with 2).
+    // (one token against 301: pieces of 1 9.0 us, of 2 10.1); a 16-bit one of 2 is as
+    // fast as of 1 and makes fewer parts (one token against 301 9.1 / 8.9, 8 sequences
+    // behind 2048 16.9 / 17.0; of 3 9.9, 18.0).
     p.min_chunk = dtype == DT_F32 ? 1 : 2;
-    // 16-bit items cost as much as two tiles more (with 1 / 2 / 3: 64 sequences of up
-    // to 1000 tokens 41.0 / 33.3 / 33.5 us, of 6 rows each 66 / 52 / 48, an 8191-token
-    // prompt on tcgen05 579 / 544 / 551, without any 722); an f32 tile takes as long as
-    // an item's ends (a 900-token prompt of 9 / 3 heads 77 / 78 / 91).
+    // 16-bit items cost as much as two tiles more (with 0 / 1 / 2 / 3: 64 sequences of
+    // up to 1000 tokens 51 / 42.5 / 34.2 / 33.8 us, of 6 rows each 85 / 69 / 54 / 51, an
+    // 8191-token prompt on tcgen05 616 / 566 / 529 / 526); an f32 tile takes as long as
+    // an item's ends (a 900-token prompt of 9 / 3 heads 58 / 42 / 48 / 48).
     p.item_cost = dtype == DT_F32 ? 1 : 2;
     p.joined = pl.shared;
     p.cut = reinterpret_cast<uint4*>(ws + pl.cut[i]);

@@ -10,8 +10,9 @@
 // memory, V from shared memory ([key][element], so its descriptor is that of an
 // operand whose rows run along the columns of the product). The two row tiles
 // take turns: while one's softmax runs, the tensor cores multiply for the
-// other. All MMAs are issued by one thread and run in its order, so the next
-// S may be issued right behind the product that reads P from the same columns.
+// other. A row tile's MMAs are all issued by one thread and run in its order, so
+// its next S may be issued right behind the product that reads P from the same
+// columns.
 //
 // O stays in tensor memory. It is rescaled only when a row's maximum has grown
 // by more than 2^8 since the last time: until then P is taken relative to the
@@ -25,8 +26,8 @@
 // hold only a few in advance), 9 loads Q (a box of group heads x tokens), and keys
 // and values page by page, 11 only hands its registers to the softmax warps, for
 // which a row of S is 128 registers. (Two threads per row, 16 softmax warps of 96
-// registers, take 592 us for a prompt of 8191 tokens and not 528: they spill, and
-// pairs have to agree on every tile's maximum.)
+// registers, took 12 % longer for a prompt of 8191 tokens, now 529 us: they spill,
+// and pairs have to agree on every tile's maximum.)
 #include "paged_attention.cuh"
 
 namespace yl {
@@ -363,7 +364,7 @@ __global__ void __launch_bounds__(384, 1)
         if (mine && !wait(&p_full[x], p_phase)) break;
         // The row tiles' MMAs alternate, each tile's at one go: mixed, both
         // tiles' S would be there at the same time, both softmaxes would run
-        // together, and the tensor cores would wait for both (565 us at 8191 rows, not 513).
+        // together, and the tensor cores would wait for both (10 % longer at 8191 rows).
         if ((x == 1 || turns > 0) && !wait(&turn[x], (turns - 1 + x) & 1)) break;
         ++turns;
         if (mine) {
