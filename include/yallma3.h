@@ -606,7 +606,8 @@ int yl_token_logprobs(const void* logits, int dtype, uint64_t row_stride, uint32
                       float* top_logprobs, void* stream);
 /* Device views that the calls above take: the model's (cos, sin) table
  * [*len][head_size/2][2] in the order of its rope_mode, and the batch's logits
- * [max_sessions][vocab] after yl_batch_forward. */
+ * [max_sessions][vocab] after yl_batch_forward. The next forward, on a stream
+ * of the library's own, writes over logits: calls that read them end before. */
 int yl_model_rope(const yl_model* m, const float** rope_cs, uint32_t* len);
 int yl_batch_logits(const yl_batch* b, float** logits);
 

@@ -653,7 +653,8 @@ class SessionBatch:
         return ids, logits
 
     def logits(self) -> int:
-        """Device address of the batch's logits rows [max_sessions, vocab] after forward()."""
+        """Device address of the batch's logits rows [max_sessions, vocab] after forward(); the next forward() writes
+        over them, so calls that read them have to end before."""
         p = _P()
         _check(_lib.yl_batch_logits(self._h, C.byref(p)))
         return p.value
